@@ -1,0 +1,181 @@
+/*
+ * larynx_kv.h -- C ABI of the paged key/value cache held in 4 bits (sm_100a).
+ *
+ * Stands beside lx_flow_op_attention (larynx_flow.h), which takes dense keys
+ * and values: these entry points keep the keys and values of many sequences in
+ * pages of 4-bit codes, attend to them for one or many new rows a sequence,
+ * and share, copy, free and compact the pages.  With the block-causal chunk
+ * mask a frame's keys and values do not change once its chunk is complete, so
+ * a streaming caller keeps them instead of recomputing them; the single-token
+ * form with grouped query heads serves the autoregressive stage in front of
+ * the Flow decoder.  No counterpart in the reference, which keeps no keys or
+ * values between calls (src/flow/flow.cpp:110-308) and leaves the cache of its
+ * token stage to ggml.
+ *
+ * Like the other per-op entry points these work on the caller's buffers.  All
+ * calls but lx_kv_status are asynchronous on `stream` (a cudaStream_t, NULL =
+ * the default stream of cache->device), allocate nothing, keep nothing between
+ * calls and can be captured into CUDA graphs.  Calls on one cache that change
+ * it, or that read what another one changes, have to be ordered by the caller
+ * (one stream, or events); calls that only read a cache (lx_kv_read,
+ * lx_kv_attention) may overlap.  The calls run on cache->device, whichever
+ * device is current, and leave the current device as it was.
+ *
+ * Status: LX_OK, LX_ERR_ARG (nothing was enqueued), LX_ERR_CUDA.  What only
+ * the device can see (a full pool, a bad slot) is recorded in the sticky bits
+ * of *cache->error and never reads or writes out of bounds; lx_kv_status
+ * returns them.
+ */
+#ifndef LARYNX_KV_H
+#define LARYNX_KV_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "larynx_flow.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Element types of rows. */
+#define LX_KV_BF16 0
+#define LX_KV_FP16 1
+#define LX_KV_FP32 2 /* lx_kv_write, lx_kv_read */
+
+/* Bits of *cache->error. */
+#define LX_KV_FULL 1  /* not enough free pages: the entry was not served      */
+#define LX_KV_SLOT 2  /* slot out of range, named twice, or not empty          */
+#define LX_KV_WIDTH 4 /* the sequence would need more than max_pages pages     */
+#define LX_KV_PAGE 8  /* a table holds a page id outside [0, n_pages)          */
+#define LX_KV_ROWS 16 /* row offsets out of range, or rows outside a sequence  */
+
+/* The start that lx_kv_extend gives an entry it did not serve. */
+#define LX_KV_REFUSED INT32_MIN
+
+/* Most entries of one call of lx_kv_extend, lx_kv_fork, lx_kv_copy, lx_kv_free. */
+#define LX_KV_MAX_BATCH 4096
+
+/* A cache: geometry and device buffers, all owned by the caller.
+ *
+ * pool: [n_layers][n_pages][kv_heads][page / 16] blocks, 16-byte aligned.  A
+ * block holds 16 tokens of one head: K codes (512 bytes for every 64
+ * channels), V codes (the same), K parameters, V parameters (64 bytes for
+ * every group each).  head_dim is 64 or 128; a group is 32 or 64 channels.
+ *
+ * A group of a token is held as codes c = rint((x - m) / s), 0 <= c <= 15, with
+ * m = min(x) rounded down to bf16 and s = (max(x) - m) / 15 rounded up to bf16
+ * (at least 2^-126), and stands for c s + m.  The rounding is that of exact
+ * arithmetic, ties to even.  A group with a NaN or an infinity, or whose range
+ * does not fit fp32, is held as s = m = NaN and reads as NaN.
+ *
+ * Within a block (t the token, d the channel, h = d / 64, w = d % 64 / 32):
+ *   K code (t, d): e = d % 8, 32-bit word at 512 h + 16 (4 (t % 8) + d % 32 / 8) + 8 (t / 8) + 4 w,
+ *                  bits 4 (e / 2) + 16 (e % 2) and up;
+ *   V code (t, d): 16-bit word at 512 (head_dim / 64) + 512 h + 16 (4 (d % 32 / 4) + t % 8 / 2)
+ *                  + 8 (t / 8) + 4 w + 2 (t % 2), bits 4 (d % 4) and up;
+ *   K parameters (t, group g): bf16 s, bf16 m at 1024 (head_dim / 64) + 64 g
+ *                  + 4 (4 (t % 8 / 2) + 2 (t / 8) + t % 2); V's 64 (head_dim / group) bytes further.
+ * (The order in which the matrix instructions of lx_kv_attention take them.)
+ *
+ * table: [n_seq][max_pages] page ids of each sequence slot, -1 past its last
+ * page; lengths: [n_seq] tokens; refs: [n_pages] how many table entries hold
+ * each page (0 = free); scratch: lx_kv_scratch_ints() ints, no initial value;
+ * error: one int of sticky bits. */
+typedef struct lx_kv_cache {
+  int32_t device;
+  int32_t n_layers, n_pages, n_seq, max_pages;
+  int32_t kv_heads;
+  int32_t head_dim; /* 64 or 128            */
+  int32_t group;    /* 32 or 64             */
+  int32_t page;     /* 16, 32, 64 or 128    */
+  void* pool;
+  int32_t* table;
+  int32_t* lengths;
+  int32_t* refs;
+  int32_t* scratch;
+  int32_t* error;
+} lx_kv_cache;
+
+/* The rows of a batch: entry i has rows row0[i] .. row0[i + 1] - 1 of the
+ * caller's packed arrays, for positions start[i] + 0, 1, ... of slot seqs[i].
+ * Device arrays; `total` counts all packed rows and max_rows is at least the
+ * most rows of one entry (rows past either are not touched). */
+typedef struct lx_kv_rows {
+  int32_t n, total, max_rows;
+  const int32_t* seqs;  /* [n], or NULL: slots 0 .. n - 1                         */
+  const int32_t* row0;  /* [n + 1], or NULL: max_rows rows each, total = n max_rows */
+  const int32_t* start; /* [n], or NULL: the last rows of each sequence (negative
+                           where there are more rows than tokens)               */
+} lx_kv_rows;
+
+/* Bytes of the pool; 0 when the geometry is not valid. */
+size_t lx_kv_pool_bytes(const lx_kv_cache* c);
+/* Ints of scratch; 0 when the geometry is not valid. */
+size_t lx_kv_scratch_ints(const lx_kv_cache* c);
+
+/* Empties the cache: lengths 0, tables -1, refs 0, error 0 (pool untouched). */
+int lx_kv_reset(const lx_kv_cache* c, void* stream);
+
+/* Waits for the stream, returns the error bits in *bits and clears them. */
+int lx_kv_status(const lx_kv_cache* c, int32_t* bits, void* stream);
+
+/* Grows sequence seqs[i] by counts[i] tokens (device arrays): start[i] gets
+ * its old length.  New pages are the free ones of lowest id, given out in the
+ * order of the batch; a last page that is not full and shared with another
+ * sequence is replaced by a copy first (all layers), so that lx_kv_write never
+ * changes a fork.  Entry i is served if the pages needed by entries 0 .. i fit the free ones; an entry that
+ * is not served gets start[i] = LX_KV_REFUSED (its rows are skipped by the
+ * other calls) and leaves its sequence as it was. */
+int lx_kv_extend(const lx_kv_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, int32_t* start,
+                 void* stream);
+
+/* Quantises rows k, v ([total][kv_heads][head_dim], element strides k_row,
+ * k_head, v_row, v_head; channels contiguous) into one layer.  Rows outside
+ * their sequence or on a page held by two sequences are skipped (LX_KV_ROWS);
+ * two rows for one position: one of them wins. */
+int lx_kv_write(const lx_kv_cache* c, int32_t layer, const lx_kv_rows* rows, int32_t dtype, const void* k,
+                int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* stream);
+
+/* The values of rows in one layer, in the layout of lx_kv_write.  Rows outside
+ * their sequence, or of refused entries, read as 0. */
+int lx_kv_read(const lx_kv_cache* c, int32_t layer, const lx_kv_rows* rows, int32_t dtype, void* k, int64_t k_row,
+               int64_t k_head, void* v, int64_t v_row, int64_t v_head, void* stream);
+
+/* out = softmax(scale q k^T + mask) v over the cache, per query head h with
+ * kv head h / (q_heads / kv_heads).  q, out: [total][q_heads][head_dim] (element
+ * strides; channels contiguous), bf16 or fp16; lse: [total][q_heads] fp32 log of
+ * the sum of exponentials (natural), contiguous, or NULL.
+ * A row at position p sees keys [lo, hi):
+ *   chunk == 0: [0, length);
+ *   chunk  > 0: hi = min(length, (floor(p / chunk) + 1) chunk), and with
+ *   left >= 0   lo = max(0, floor(p / chunk) chunk - left), else lo = 0
+ * (chunk 1 is causal; left < 0 looks back without limit).  A row that sees
+ * nothing gets zeros and lse = -inf; so do the rows of refused entries.  Keys on a page that is not in the pool are not seen (LX_KV_PAGE).
+ * max_len: an upper bound of the lengths, which only steers how the work is
+ * split; 0 = max_pages * page.  The result does not depend on other entries. */
+int lx_kv_attention(const lx_kv_cache* c, int32_t layer, const lx_kv_rows* rows, int32_t q_heads, int32_t dtype,
+                    const void* q, int64_t q_row, int64_t q_head, void* out, int64_t o_row, int64_t o_head,
+                    float* lse, float scale, int32_t chunk, int32_t left, int32_t max_len, void* stream);
+
+/* dst[i] shares every page of src[i].  dst[i] has to be empty, and named once. */
+int lx_kv_fork(const lx_kv_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream);
+
+/* dst[i] becomes a copy of src[i] on fresh pages (as lx_kv_extend gives them;
+ * all layers).  dst[i] has to be empty, and named once. */
+int lx_kv_copy(const lx_kv_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream);
+
+/* Cuts sequence seqs[i] to its first keep[i] tokens (0 frees it; the least
+ * keep of a slot named twice counts; one that is longer changes nothing). */
+int lx_kv_free(const lx_kv_cache* c, int32_t n, const int32_t* seqs, const int32_t* keep, void* stream);
+
+/* Makes the used pages 0 .. U - 1: the used pages of id >= U move to the free
+ * ids below U, both in ascending order, with all layers and tables.  *used
+ * (device) gets U. */
+int lx_kv_compact(const lx_kv_cache* c, int32_t* used, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* LARYNX_KV_H */

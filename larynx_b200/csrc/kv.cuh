@@ -1,0 +1,134 @@
+// Shared pieces of the paged 4-bit key/value cache (include/larynx_kv.h): the
+// geometry of a block, device-side reading of a batch, argument checks and
+// launches.
+//
+// Every index that comes from device memory (slots, page ids, row offsets,
+// lengths) is checked before it is used; what does not hold sets a bit of the
+// cache's error word and the work is skipped.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/larynx_kv.h"
+#include "kernels.h"
+
+namespace lx {
+namespace kv {
+
+constexpr int BLOCK = 16;  // tokens of a block: the key side of one m16n8k16 product with P
+
+constexpr int MAX_TOKENS = 1 << 30;  // of a sequence's table
+constexpr int MAX_ROWS = 1 << 28;    // packed rows of a call
+
+__host__ __device__ constexpr int block_bytes(int dim, int group) { return dim / 64 * 1024 + 128 * (dim / group); }
+__host__ __device__ constexpr int param_offset(int dim) { return dim / 64 * 1024; }
+// Slot of token t (0..15) among a group's 16 parameters: the four tokens that
+// a lane of the score tile holds, t = 2 j + {0, 1, 8, 9}, are neighbours.
+__host__ __device__ constexpr int param_slot(int t) { return t % 8 / 2 * 4 + t / 8 * 2 + t % 2; }
+
+// First byte of block b (tokens 16 b ..) of `page` for one head of one layer.
+__device__ __forceinline__ size_t block_at(const lx_kv_cache& c, int layer, int page, int head, int in_page) {
+  const size_t heads = (static_cast<size_t>(layer) * c.n_pages + page) * c.kv_heads + head;
+  return (heads * (c.page / BLOCK) + in_page) * block_bytes(c.head_dim, c.group);
+}
+
+__device__ __forceinline__ void flag(const lx_kv_cache& c, int bit) { atomicOr(c.error, bit); }
+
+// Length of a slot, clamped to what its table can hold.
+__device__ __forceinline__ int length_of(const lx_kv_cache& c, int slot) {
+  const int len = c.lengths[slot], most = c.max_pages * c.page;
+  return len < 0 ? 0 : len > most ? most : len;
+}
+
+__device__ __forceinline__ int pages_of(const lx_kv_cache& c, int tokens) { return (tokens + c.page - 1) / c.page; }
+
+// Entry i of a batch: its slot (-1: out of range), first packed row, rows.
+struct Entry {
+  int slot, row0, rows;
+};
+__device__ __forceinline__ Entry entry_of(const lx_kv_cache& c, const lx_kv_rows& r, int i) {
+  Entry e;
+  e.slot = r.seqs ? r.seqs[i] : i;
+  if (e.slot < 0 || e.slot >= c.n_seq) {
+    e.slot = -1;
+    flag(c, LX_KV_SLOT);
+  }
+  long long first = r.row0 ? r.row0[i] : static_cast<long long>(i) * r.max_rows;
+  long long end = r.row0 ? r.row0[i + 1] : first + r.max_rows;
+  if (first < 0 || end < first || end > r.total || end - first > r.max_rows) {
+    flag(c, LX_KV_ROWS);
+    first = first < 0 ? 0 : first;
+    end = end > r.total ? r.total : end;
+    end = end - first > r.max_rows ? first + r.max_rows : end;
+  }
+  e.row0 = static_cast<int>(first);
+  e.rows = end > first ? static_cast<int>(end - first) : 0;
+  return e;
+}
+
+// Position of the first row of entry i, or LX_KV_REFUSED.  (Clamped so that sums
+// with row counts stay in 32 bits; no sequence reaches that far.)
+__device__ __forceinline__ int start_of(const lx_kv_rows& r, int i, int len, int rows) {
+  const int s = r.start ? r.start[i] : len - rows;
+  return s == LX_KV_REFUSED ? s : min(max(s, -MAX_ROWS), MAX_TOKENS);
+}
+
+// ---- host side ---------------------------------------------------------------
+inline bool geometry_ok(const lx_kv_cache* c) {
+  if (!c || c->n_layers <= 0 || c->n_pages <= 0 || c->n_seq <= 0 || c->max_pages <= 0 || c->kv_heads <= 0) return false;
+  if (c->head_dim != 64 && c->head_dim != 128) return false;
+  if (c->group != 32 && c->group != 64) return false;
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return false;
+  // positions and page counts are 32-bit
+  return c->max_pages <= MAX_TOKENS / c->page && c->n_pages <= 0x10000000 && c->kv_heads <= 65535;
+}
+
+inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+inline bool cache_ok(const lx_kv_cache* c) {
+  return geometry_ok(c) && c->device >= 0 && c->pool && aligned(c->pool, 16) && c->table && c->lengths && c->refs &&
+         c->scratch && c->error && aligned(c->table, 4) && aligned(c->lengths, 4) && aligned(c->refs, 4) &&
+         aligned(c->scratch, 4) && aligned(c->error, 4);
+}
+
+inline bool rows_ok(const lx_kv_rows* r) {
+  if (!r || r->n <= 0 || r->total < 0 || r->max_rows < 0 || r->total > MAX_ROWS || r->max_rows > MAX_ROWS)
+    return false;
+  return r->row0 || static_cast<long long>(r->n) * r->max_rows == r->total;
+}
+
+// Makes the cache's device current for the scope of a call.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    ok_ = cudaGetDevice(&before_) == cudaSuccess;
+    if (ok_ && before_ != device) {
+      ok_ = cudaSetDevice(device) == cudaSuccess;
+      changed_ = ok_;
+    }
+  }
+  ~OnDevice() {
+    if (changed_) cudaSetDevice(before_);
+  }
+  bool ok() const { return ok_; }
+
+ private:
+  int before_ = 0;
+  bool ok_ = false, changed_ = false;
+};
+
+// A plain launch with its own status (not the thread's last error, which may
+// be another call's).
+template <typename... KArgs, typename... Args>
+inline bool launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) == cudaSuccess;
+}
+
+}  // namespace kv
+}  // namespace lx

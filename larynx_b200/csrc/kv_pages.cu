@@ -1,0 +1,490 @@
+// Pages of the 4-bit cache: reserving, sharing, copying, freeing, compacting.
+//
+// The state (tables, lengths, reference counts) lives on the device and every
+// call works on it in stream order, without the host knowing it.  A call is a
+// planning kernel, which decides in one block which page goes where, and for
+// calls that move data a copy kernel over the whole GPU that takes its list of
+// pages from the cache's scratch.
+#include <climits>
+
+#include "kv.cuh"
+
+namespace lx {
+namespace kv {
+namespace {
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int TILE = 4 * PLAN_THREADS;  // pages that the planning block takes at once
+
+// scratch: header, then three lists of n_pages
+constexpr int HEAD = 16;
+constexpr int MOVES = 0, USED = 1;  // words of the header
+__device__ __forceinline__ int* src_list(const lx_kv_cache& c) { return c.scratch + HEAD; }
+__device__ __forceinline__ int* dst_list(const lx_kv_cache& c) { return c.scratch + HEAD + c.n_pages; }
+__device__ __forceinline__ int* place_list(const lx_kv_cache& c) { return c.scratch + HEAD + 2 * c.n_pages; }
+
+__device__ __forceinline__ bool page_ok(const lx_kv_cache& c, int page) { return page >= 0 && page < c.n_pages; }
+
+__device__ __forceinline__ int32_t* row_of(const lx_kv_cache& c, int slot) {
+  return c.table + static_cast<size_t>(slot) * c.max_pages;
+}
+
+// Exclusive sum over the block of x, and the block's total.
+__device__ __forceinline__ int block_scan(int x, int* total) {
+  __shared__ int part[32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int sum = x;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
+  }
+  if (lane == 31) part[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    int y = part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    part[lane] = y;
+  }
+  __syncthreads();
+  const int before = warp ? part[warp - 1] : 0;
+  *total = part[31];
+  __syncthreads();
+  return before + sum - x;
+}
+
+// Which entry of a batch names a slot first: a hash table in shared memory.
+struct FirstNamed {
+  int *key, *who;
+  int mask;
+  __device__ void clear() {
+    for (int i = threadIdx.x; i <= mask; i += blockDim.x) {
+      key[i] = -1;
+      who[i] = INT_MAX;
+    }
+  }
+  __device__ int find(int slot) const {
+    int at = static_cast<int>(static_cast<uint32_t>(slot) * 2654435761u >> 8) & mask;
+    while (key[at] != slot) at = (at + 1) & mask;
+    return at;
+  }
+  __device__ void name(int slot, int i) {
+    int at = static_cast<int>(static_cast<uint32_t>(slot) * 2654435761u >> 8) & mask;
+    for (;;) {
+      const int was = atomicCAS(&key[at], -1, slot);
+      if (was == -1 || was == slot) break;
+      at = (at + 1) & mask;
+    }
+    atomicMin(&who[at], i);
+  }
+};
+inline int hash_slots(int n) {
+  int m = 64;
+  while (m < 2 * n) m *= 2;
+  return m;
+}
+
+// lx_kv_extend (COPY false: a = seqs, b = counts) and lx_kv_copy (a = src, b = dst).
+template <bool COPY>
+__global__ void __launch_bounds__(PLAN_THREADS)
+    k_kv_grow(const lx_kv_cache c, int n, int hash, const int* __restrict__ a, const int* __restrict__ b, int* start) {
+  extern __shared__ int sm[];
+  int* before = sm;          // [n + 1] pages that earlier entries need
+  int* slot = before + n + 1;  // [n] the sequence that grows, -1: refused
+  int* tail = slot + n;        // [n] page to copy first, -1: none (COPY: the source slot)
+  int* len = tail + n;         // [n] tokens before the call (COPY: of the source)
+  FirstNamed named{len + n, len + n + hash, hash - 1};
+  __shared__ int moves;
+  const int tid = threadIdx.x;
+  if (tid == 0) moves = 0;
+  named.clear();
+  __syncthreads();
+  for (int i = tid; i < n; i += PLAN_THREADS) {
+    const int s = COPY ? b[i] : a[i];
+    if (s >= 0 && s < c.n_seq) named.name(s, i);
+  }
+  __syncthreads();
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+    const int i = i0 + tid;
+    int need = 0;
+    if (i < n) {
+      int s = COPY ? b[i] : a[i], extra = -1, tokens = 0;
+      if (s < 0 || s >= c.n_seq || named.who[named.find(s)] != i) {
+        flag(c, LX_KV_SLOT);
+        s = -1;
+      } else if (COPY) {
+        extra = a[i];
+        if (extra < 0 || extra >= c.n_seq || c.lengths[s] != 0) {
+          flag(c, LX_KV_SLOT);
+          s = -1;
+        } else {
+          tokens = length_of(c, extra);
+          need = pages_of(c, tokens);
+        }
+      } else {
+        const int count = b[i];
+        tokens = length_of(c, s);
+        if (count < 0 || static_cast<long long>(tokens) + count > static_cast<long long>(c.max_pages) * c.page) {
+          flag(c, count < 0 ? LX_KV_ROWS : LX_KV_WIDTH);
+          s = -1;
+        } else {
+          const int old = pages_of(c, tokens);
+          need = pages_of(c, tokens + count) - old;
+          if (count > 0 && tokens % c.page != 0) {
+            const int p = row_of(c, s)[old - 1];
+            if (!page_ok(c, p)) {
+              flag(c, LX_KV_PAGE);
+              s = -1;
+              need = 0;
+            } else if (c.refs[p] > 1) {
+              extra = p;
+              ++need;
+            }
+          }
+        }
+      }
+      slot[i] = s;
+      tail[i] = extra;
+      len[i] = tokens;
+    }
+    int total;
+    const int at = block_scan(need, &total);
+    if (i < n) before[i] = base + at;
+    base += total;
+  }
+  if (tid == 0) before[n] = base;
+  __syncthreads();
+  // how many pages are free
+  int count = 0;
+  for (int p = tid; p < c.n_pages; p += PLAN_THREADS) count += c.refs[p] == 0;
+  int n_free;
+  block_scan(count, &n_free);
+  // give them out
+  const int wanted = before[n];
+  int rank0 = 0;
+  for (int p0 = 0; p0 < c.n_pages && rank0 < wanted; p0 += TILE) {
+    int is_free = 0;
+    for (int x = 0; x < 4; ++x) {
+      const int p = p0 + 4 * tid + x;
+      if (p < c.n_pages && c.refs[p] == 0) is_free |= 1 << x;
+    }
+    int total;
+    int rank = rank0 + block_scan(__popc(is_free), &total);
+    rank0 += total;
+    for (int x = 0; x < 4; ++x) {
+      if (!(is_free >> x & 1)) continue;
+      const int p = p0 + 4 * tid + x, r = rank++;
+      if (r >= wanted) break;
+      int lo = 0, hi = n;  // the entry with before[lo] <= r < before[lo + 1]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (before[mid] <= r)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      if (before[lo + 1] > n_free) break;  // not served, nor is any later one
+      const int s = slot[lo], k = r - before[lo];
+      c.refs[p] = 1;
+      if (COPY) {
+        row_of(c, s)[k] = p;
+        const int from = row_of(c, tail[lo])[k];
+        src_list(c)[r] = from;
+        dst_list(c)[r] = p;
+        if (!page_ok(c, from)) flag(c, LX_KV_PAGE);
+        atomicMax(&moves, r + 1);
+      } else {
+        const int old = pages_of(c, len[lo]);
+        if (tail[lo] >= 0) {
+          row_of(c, s)[old - 1 + k] = p;
+          if (k == 0) {
+            const int m = atomicAdd(&moves, 1);
+            src_list(c)[m] = tail[lo];
+            dst_list(c)[m] = p;
+          }
+        } else {
+          row_of(c, s)[old + k] = p;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += PLAN_THREADS) {
+    const int s = slot[i];
+    const bool served = s >= 0 && before[i + 1] <= n_free;
+    if (s >= 0 && !served) flag(c, LX_KV_FULL);
+    if (COPY) {
+      if (served) c.lengths[s] = len[i];
+    } else {
+      start[i] = served ? len[i] : LX_KV_REFUSED;
+      if (served) {
+        c.lengths[s] = len[i] + b[i];
+        if (tail[i] >= 0) atomicSub(&c.refs[tail[i]], 1);
+      }
+    }
+  }
+  if (tid == 0) c.scratch[MOVES] = moves;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS)
+    k_kv_fork(const lx_kv_cache c, int n, int hash, const int* __restrict__ src, const int* __restrict__ dst) {
+  extern __shared__ int sm[];
+  int* len = sm;  // [n] tokens to share, -1: refused
+  FirstNamed named{len + n, len + n + hash, hash - 1};
+  named.clear();
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
+    if (dst[i] >= 0 && dst[i] < c.n_seq) named.name(dst[i], i);
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    const int s = src[i], d = dst[i];
+    if (s < 0 || s >= c.n_seq || d < 0 || d >= c.n_seq || named.who[named.find(d)] != i || c.lengths[d] != 0) {
+      flag(c, LX_KV_SLOT);
+      len[i] = -1;
+    } else {
+      len[i] = length_of(c, s);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x / 32; i < n; i += PLAN_THREADS / 32) {
+    if (len[i] < 0) continue;
+    const int s = src[i], d = dst[i], pages = pages_of(c, len[i]);
+    for (int k = threadIdx.x % 32; k < pages; k += 32) {
+      const int p = row_of(c, s)[k];
+      if (page_ok(c, p))
+        atomicAdd(&c.refs[p], 1);
+      else
+        flag(c, LX_KV_PAGE);
+      row_of(c, d)[k] = p;
+    }
+    if (threadIdx.x % 32 == 0) c.lengths[d] = len[i];
+  }
+}
+
+// One warp an entry.  Entries may name a slot twice: each table entry is taken
+// off by whoever exchanges it first, and the length takes the least keep.
+__global__ void k_kv_free(const lx_kv_cache c, int n, const int* __restrict__ seqs, const int* __restrict__ keep) {
+  const int i = (blockIdx.x * blockDim.x + threadIdx.x) / 32, lane = threadIdx.x % 32;
+  if (i >= n) return;
+  const int s = seqs[i], k0 = keep[i];
+  if (s < 0 || s >= c.n_seq || k0 < 0) {
+    if (lane == 0) flag(c, k0 < 0 ? LX_KV_ROWS : LX_KV_SLOT);
+    return;
+  }
+  int len = 0;
+  if (lane == 0) len = min(atomicMin(&c.lengths[s], k0), c.max_pages * c.page);
+  len = __shfl_sync(0xffffffffu, len, 0);
+  if (k0 >= len) return;
+  const int pages = pages_of(c, len);
+  for (int k = pages_of(c, k0) + lane; k < pages; k += 32) {
+    const int p = atomicExch(&row_of(c, s)[k], -1);
+    if (page_ok(c, p)) {
+      if (atomicSub(&c.refs[p], 1) <= 0) {
+        atomicAdd(&c.refs[p], 1);
+        flag(c, LX_KV_PAGE);
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) k_kv_compact(const lx_kv_cache c, int* used) {
+  const int tid = threadIdx.x;
+  int count = 0, u;
+  for (int p = tid; p < c.n_pages; p += PLAN_THREADS) count += c.refs[p] != 0;
+  block_scan(count, &u);
+  int holes = 0, movers = 0;
+  for (int p0 = 0; p0 < c.n_pages; p0 += TILE) {
+    int hole = 0, mover = 0;
+    for (int x = 0; x < 4; ++x) {
+      const int p = p0 + 4 * tid + x;
+      if (p >= c.n_pages) continue;
+      const bool held = c.refs[p] != 0;
+      if (p < u && !held) hole |= 1 << x;
+      if (p >= u) {
+        if (held) mover |= 1 << x;
+        place_list(c)[p] = p;
+      }
+    }
+    int total;
+    int at = holes + block_scan(__popc(hole), &total);
+    holes += total;
+    int from = movers + block_scan(__popc(mover), &total);
+    movers += total;
+    for (int x = 0; x < 4; ++x) {
+      const int p = p0 + 4 * tid + x;
+      if (hole >> x & 1) dst_list(c)[at++] = p;
+      if (mover >> x & 1) src_list(c)[from++] = p;
+    }
+  }
+  __syncthreads();
+  for (int k = tid; k < movers; k += PLAN_THREADS) {
+    const int from = src_list(c)[k], to = dst_list(c)[k];
+    place_list(c)[from] = to;
+    c.refs[to] = c.refs[from];
+    c.refs[from] = 0;
+  }
+  if (tid == 0) {
+    c.scratch[MOVES] = movers;
+    c.scratch[USED] = u;
+    *used = u;
+  }
+}
+
+constexpr int MOVE_THREADS = 256;
+constexpr int PIECE = 16 * MOVE_THREADS * 4;  // bytes that a block copies at once
+
+// Copies the listed pages in every layer; REMAP: also renames them in the tables.
+template <bool REMAP>
+__global__ void __launch_bounds__(MOVE_THREADS) k_kv_move(const lx_kv_cache c) {
+  const int moves = c.scratch[MOVES];
+  if (moves == 0) return;
+  const size_t bytes = static_cast<size_t>(c.kv_heads) * (c.page / BLOCK) * block_bytes(c.head_dim, c.group);
+  const int pieces = static_cast<int>((bytes + PIECE - 1) / PIECE);
+  const long long items = static_cast<long long>(moves) * c.n_layers * pieces;
+  uint8_t* pool = static_cast<uint8_t*>(c.pool);
+  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    const int piece = static_cast<int>(it % pieces);
+    const int layer = static_cast<int>(it / pieces % c.n_layers), m = static_cast<int>(it / pieces / c.n_layers);
+    const int from = src_list(c)[m], to = dst_list(c)[m];
+    if (!page_ok(c, from) || !page_ok(c, to)) continue;
+    const size_t off = static_cast<size_t>(piece) * PIECE;
+    const uint8_t* s = pool + (static_cast<size_t>(layer) * c.n_pages + from) * bytes + off;
+    uint8_t* d = pool + (static_cast<size_t>(layer) * c.n_pages + to) * bytes + off;
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const size_t o = 16 * (threadIdx.x + static_cast<size_t>(i) * MOVE_THREADS);
+      if (off + o < bytes) x[i] = *reinterpret_cast<const uint4*>(s + o);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const size_t o = 16 * (threadIdx.x + static_cast<size_t>(i) * MOVE_THREADS);
+      if (off + o < bytes) *reinterpret_cast<uint4*>(d + o) = x[i];
+    }
+  }
+  if (REMAP) {
+    const int u = c.scratch[USED];
+    const long long cells = static_cast<long long>(c.n_seq) * c.max_pages;
+    for (long long i = blockIdx.x * static_cast<long long>(MOVE_THREADS) + threadIdx.x; i < cells;
+         i += static_cast<long long>(gridDim.x) * MOVE_THREADS) {
+      const int p = c.table[i];
+      if (p >= u && p < c.n_pages) c.table[i] = place_list(c)[p];
+    }
+  }
+}
+
+template <typename K>
+bool allow_smem(K kernel, size_t bytes) {
+  return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                    static_cast<int>(bytes)) == cudaSuccess;
+}
+
+bool batch_ok(const lx_kv_cache* c, int n, const void* a, const void* b) {
+  return cache_ok(c) && n > 0 && n <= LX_KV_MAX_BATCH && a && b && aligned(a, 4) && aligned(b, 4);
+}
+
+template <bool REMAP>
+bool move(const lx_kv_cache& c, cudaStream_t s) {
+  return launch(k_kv_move<REMAP>, dim3(4 * num_sms()), dim3(MOVE_THREADS), 0, s, c);
+}
+
+template <bool COPY>
+int grow(const lx_kv_cache* c, int n, const int32_t* a, const int32_t* b, int32_t* start, void* stream) {
+  OnDevice on(c->device);
+  if (!on.ok()) return LX_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int hash = hash_slots(n);
+  const size_t smem = (static_cast<size_t>(4) * n + 1 + 2 * hash) * sizeof(int);
+  if (!allow_smem(k_kv_grow<COPY>, smem)) return LX_ERR_CUDA;
+  if (!launch(k_kv_grow<COPY>, dim3(1), dim3(PLAN_THREADS), smem, s, *c, n, hash, a, b, start)) return LX_ERR_CUDA;
+  return move<false>(*c, s) ? LX_OK : LX_ERR_CUDA;
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace lx
+
+using namespace lx::kv;
+
+extern "C" {
+
+size_t lx_kv_pool_bytes(const lx_kv_cache* c) {
+  if (!geometry_ok(c)) return 0;
+  return static_cast<size_t>(c->n_layers) * c->n_pages * c->kv_heads * (c->page / BLOCK) *
+         block_bytes(c->head_dim, c->group);
+}
+
+size_t lx_kv_scratch_ints(const lx_kv_cache* c) {
+  return geometry_ok(c) ? HEAD + static_cast<size_t>(3) * c->n_pages : 0;
+}
+
+int lx_kv_reset(const lx_kv_cache* c, void* stream) {
+  if (!cache_ok(c)) return LX_ERR_ARG;
+  OnDevice on(c->device);
+  if (!on.ok()) return LX_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool ok = cudaMemsetAsync(c->lengths, 0, sizeof(int) * c->n_seq, s) == cudaSuccess &&
+                  cudaMemsetAsync(c->table, 0xFF, sizeof(int) * c->n_seq * static_cast<size_t>(c->max_pages), s) ==
+                      cudaSuccess &&
+                  cudaMemsetAsync(c->refs, 0, sizeof(int) * static_cast<size_t>(c->n_pages), s) == cudaSuccess &&
+                  cudaMemsetAsync(c->error, 0, sizeof(int), s) == cudaSuccess;
+  return ok ? LX_OK : LX_ERR_CUDA;
+}
+
+int lx_kv_status(const lx_kv_cache* c, int32_t* bits, void* stream) {
+  if (!cache_ok(c) || !bits) return LX_ERR_ARG;
+  OnDevice on(c->device);
+  if (!on.ok()) return LX_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool ok = cudaMemcpyAsync(bits, c->error, sizeof(int), cudaMemcpyDeviceToHost, s) == cudaSuccess &&
+                  cudaMemsetAsync(c->error, 0, sizeof(int), s) == cudaSuccess && cudaStreamSynchronize(s) == cudaSuccess;
+  return ok ? LX_OK : LX_ERR_CUDA;
+}
+
+int lx_kv_extend(const lx_kv_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, int32_t* start,
+                 void* stream) {
+  if (!batch_ok(c, n, seqs, counts) || !start || !aligned(start, 4)) return LX_ERR_ARG;
+  return grow<false>(c, n, seqs, counts, start, stream);
+}
+
+int lx_kv_copy(const lx_kv_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream) {
+  if (!batch_ok(c, n, src, dst)) return LX_ERR_ARG;
+  return grow<true>(c, n, src, dst, nullptr, stream);
+}
+
+int lx_kv_fork(const lx_kv_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream) {
+  if (!batch_ok(c, n, src, dst)) return LX_ERR_ARG;
+  OnDevice on(c->device);
+  if (!on.ok()) return LX_ERR_CUDA;
+  const int hash = hash_slots(n);
+  const size_t smem = (static_cast<size_t>(n) + 2 * hash) * sizeof(int);
+  if (!allow_smem(k_kv_fork, smem)) return LX_ERR_CUDA;
+  return launch(k_kv_fork, dim3(1), dim3(PLAN_THREADS), smem, static_cast<cudaStream_t>(stream), *c, n, hash, src, dst)
+             ? LX_OK
+             : LX_ERR_CUDA;
+}
+
+int lx_kv_free(const lx_kv_cache* c, int32_t n, const int32_t* seqs, const int32_t* keep, void* stream) {
+  if (!batch_ok(c, n, seqs, keep)) return LX_ERR_ARG;
+  OnDevice on(c->device);
+  if (!on.ok()) return LX_ERR_CUDA;
+  return launch(k_kv_free, dim3((n + 3) / 4), dim3(128), 0, static_cast<cudaStream_t>(stream), *c, n, seqs, keep)
+             ? LX_OK
+             : LX_ERR_CUDA;
+}
+
+int lx_kv_compact(const lx_kv_cache* c, int32_t* used, void* stream) {
+  if (!cache_ok(c) || !used || !aligned(used, 4)) return LX_ERR_ARG;
+  OnDevice on(c->device);
+  if (!on.ok()) return LX_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!launch(k_kv_compact, dim3(1), dim3(PLAN_THREADS), 0, s, *c, used)) return LX_ERR_CUDA;
+  return move<true>(*c, s) ? LX_OK : LX_ERR_CUDA;
+}
+
+}  // extern "C"

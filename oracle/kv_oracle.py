@@ -1,0 +1,247 @@
+"""CPU oracle for the paged 4-bit key/value cache (TEST INFRASTRUCTURE ONLY).
+
+The parity checker for the operators of ``include/larynx_kv.h``: quantising in
+exact rational arithmetic where it matters, attention in float64, the page
+operations as plain Python over lists.  No reference counterpart: the reference
+keeps no keys or values between calls.  Only ``tests/`` may import this module.
+"""
+
+from __future__ import annotations
+
+from fractions import Fraction
+
+import numpy as np
+
+FULL, SLOT, WIDTH, PAGE, ROWS = 1, 2, 4, 8, 16
+REFUSED = -2 ** 31
+
+
+def bf16_bits_value(bits):
+    return (np.asarray(bits, np.uint32) << 16).view(np.float32)
+
+
+def bf16_down(x: float) -> np.float32:
+    """The bf16 value at or below the float32 x (an infinity where there is none)."""
+    u = int(np.float32(x).view(np.uint32))
+    if u >> 31:
+        u += 0xFFFF
+    return bf16_bits_value(u >> 16)[()]
+
+
+def _least_step(range_: Fraction) -> np.float32:
+    """The least bf16 value s >= 2^-126 with 15 s >= range."""
+    s = np.float32(2.0 ** -126)
+    if 15 * Fraction(float(s)) >= range_:
+        return s
+    bits = int(np.float32(float(range_) / 15).view(np.uint32)) >> 16
+    bits = max(bits - 2, 0x0080)
+    while 15 * Fraction(float(bf16_bits_value(bits)[()])) < range_:
+        bits += 1
+    return bf16_bits_value(bits)[()]
+
+
+def quantise_group(x):
+    """One group (float32 values) -> codes, s, m; codes None where s = m = NaN."""
+    x = np.asarray(x, np.float32)
+    if not np.isfinite(x).all():
+        return None, np.float32(np.nan), np.float32(np.nan)
+    m = bf16_down(x.min())
+    with np.errstate(over="ignore"):
+        if not np.isfinite(m) or not np.isfinite(np.float32(x.max()) - np.float32(m)):
+            return None, np.float32(np.nan), np.float32(np.nan)
+    fm = Fraction(float(m))
+    s = _least_step(Fraction(float(x.max())) - fm)
+    fs = Fraction(float(s))
+    codes = np.array([round((Fraction(float(v)) - fm) / fs) for v in x], np.int64)  # ties to even
+    assert codes.min() >= 0 and codes.max() <= 15
+    return codes, s, m
+
+
+def quantise(x, group):
+    """[..., dim] -> the float32 values that its groups stand for."""
+    x = np.asarray(x, np.float32)
+    flat = x.reshape(-1, group)
+    out = np.empty(flat.shape, np.float32)
+    for i, row in enumerate(flat):
+        codes, s, m = quantise_group(row)
+        out[i] = np.nan if codes is None else (codes * float(s) + float(m)).astype(np.float32)
+    return out.reshape(x.shape)
+
+
+def unpack_block(block, dim, group):
+    """The bytes of one block -> K and V values [16, dim] in float64, by the places the header gives."""
+    block = np.asarray(block, np.uint8)
+    k, v = np.empty((16, dim)), np.empty((16, dim))
+    for t in range(16):
+        for d in range(dim):
+            h, w, e = d // 64, d % 64 // 32, d % 8
+            at = 512 * h + 16 * (4 * (t % 8) + d % 32 // 8) + 8 * (t // 8) + 4 * w
+            word = int(block[at:at + 4].view(np.uint32)[0])
+            ck = word >> (4 * (e // 2) + 16 * (e % 2)) & 15
+            at = 512 * (dim // 64) + 512 * h + 16 * (4 * (d % 32 // 4) + t % 8 // 2) + 8 * (t // 8) + 4 * w + 2 * (t % 2)
+            cv = int(block[at:at + 2].view(np.uint16)[0]) >> (4 * (d % 4)) & 15
+            at = 1024 * (dim // 64) + 64 * (d // group) + 4 * (4 * (t % 8 // 2) + 2 * (t // 8) + t % 2)
+            for out, code, p in ((k, ck, at), (v, cv, at + 64 * (dim // group))):
+                s, m = bf16_bits_value(block[p:p + 4].view(np.uint16))
+                out[t, d] = code * float(s) + float(m)
+    return k, v
+
+
+def visible(p: int, length: int, chunk: int, left: int):
+    """[lo, hi) of the keys that a row at position p sees."""
+    if chunk == 0:
+        return 0, length
+    begin = p // chunk * chunk
+    return (max(0, begin - left) if left >= 0 else 0), min(length, begin + chunk)
+
+
+def attention(q, k, v, positions, scale, chunk, left, seen=None):
+    """q [rows, heads, dim], k and v [keys, kv heads, dim] in float64.  Returns
+    out, lse, and the bound's parts: the largest sum of |q| |k| scale over the visible keys
+    of each (row, head), and the weighted sum of |v| per output.  `seen`: keys that exist (bool), default all."""
+    rows, heads, dim = q.shape
+    per = heads // k.shape[1]
+    out, lse = np.zeros(q.shape), np.full((rows, heads), -np.inf)
+    size, weight = np.zeros((rows, heads)), np.zeros(q.shape)
+    for r, p in enumerate(positions):
+        lo, hi = visible(p, k.shape[0], chunk, left)
+        at = np.arange(lo, max(lo, hi))
+        if seen is not None:
+            at = at[seen[at]]
+        if at.size == 0:
+            continue
+        for h in range(heads):
+            kk, vv = k[at, h // per], v[at, h // per]
+            s = kk @ q[r, h] * scale
+            top = s.max()
+            w = np.exp(s - top)
+            lse[r, h] = top + np.log(w.sum())
+            w /= w.sum()
+            out[r, h] = w @ vv
+            size[r, h] = (np.abs(kk) @ np.abs(q[r, h])).max() * abs(scale)
+            weight[r, h] = w @ np.abs(vv)
+    return out, lse, size, weight
+
+
+class Pages:
+    """Tables, lengths, reference counts and page contents (any value per page)."""
+
+    def __init__(self, n_pages, n_seq, max_pages, page):
+        self.n_pages, self.n_seq, self.width, self.page = n_pages, n_seq, max_pages, page
+        self.table = [[-1] * max_pages for _ in range(n_seq)]
+        self.length, self.refs = [0] * n_seq, [0] * n_pages
+        self.data = [None] * n_pages
+        self.error = 0
+
+    def _of(self, tokens):
+        return -(-tokens // self.page)
+
+    def _served(self, needs):
+        """Which entries the free pages serve, and the pages they get."""
+        free = [p for p in range(self.n_pages) if self.refs[p] == 0]
+        got, at = [], 0
+        for need in needs:
+            got.append(free[at:at + need] if at + need <= len(free) else None)
+            at += need
+        return got
+
+    def _dupes(self, slots):
+        return [s in slots[:i] for i, s in enumerate(slots)]
+
+    def extend(self, seqs, counts):
+        dup, needs, ok, tails = self._dupes(seqs), [], [], []
+        for s, n, d in zip(seqs, counts, dup):
+            need, tail, fine = 0, None, True
+            if not 0 <= s < self.n_seq or d:
+                self.error |= SLOT
+                fine = False
+            elif n < 0:
+                self.error |= ROWS
+                fine = False
+            elif self.length[s] + n > self.width * self.page:
+                self.error |= WIDTH
+                fine = False
+            else:
+                length = self.length[s]
+                need = self._of(length + n) - self._of(length)
+                if n > 0 and length % self.page and self.refs[self.table[s][self._of(length) - 1]] > 1:
+                    tail = self.table[s][self._of(length) - 1]
+                    need += 1
+            needs.append(need)
+            ok.append(fine)
+            tails.append(tail)
+        start, drop = [], []
+        for s, n, fine, tail, got in zip(seqs, counts, ok, tails, self._served(needs)):
+            if not fine or got is None:
+                self.error |= FULL if fine else 0
+                start.append(REFUSED)
+                continue
+            start.append(self.length[s])
+            old = self._of(self.length[s])
+            got = list(got)
+            for p in got:
+                self.refs[p] = 1
+            if tail is not None:
+                drop.append((tail, got[0]))
+                self.table[s][old - 1] = got.pop(0)
+            self.table[s][old:old + len(got)] = got
+            self.length[s] += n
+        for tail, to in drop:
+            self.refs[tail] -= 1
+            self.data[to] = self.data[tail]
+        return start
+
+    def _pairs(self, src, dst):
+        got = []
+        before = list(self.length)
+        for s, d, dup in zip(src, dst, self._dupes(dst)):
+            fine = 0 <= s < self.n_seq and 0 <= d < self.n_seq and not dup and before[d] == 0
+            self.error |= 0 if fine else SLOT
+            got.append(fine)
+        return got, before
+
+    def fork(self, src, dst):
+        fine, before = self._pairs(src, dst)
+        for s, d, f in zip(src, dst, fine):
+            if f:
+                pages = self.table[s][:self._of(before[s])]
+                for p in pages:
+                    self.refs[p] += 1
+                self.table[d][:len(pages)] = pages
+                self.length[d] = before[s]
+
+    def copy(self, src, dst):
+        fine, before = self._pairs(src, dst)
+        needs = [self._of(before[s]) if f else 0 for s, f in zip(src, fine)]
+        for s, d, f, got in zip(src, dst, fine, self._served(needs)):
+            if not f or got is None:
+                self.error |= FULL if f else 0
+                continue
+            for a, b in zip(self.table[s], got):
+                self.data[b] = self.data[a]
+                self.refs[b] = 1
+            self.table[d][:len(got)] = got
+            self.length[d] = before[s]
+
+    def free(self, seqs, keep):
+        for s, n in zip(seqs, keep):
+            if not 0 <= s < self.n_seq or n < 0:
+                self.error |= ROWS if n < 0 else SLOT
+                continue
+            if n >= self.length[s]:
+                continue
+            for c in range(self._of(n), self._of(self.length[s])):
+                self.refs[self.table[s][c]] -= 1
+                self.table[s][c] = -1
+            self.length[s] = n
+
+    def compact(self):
+        used = sum(r > 0 for r in self.refs)
+        holes = [p for p in range(used) if self.refs[p] == 0]
+        movers = [p for p in range(used, self.n_pages) if self.refs[p] > 0]
+        place = dict(zip(movers, holes))
+        for a, b in place.items():
+            self.refs[b], self.refs[a] = self.refs[a], 0
+            self.data[b] = self.data[a]
+        self.table = [[place.get(p, p) for p in row] for row in self.table]
+        return used

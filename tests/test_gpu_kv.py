@@ -1,0 +1,650 @@
+"""The paged 4-bit cache on the GPU, through the C ABI, against oracle/kv_oracle.py
+(exact quantising, attention in float64, pages as plain lists).
+
+Attention's bound, per output: its rounding, half a step of the type
+(2^-8 relative in bf16, 2^-11 in fp16), plus 2^-10 of the weighted sum of |v| for the
+probabilities' rounding to fp16 (half a step is 2^-11, once in the numerator; the
+denominator is not rounded), plus the effect of the scores' error: a score is a sum in fp32 of
+at most 2 * 128 terms, each off by at most a few 2^-24, so it is off by at most dS = 2^-16 times the sum of
+|q| |k| scale (256 * 2^-24), and 2^-18 for the exponential's own error; weights then move by at most 2 dS relative.
+lse moves by at most dS + 2^-20 + 2^-22 |lse|."""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from oracle import kv_oracle as ko  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+TORCH = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+HALF = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11, "fp32": 2.0 ** -24}
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+class Cache:
+    """A KVCache with its buffers."""
+
+    def __init__(self, layers=1, n_pages=32, n_seq=4, max_pages=8, heads=2, dim=64, group=64, page=16, fill=None):
+        from larynx_b200 import kv
+        self.kv, self.heads, self.dim, self.group, self.page, self.layers = kv, heads, dim, group, page, layers
+        self.n_pages, self.n_seq, self.width = n_pages, n_seq, max_pages
+        self.pool = torch.empty(kv.pool_bytes(layers, n_pages, heads, dim, group, page), dtype=torch.uint8, device="cuda")
+        if fill is None:
+            self.pool.random_(0, 256)
+        elif fill >= 0:
+            self.pool.fill_(fill)
+        self.table = torch.zeros(n_seq, max_pages, dtype=torch.int32, device="cuda")
+        self.lengths = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
+        self.refs = torch.zeros(n_pages, dtype=torch.int32, device="cuda")
+        self.scratch = torch.randint(-9, 9, (kv.scratch_ints(n_pages, n_seq, max_pages),), dtype=torch.int32, device="cuda")
+        self.error = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self.c = kv.KVCache(layers, n_pages, n_seq, max_pages, heads, dim, group, page, self.pool.data_ptr(),
+                            self.table.data_ptr(), self.lengths.data_ptr(), self.refs.data_ptr(),
+                            self.scratch.data_ptr(), self.error.data_ptr())
+        self.c.reset()
+
+    def bytes(self):
+        """[layers, pages, heads, blocks, bytes]"""
+        return self.pool.view(self.layers, self.n_pages, self.heads, self.page // 16, -1)
+
+    def grow(self, seqs, counts):
+        a, b, s = i32(seqs), i32(counts), i32([99] * len(seqs))
+        self.c.extend(len(seqs), a.data_ptr(), b.data_ptr(), s.data_ptr())
+        return s
+
+    def pairs(self, what, a, b):
+        x, y = i32(a), i32(b)
+        getattr(self.c, what)(len(a), x.data_ptr(), y.data_ptr())
+        torch.cuda.synchronize()
+
+    def batch(self, counts, seqs=None, start=None, max_rows=None):
+        seqs, row0, start = (v if v is None or torch.is_tensor(v) else i32(v) for v in
+                             (seqs, [sum(counts[:i]) for i in range(len(counts) + 1)], start))
+        p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+        rows = self.c.rows(len(counts), sum(counts), max(counts) if max_rows is None else max_rows, p(seqs), p(row0),
+                           p(start))
+        rows.keep = seqs, row0, start  # alive as long as the batch
+        return rows
+
+    def write(self, k, v, rows, dtype, layer=0, **kw):
+        self.c.write(layer, rows, dtype, k.data_ptr(), v.data_ptr(), **kw)
+
+    def read(self, rows, total, dtype="fp32", layer=0):
+        k = torch.full((total, self.heads, self.dim), 7.0, dtype=TORCH[dtype], device="cuda")
+        v = torch.full_like(k, 7.0)
+        self.c.read(layer, rows, dtype, k.data_ptr(), v.data_ptr())
+        torch.cuda.synchronize()
+        return k, v
+
+    def fill(self, lengths, seed=0, layer=0, scale=1.0):
+        """Grow all slots to `lengths` and write random rows; the values they read as, per slot, in float64."""
+        g = torch.Generator().manual_seed(seed)
+        start = self.grow(list(range(len(lengths))), lengths)
+        k = torch.randn(sum(lengths), self.heads, self.dim, generator=g) * scale + torch.randn(self.heads, self.dim, generator=g)
+        v = torch.randn(sum(lengths), self.heads, self.dim, generator=g)
+        kd, vd = k.cuda(), v.cuda()
+        rows = self.batch(lengths, start=start, max_rows=max(lengths))
+        if sum(lengths):
+            self.write(kd, vd, rows, "fp32", layer=layer)
+        torch.cuda.synchronize()
+        kq, vq = (ko.quantise(x.numpy(), self.group).astype(np.float64) for x in (k, v))
+        at = np.cumsum([0] + list(lengths))
+        return [(kq[a:b], vq[a:b]) for a, b in zip(at, at[1:])]
+
+    def attend(self, q, rows, dtype, scale=0.125, chunk=0, left=-1, layer=0, max_len=0, lse=True, out=None, **kw):
+        heads = q.shape[1]
+        out = torch.full(q.shape, 3.0, dtype=q.dtype, device="cuda") if out is None else out
+        l = torch.full(q.shape[:2], 3.0, device="cuda")
+        self.c.attention(layer, rows, heads, dtype, q.data_ptr(), out.data_ptr(), lse=l.data_ptr() if lse else 0,
+                         scale=scale, chunk=chunk, left=left, max_len=max_len, **kw)
+        return out, l
+
+
+def check(out, lse, want, dtype):
+    """`want`: (out, lse, size, weight) of ko.attention."""
+    ref, rl, size, weight = want
+    out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    ds = 2.0 ** -16 * size + 2.0 ** -18
+    tol = HALF[dtype] * np.abs(ref) + (2.0 ** -10 + 2 * ds[..., None]) * weight + 2.0 ** -25
+    bad = np.abs(out - ref) > tol
+    assert np.isfinite(out).all() and not bad.any(), (np.argwhere(bad)[:4], np.abs(out - ref).max())
+    none = np.isinf(rl)
+    assert (np.isneginf(lse) == none).all()
+    assert (out[none] == 0).all()
+    tol = ds + 2.0 ** -20 + 2.0 ** -22 * np.abs(np.where(none, 0, rl))
+    assert (np.abs(np.where(none, 0, lse) - np.where(none, 0, rl)) <= tol).all()
+
+
+# ---------------------------------------------------------------------------
+# writing and reading
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim,group,page", [(64, 64, 16), (64, 32, 32), (128, 64, 64), (128, 32, 128)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_write_read(dim, group, page, dtype):
+    """Values come back as the oracle's quantiser gives them, in two steps that end and begin inside a block."""
+    c = Cache(layers=2, n_pages=40, n_seq=3, max_pages=11, heads=3, dim=dim, group=group, page=page)
+    g = torch.Generator().manual_seed(dim + group)
+    first, more = [5, 0, 37], [1, 33, 60]
+    k, v = (torch.randn(sum(first) + sum(more), 3, dim, generator=g).to(TORCH[dtype]) for _ in range(2))
+    kd, vd = k.cuda(), v.cuda()
+    done = 0
+    before = c.pool.clone()
+    for counts in (first, more):
+        start = c.grow([0, 1, 2], counts)
+        n = sum(counts)
+        a, b = kd[done:done + n].contiguous(), vd[done:done + n].contiguous()
+        c.write(a, b, c.batch(counts, start=start), dtype, layer=1)
+        for out in ("fp32", dtype):
+            gk, gv = c.read(c.batch(counts, start=start), n, out, layer=1)
+            for got, x in ((gk, k), (gv, v)):
+                want = torch.from_numpy(ko.quantise(x[done:done + n].float().numpy(), group)).to(TORCH[out])
+                assert torch.equal(got.cpu(), want)
+        done += n
+    assert c.c.status() == 0
+    # the other layer was not touched
+    assert torch.equal(c.bytes()[0], before.view_as(c.pool).view(c.bytes().shape)[0])
+
+
+def test_layout_is_the_documented_one():
+    for dim, group in ((64, 64), (64, 32), (128, 64), (128, 32)):
+        c = Cache(n_pages=3, n_seq=1, max_pages=2, heads=2, dim=dim, group=group, page=32)
+        (k, v), = c.fill([45], seed=dim + group)
+        table = c.table.cpu().numpy()[0]
+        data = c.bytes().cpu().numpy()
+        for b in range(3):
+            for h in range(2):
+                bk, bv = ko.unpack_block(data[0, table[b // 2], h, b % 2], dim, group)
+                n = min(16, 45 - 16 * b)
+                assert np.array_equal(bk[:n].astype(np.float32), k[16 * b:16 * b + n, h].astype(np.float32))
+                assert np.array_equal(bv[:n].astype(np.float32), v[16 * b:16 * b + n, h].astype(np.float32))
+
+
+def test_write_special_values():
+    """Ties, constant groups, values next to a border, wide exponents, subnormals, the ends of the range, NaN
+    and infinities (which make their own group NaN and no other)."""
+    rng = np.random.default_rng(5)
+    rows = []
+    for s, m in ((1.0, 0.0), (0.375, -2.5), (2.0 ** -100, 2.0 ** -99)):  # every tie, and its neighbours
+        base = [m, m + 15 * s] + [m + (c + 0.5) * s for c in range(15)]
+        for x in (base, np.nextafter(np.float32(base), np.float32(np.inf)), np.nextafter(np.float32(base), np.float32(-np.inf))):
+            r = np.resize(np.float32(x), 32)
+            r[0], r[1] = m, m + 15 * s
+            rows.append(r)
+    rows.append(np.full(32, -1.7, np.float32))
+    rows.append(np.zeros(32, np.float32))
+    rows.append(np.resize(np.float32([1.0, -1e-8, 1e-20, -1e-30, 0.33333]), 32))
+    rows.append((rng.standard_normal(32) * 1e-39).astype(np.float32))
+    rows.append((rng.standard_normal(32) * 1e37).astype(np.float32))
+    rows.append(np.resize(np.float32([3.3e38, 1.0]), 32))
+    for bad in (np.nan, np.inf, -np.inf):
+        r = rng.standard_normal(32).astype(np.float32)
+        r[7] = bad
+        rows.append(r)
+    rows.append(np.resize(np.float32([-3.3e38, 3.3e38]), 32))
+    for _ in range(20):
+        rows.append((rng.standard_normal(32) * np.exp(rng.uniform(-30, 30, 32))).astype(np.float32))
+    while len(rows) % 2:
+        rows.append(rng.standard_normal(32).astype(np.float32))
+    x = np.stack(rows).reshape(-1, 1, 64)
+    c = Cache(n_pages=8, n_seq=1, max_pages=6, heads=1, group=32)
+    d = torch.from_numpy(x).cuda()
+    r = c.batch([len(x)], start=c.grow([0], [len(x)]))
+    c.write(d, d, r, "fp32")
+    for got in c.read(r, len(x)):
+        want = ko.quantise(x, 32)
+        assert np.array_equal(got.cpu().numpy(), want, equal_nan=True)
+
+
+def test_write_many_random_bits():
+    """Random fp32 values by the million: the codes are those of exact arithmetic (float64 division, whose ties are exact here)."""
+    c = Cache(n_pages=300, n_seq=1, max_pages=300, heads=8, dim=128, group=64, page=16)
+    n = 4800
+    g = torch.Generator("cuda").manual_seed(2)
+    x = torch.randn(n, 8, 128, device="cuda", generator=g)
+    r = c.batch([n], start=c.grow([0], [n]))
+    c.write(x, x, r, "fp32")
+    got, _ = c.read(r, n)
+    y = x.double().view(n, 8, 2, 64)
+    lo, hi = y.amin(-1, keepdim=True), y.amax(-1, keepdim=True)
+    part, power = torch.frexp(lo)
+    m = torch.ldexp(torch.floor(part * 256), power - 8)
+    part, power = torch.frexp((hi - m) / 15)
+    s = torch.ldexp(torch.ceil(part * 256), power - 8)
+    want = (torch.round((y - m) / s) * s + m).float().view(n, 8, 128)
+    assert torch.equal(got, want)
+
+
+def test_write_strides_seqs_and_rows_left_alone():
+    """Strided, unaligned rows; slots in another order; rows past the total and rows of refused entries stay as they were."""
+    c = Cache(n_pages=30, n_seq=5, max_pages=6, heads=2)
+    big = torch.randn(60, 3, 2, 69, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    k, v = big[:, 0, :, 1:65], big[:, 2, :, 4:68]
+    seqs, counts = [3, 0, 4], [20, 7, 33]
+    start = c.grow(seqs, counts)
+    rows = c.batch(counts, seqs=seqs, start=start)
+    st = (big.stride(0), big.stride(2))
+    c.write(k, v, rows, "bf16", k_strides=st, v_strides=st)
+    gk = torch.full((70, 2, 130), 5.0, device="cuda")
+    gv = torch.full((70, 2, 130), 5.0, device="cuda")
+    c.c.read(0, rows, "fp32", gk[:, :, 3:].data_ptr(), gv[:, :, 64:].data_ptr(), k_strides=(260, 130), v_strides=(260, 130))
+    torch.cuda.synchronize()
+    for got, x, a in ((gk, k, 3), (gv, v, 64)):
+        want = torch.from_numpy(ko.quantise(x.float().cpu().numpy(), 64))
+        assert torch.equal(got[:60, :, a:a + 64].cpu(), want)
+        assert (got[60:] == 5).all() and (got[:, :, :a] == 5).all() and (got[:, :, a + 64:] == 5).all()
+    assert c.c.status() == 0
+    # entries that were not served: nothing is written, zeros are read
+    before = c.pool.clone()
+    rows = c.batch([3, 2], seqs=[0, 1], start=[ko.REFUSED] * 2)
+    c.write(k, v, rows, "bf16", k_strides=st, v_strides=st)
+    gk, _ = c.read(rows, 6)
+    assert torch.equal(c.pool, before) and (gk[:5] == 0).all() and (gk[5] == 7).all()
+    assert c.c.status() == 0
+
+
+def test_write_outside_and_bad_pages():
+    """Rows outside the sequence, bad slots, bad pages and pages shared with a fork: flagged, skipped, read as 0."""
+    c = Cache(n_pages=10, n_seq=4, max_pages=3)
+    c.fill([20, 5, 0, 0], seed=4)
+    before = c.pool.clone()
+    x = torch.randn(40, 2, 64, device="cuda")
+    for seqs, start, counts, bit in (([0], [20], [4], c.kv.ROWS), ([2], [0], [1], c.kv.ROWS), ([9], [0], [3], c.kv.SLOT),
+                                     ([-1], [0], [3], c.kv.SLOT), ([0], [2 ** 31 - 1], [3], c.kv.ROWS),
+                                     ([0], [-2], [2], c.kv.ROWS), ([0], [-2 ** 31 + 1], [3], c.kv.ROWS)):
+        rows = c.batch(counts, seqs=seqs, start=start)
+        c.write(x, x, rows, "fp32")
+        got, _ = c.read(rows, sum(counts))
+        assert (got == 0).all() and c.c.status() & bit
+        assert torch.equal(c.pool, before)
+    rows = c.batch([3], seqs=[1])
+    rows.max_rows = 2  # more rows than were announced: the third is not touched
+    got, _ = c.read(rows, 3)
+    assert c.c.status() & c.kv.ROWS and (got[2] == 7).all()
+    # a start before the sequence (start None, more rows than tokens)
+    rows = c.batch([8], seqs=[1])
+    got, _ = c.read(rows, 8)
+    assert (got[:3] == 0).all() and (got[3:] != 0).any()
+    # a shared page
+    c.pairs("fork", [1], [2])
+    c.c.status()
+    rows = c.batch([2], seqs=[2], start=[0])
+    c.write(x, x, rows, "fp32")
+    assert c.c.status() & c.kv.ROWS and torch.equal(c.pool, before)
+    # a page that is not in the pool
+    c.table[0, 0] = 77
+    rows = c.batch([20], seqs=[0], start=[0])
+    c.write(x, x, rows, "fp32")
+    got, _ = c.read(rows, 20)
+    assert c.c.status() & c.kv.PAGE and (got[:16] == 0).all() and (got[16:] != 0).any()
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+ATT = [
+    # dim, group, page, kv heads, per kv head, lengths, rows, chunk, left
+    (64, 64, 16, 2, 1, [1, 17, 40], [1, 1, 1], 1, -1),
+    (64, 32, 32, 1, 7, [0, 1, 100, 33], [1, 1, 1, 1], 0, -1),
+    (128, 64, 64, 2, 4, [300, 5, 129], [1, 2, 1], 1, -1),
+    (128, 32, 128, 1, 3, [130, 64], [3, 5], 0, -1),
+    (64, 64, 16, 3, 1, [106, 56, 81, 16], [56, 56, 31, 16], 25, -1),
+    (64, 64, 32, 2, 2, [150, 40, 70], [37, 40, 1], 1, 20),
+    (64, 32, 16, 1, 5, [90, 33], [90, 20], 1, -1),
+    (128, 64, 16, 1, 2, [140, 77], [129, 9], 50, 0),
+    (64, 64, 64, 1, 1, [64, 128], [64, 65], 16, 16),
+    (128, 32, 32, 2, 8, [70, 3], [19, 3], 7, 5),
+    # more rows than tokens: the first rows lie before the sequence and see nothing
+    (64, 64, 16, 1, 2, [3, 0], [10, 4], 1, -1),
+    (64, 64, 16, 1, 2, [3, 0], [10, 4], 0, -1),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ATT)))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attention(case, dtype):
+    dim, group, page, heads, per, lengths, counts, chunk, left = ATT[case]
+    wide = max(-(-n // page) for n in lengths) + 2
+    c = Cache(layers=2, n_pages=sum(-(-n // page) for n in lengths) + 5, n_seq=len(lengths), max_pages=wide, heads=heads, dim=dim, group=group, page=page)
+    held = c.fill(lengths, seed=case, layer=1)
+    g = torch.Generator().manual_seed(100 + case)
+    q = torch.randn(sum(counts), heads * per, dim, generator=g).to(TORCH[dtype])
+    rows = c.batch(counts)
+    out, lse = c.attend(q.cuda(), rows, dtype, scale=dim ** -0.5, chunk=chunk, left=left, layer=1)
+    torch.cuda.synchronize()
+    assert c.c.status() == 0
+    at = 0
+    for (k, v), n in zip(held, counts):
+        pos = [len(k) - n + t for t in range(n)]
+        want = ko.attention(q[at:at + n].double().numpy(), k, v, pos, dim ** -0.5, chunk, left)
+        check(out[at:at + n], lse[at:at + n], want, dtype)
+        at += n
+
+
+@pytest.mark.parametrize("length", [1, 15, 16, 255, 1025, 4099])
+@pytest.mark.parametrize("dim,per", [(64, 1), (128, 4)])
+def test_attention_long(length, dim, per):
+    """One row over growing lengths, with a bound of the length that is right, far too large, or absent."""
+    c = Cache(n_pages=300, n_seq=2, max_pages=280, heads=2, dim=dim, group=64, page=16)
+    (k, v), _ = c.fill([length, 0], seed=length)
+    q = torch.randn(1, 2 * per, dim, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    want = ko.attention(q.double().numpy(), k, v, [length - 1], 0.1, 1, -1)
+    got = []
+    for most in (0, length, 1, 280 * 16):
+        out, lse = c.attend(q.cuda(), c.batch([1]), "bf16", scale=0.1, chunk=1, max_len=most)
+        torch.cuda.synchronize()
+        check(out, lse, want, "bf16")
+        got.append(out)
+    out, lse = c.attend(q.cuda(), c.batch([1]), "bf16", scale=0.1, chunk=1, max_len=1)
+    assert torch.equal(out, got[2])  # the same call, the same bits
+
+
+def test_attention_options():
+    """Slots in any order and twice, no row offsets, given positions, strided and unaligned rows, no lse; rows past
+    the last one stay as they were."""
+    c = Cache(n_pages=40, n_seq=4, max_pages=8, heads=2)
+    held = c.fill([50, 3, 101, 64], seed=9)
+    big = torch.randn(9, 5, 4, 70, generator=torch.Generator().manual_seed(2)).to(torch.float16).cuda()
+    q = big[:, 1, :, 3:67]
+    out = torch.full((9, 6, 80), 3.0, dtype=torch.float16, device="cuda")
+    seqs, pos = [2, 0, 2, 1], [40, 49, 7, 2]
+    s, p = i32(seqs), i32(pos)
+    rows = c.c.rows(4, 8, 2, s.data_ptr(), 0, p.data_ptr())  # two rows each
+    c.attend(q, rows, "fp16", scale=0.2, chunk=10, left=15, lse=False, out=out[:, 1:5, 5:69],
+             q_strides=(big.stride(0), big.stride(2)), out_strides=(480, 80))
+    torch.cuda.synchronize()
+    assert (out[8] == 3).all() and (out[:, 0] == 3).all() and (out[:, 5] == 3).all()
+    assert (out[:, :, :5] == 3).all() and (out[:, :, 69:] == 3).all()
+    for i in range(4):
+        k, v = held[seqs[i]]
+        want = ko.attention(q[2 * i:2 * i + 2].double().cpu().numpy(), k, v, [pos[i], pos[i] + 1], 0.2, 10, 15)
+        lse = torch.from_numpy(want[1])
+        check(out[2 * i:2 * i + 2, 1:5, 5:69], lse, want, "fp16")
+    # entries that were not served, and bad slots: zeros
+    rows = c.batch([1, 2], seqs=[0, 7], start=[ko.REFUSED, 5])
+    out, lse = c.attend(q[:3].contiguous(), rows, "fp16")
+    torch.cuda.synchronize()
+    assert (out == 0).all() and torch.isneginf(lse).all() and c.c.status() == c.kv.SLOT
+
+
+def test_attention_values_that_must_not_matter():
+    """NaN in keys behind the end, behind the chunk and before the window, and in pages of nobody: no effect; in a key
+    that is seen: NaN, in V only in the channels of its group.  Pages outside the pool are not seen."""
+    c = Cache(n_pages=12, n_seq=2, max_pages=6, heads=1, dim=64, group=32, fill=0xFF)  # NaN everywhere
+    (k, v), _ = c.fill([70, 0], seed=1)
+    q = torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    bad = torch.full((1, 1, 64), float("nan"), device="cuda")
+    for at in (5, 69):  # one key before the window, one behind the chunk
+        c.write(bad, bad, c.batch([1], start=[at]), "fp32")
+    rows = c.batch([3], start=[40])
+    out, lse = c.attend(q.cuda(), rows, "bf16", chunk=20, left=25)
+    torch.cuda.synchronize()
+    check(out, lse, ko.attention(q.double().numpy(), k, v, [40, 41, 42], 0.125, 20, 25), "bf16")
+    out, lse = c.attend(q.cuda(), rows, "bf16", chunk=0)
+    torch.cuda.synchronize()
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    c.write(torch.from_numpy(k[69:].astype(np.float32)).cuda(), bad, c.batch([1], start=[69]), "fp32")
+    half = torch.from_numpy(v[5:6].astype(np.float32)).cuda()
+    half[..., 40] = float("nan")
+    c.write(torch.from_numpy(k[5:6].astype(np.float32)).cuda(), half, c.batch([1], start=[5]), "fp32")
+    out, lse = c.attend(q.cuda(), rows, "bf16", chunk=60)
+    torch.cuda.synchronize()
+    assert torch.isfinite(out[..., :32]).all() and torch.isnan(out[..., 32:]).all() and torch.isfinite(lse).all()
+    # a page outside the pool
+    table = c.table.clone()
+    c.table[0, 1] = 12
+    c.table[0, 3] = -5
+    seen = np.ones(70, bool)
+    seen[16:32] = seen[48:64] = False
+    seen[5] = False
+    out, lse = c.attend(q.cuda(), rows, "bf16", chunk=60, left=0)
+    torch.cuda.synchronize()
+    assert c.c.status() == c.kv.PAGE
+    c.table.copy_(table)
+    got_k, got_v = c.read(c.batch([70], start=[0]), 70)
+    kk, vv = got_k.double().cpu().numpy(), got_v.double().cpu().numpy()
+    want = ko.attention(q.double().numpy(), kk, vv, [40, 41, 42], 0.125, 60, 0, seen=seen | (np.arange(70) == 5))
+    ok = torch.isfinite(torch.from_numpy(want[0]))
+    assert torch.equal(torch.isfinite(out.cpu()), ok)
+    check(out[..., :32], lse, tuple(x[..., :32] if x.ndim == 3 else x for x in want), "bf16")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("count", [1, 40])
+def test_attention_ranges(dim, count):
+    """Scores that grow along the sequence, values whose size varies by 2^60 from token to token, large and tiny
+    queries, a long tail behind a sink: sums keep their precision."""
+    n = 900
+    c = Cache(n_pages=70, n_seq=1, max_pages=60, heads=2, dim=dim, group=64)
+    g = torch.Generator().manual_seed(8)
+    k = torch.randn(n, 2, dim, generator=g)
+    k[:, 0] += torch.linspace(-3, 3, n)[:, None]
+    k[3, 1] *= 4
+    v = torch.randn(n, 2, dim, generator=g)
+    v[:, 0] *= torch.exp2(torch.randint(-30, 31, (n, 1), generator=g).float())
+    v[0, 1] *= 1e-6
+    r = c.batch([n], start=c.grow([0], [n]))
+    kd, vd = k.cuda(), v.cuda()
+    c.write(kd, vd, r, "fp32")
+    kq, vq = (ko.quantise(x.numpy(), 64).astype(np.float64) for x in (k, v))
+    for size in (1.0, 2.0 ** 40, 2.0 ** -40):
+        q = (torch.randn(count, 4, dim, generator=g) + 0.5).to(torch.bfloat16)
+        q[:, 1] *= 0.001
+        q = (q.float() * size).to(torch.bfloat16)
+        out, lse = c.attend(q.cuda(), c.batch([count]), "bf16", scale=0.3 / size, chunk=1)
+        torch.cuda.synchronize()
+        check(out, lse, ko.attention(q.double().numpy(), kq, vq, [n - count + t for t in range(count)], 0.3 / size, 1, -1), "bf16")
+
+
+def test_attention_beyond_32_bits():
+    """A pool of over 4 GiB: pages at its end are found."""
+    n_pages = (1 << 32) // (16 * 16 * 72) + 2000
+    c = Cache(layers=1, n_pages=n_pages, n_seq=1, max_pages=8, heads=16, fill=-1)
+    c.refs[: n_pages - 6] = 1
+    (k, v), = c.fill([83], seed=3)
+    assert int(c.table[0, 0]) == n_pages - 6
+    q = torch.randn(2, 16, 64, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    out, lse = c.attend(q.cuda(), c.batch([2]), "bf16", chunk=1)
+    torch.cuda.synchronize()
+    check(out, lse, ko.attention(q.double().numpy(), k, v, [81, 82], 0.125, 1, -1), "bf16")
+
+
+def test_calls_on_other_streams_and_in_graphs():
+    """Two graphs of calls on the same cache, replayed at once on two streams with new inputs, give what plain calls
+    give; so does a call on a stream that is not the current one."""
+    c = Cache(n_pages=200, n_seq=6, max_pages=90, heads=4, dim=128, group=64)
+    c.fill([700, 33, 1200, 5, 64, 90], seed=2)
+    g = torch.Generator("cuda").manual_seed(4)
+    qs = [torch.randn(6, 16, 128, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2)]
+    outs = [torch.zeros_like(q) for q in qs]
+    rows = c.batch([1] * 6)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    for s, q, o in zip(streams, qs, outs):
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            for _ in range(4):
+                c.attend(q, rows, "bf16", chunk=1, lse=False, out=o, max_len=1200, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(graph)
+    for _ in range(3):
+        for q in qs:
+            q.copy_(torch.randn(q.shape, device="cuda", generator=g))
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for q, o in zip(qs, outs):
+            want, _ = c.attend(q, rows, "bf16", chunk=1, max_len=1200)
+            torch.cuda.synchronize()
+            assert torch.equal(o, want)
+    other, _ = c.attend(qs[0], rows, "bf16", chunk=1, max_len=1200, stream=streams[1].cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(other, outs[0])
+
+
+# ---------------------------------------------------------------------------
+# pages
+# ---------------------------------------------------------------------------
+class Both:
+    """A cache and the oracle's pages, driven alike.  A page's content in the oracle is its bytes in every layer."""
+
+    def __init__(self, n_pages, n_seq, max_pages, page=16, layers=3, heads=1, seed=0):
+        self.c = Cache(layers=layers, n_pages=n_pages, n_seq=n_seq, max_pages=max_pages, heads=heads, page=page)
+        self.o = ko.Pages(n_pages, n_seq, max_pages, page)
+        self.o.data = [self.c.bytes()[:, p].cpu().numpy().tobytes() for p in range(n_pages)]
+
+    def extend(self, seqs, counts):
+        got = self.c.grow(seqs, counts)
+        torch.cuda.synchronize()
+        assert got.tolist() == self.o.extend(seqs, counts)
+        self.same()
+
+    def do(self, what, a, b):
+        self.c.pairs(what, a, b)
+        getattr(self.o, what)(a, b)
+        self.same()
+
+    def compact(self):
+        used = i32([-1])
+        self.c.c.compact(used.data_ptr())
+        torch.cuda.synchronize()
+        assert used.item() == self.o.compact()
+        self.same()
+
+    def same(self):
+        assert self.c.lengths.tolist() == self.o.length
+        assert self.c.table.tolist() == self.o.table
+        assert self.c.refs.tolist() == self.o.refs
+        assert self.c.c.status() == self.o.error
+        self.o.error = 0
+        data = self.c.bytes().cpu().numpy()
+        for p in range(self.o.n_pages):
+            assert data[:, p].tobytes() == self.o.data[p], p
+
+
+def test_pages_by_hand():
+    b = Both(n_pages=20, n_seq=8, max_pages=6)
+    b.extend([0, 2, 5], [17, 0, 32])
+    b.extend([0, 2], [14, 1])             # up to the last place of a page
+    b.extend([0], [1])                    # and over it
+    b.do("fork", [0, 5], [1, 3])
+    b.extend([1, 3, 0], [1, 1, 1])        # the shared partial page is copied; the full one is not; the last owner needs no copy
+    b.do("fork", [2, 2], [4, 6])
+    b.extend([4, 6], [2, 2])              # both leave the page they shared
+    b.do("free", [0, 1], [16, 0])
+    b.compact()
+    b.do("copy", [5, 3], [0, 1])          # 0 is not empty; 1 is
+    b.do("free", [0, 0, 5, 3, 3], [9, 3, 99, 33, 32])
+    b.compact()
+    b.compact()                           # nothing to move
+    b.do("free", list(range(8)), [0] * 8)
+    b.compact()
+
+
+def test_pages_refusals():
+    b = Both(n_pages=8, n_seq=5, max_pages=4)
+    b.extend([0, 7, -1, 1, 1, 2], [20, 3, 3, 5, 6, -2])   # bad slots, one twice, a negative count
+    b.extend([0], [60])                                   # wider than the table
+    b.extend([2, 3, 4], [60, 40, 1])                      # 4 + 3 + 1 of 5 free pages: the first alone fits
+    b.extend([3], [16])
+    b.extend([4], [1])                                    # the pool is full
+    b.do("fork", [0, 0, 9, 1], [4, 4, 3, 9])              # twice the same; bad slots
+    b.do("copy", [0], [0])                                # not empty
+    b.do("free", [0, 9, 1], [-1, 0, 0])
+    b.do("fork", [4], [0])                                # not empty
+    b.do("free", [4, 2], [0, 0])
+    b.do("copy", [0, 3, 2], [2, 4, 1])                    # copies, and an empty one; 2 was empty before the call
+    b.do("copy", [0, 3], [1, 1])
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_pages_at_random(seed):
+    rng = np.random.default_rng(seed)
+    page = int(rng.choice([16, 32, 64]))
+    n_seq = 12
+    b = Both(n_pages=int(rng.integers(20, 60)), n_seq=n_seq, max_pages=9, page=page, layers=2, heads=2)
+    for _ in range(40):
+        n = int(rng.integers(1, 8))
+        what = rng.choice(["extend", "extend", "fork", "copy", "free", "compact"])
+        a, c = rng.integers(0, n_seq, n).tolist(), rng.integers(0, n_seq, n).tolist()
+        if what == "extend":
+            b.extend(a, rng.integers(0, 2 * page, n).tolist())
+        elif what == "compact":
+            b.compact()
+        elif what == "free":
+            b.do("free", a, rng.integers(0, 5 * page, n).tolist() if rng.random() < 0.5 else [0] * n)
+        else:
+            b.do(str(what), a, c)
+
+
+def test_pages_many():
+    """More pages and entries than one sweep of the planning kernel takes."""
+    n_pages, n_seq = 9001, 4096
+    b = Both(n_pages=n_pages, n_seq=2 * n_seq + 1, max_pages=3, layers=1)
+    rng = np.random.default_rng(1)
+    order = rng.permutation(n_seq).tolist()
+    b.extend(order, rng.integers(0, 33, n_seq).tolist())
+    b.do("fork", order, [n_seq + s for s in order])
+    b.do("free", order[::2], [0] * len(order[::2]))
+    b.do("free", [n_seq + s for s in order[:1000]], [5] * 1000)
+    b.extend([n_seq + s for s in order], [3] * n_seq)
+    b.compact()
+    b.do("free", order, [0] * n_seq)
+    b.do("copy", [n_seq + s for s in order[:300]], order[:300])
+    b.compact()
+
+
+def test_generation_end_to_end():
+    """As a program uses them: prompts in, a step of single tokens, a fork that goes its own way, streams that end,
+    a compaction, and another step; attention against the rows that each sequence should hold."""
+    heads, per, dim, page = 2, 3, 64, 16
+    c = Cache(layers=2, n_pages=30, n_seq=4, max_pages=8, heads=heads, dim=dim, page=page)
+    g = torch.Generator().manual_seed(6)
+    mine = {s: [] for s in range(4)}
+
+    def step(seqs, counts):
+        start = c.grow(seqs, counts)
+        rows = c.batch(counts, seqs=seqs, start=start)
+        n = sum(counts)
+        q = torch.randn(n, heads * per, dim, generator=g).to(torch.bfloat16)
+        for layer in range(2):
+            k, v = (torch.randn(n, heads, dim, generator=g).to(torch.bfloat16) for _ in range(2))
+            c.write(k.cuda(), v.cuda(), rows, "bf16", layer=layer)
+            out, lse = c.attend(q.cuda(), rows, "bf16", chunk=1, layer=layer)
+            torch.cuda.synchronize()
+            if layer == 0:
+                continue
+            at = 0
+            for s, m in zip(seqs, counts):
+                mine[s].append((k[at:at + m].float().numpy(), v[at:at + m].float().numpy()))
+                kk, vv = (ko.quantise(np.concatenate([x[i] for x in mine[s]]), 64).astype(np.float64) for i in (0, 1))
+                want = ko.attention(q[at:at + m].double().numpy(), kk, vv, [len(kk) - m + t for t in range(m)], 0.125, 1, -1)
+                check(out[at:at + m], lse[at:at + m], want, "bf16")
+                at += m
+
+    def cut(s, keep):
+        kk, vv = (np.concatenate([x[i] for x in mine[s]])[:keep] for i in (0, 1))
+        mine[s] = [(kk, vv)]
+
+    step([0, 1, 2], [40, 7, 33])
+    step([2, 0, 1], [1, 1, 1])
+    c.pairs("fork", [0], [3])
+    mine[3] = list(mine[0])
+    step([0, 3, 2, 1], [1, 1, 1, 1])
+    c.pairs("free", [1, 0], [0, 20])
+    mine[1] = []
+    cut(0, 20)
+    used = i32([0])
+    c.c.compact(used.data_ptr())
+    step([0, 1, 2, 3], [1, 18, 1, 2])
+    c.pairs("free", [0], [0])
+    c.pairs("copy", [3], [0])
+    mine[0] = list(mine[3])
+    step([0, 3], [30, 1])
+    assert c.c.status() == 0
