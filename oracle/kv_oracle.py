@@ -68,6 +68,12 @@ def quantise(x, group):
     return out.reshape(x.shape)
 
 
+def steps(x, group):
+    """[..., dim] -> the step s of each value's group, in float64."""
+    flat = np.asarray(x, np.float32).reshape(-1, group)
+    return np.repeat([float(quantise_group(row)[1]) for row in flat], group).reshape(np.shape(x))
+
+
 def unpack_block(block, dim, group):
     """The bytes of one block -> K and V values [16, dim] in float64, by the places the header gives."""
     block = np.asarray(block, np.uint8)
@@ -95,14 +101,15 @@ def visible(p: int, length: int, chunk: int, left: int):
     return (max(0, begin - left) if left >= 0 else 0), min(length, begin + chunk)
 
 
-def attention(q, k, v, positions, scale, chunk, left, seen=None):
-    """q [rows, heads, dim], k and v [keys, kv heads, dim] in float64.  Returns
-    out, lse, and the bound's parts: the largest sum of |q| |k| scale over the visible keys
-    of each (row, head), and the weighted sum of |v| per output.  `seen`: keys that exist (bool), default all."""
+def attention(q, k, v, step, positions, scale, chunk, left, seen=None):
+    """q [rows, heads, dim], k and v [keys, kv heads, dim] in float64; step: those of v's groups.  Returns
+    out, lse, and parts of a bound: the largest sum of |q| |k| scale over the visible keys of each (row, head);
+    per output the weighted sums of |v| and of 8 steps, and the keys times the largest step.
+    `seen`: keys that exist (bool), default all."""
     rows, heads, dim = q.shape
     per = heads // k.shape[1]
     out, lse = np.zeros(q.shape), np.full((rows, heads), -np.inf)
-    size, weight = np.zeros((rows, heads)), np.zeros(q.shape)
+    size, weight, coarse, most = np.zeros((rows, heads)), np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape)
     for r, p in enumerate(positions):
         lo, hi = visible(p, k.shape[0], chunk, left)
         at = np.arange(lo, max(lo, hi))
@@ -120,7 +127,9 @@ def attention(q, k, v, positions, scale, chunk, left, seen=None):
             out[r, h] = w @ vv
             size[r, h] = (np.abs(kk) @ np.abs(q[r, h])).max() * abs(scale)
             weight[r, h] = w @ np.abs(vv)
-    return out, lse, size, weight
+            coarse[r, h] = w @ step[at, h // per] * 8
+            most[r, h] = at.size * step[at, h // per].max(0)
+    return out, lse, size, weight, coarse, most
 
 
 class Pages:

@@ -1,12 +1,17 @@
 """The paged 4-bit cache on the GPU, through the C ABI, against oracle/kv_oracle.py
 (exact quantising, attention in float64, pages as plain lists).
 
-Attention's bound, per output: its rounding, half a step of the type
-(2^-8 relative in bf16, 2^-11 in fp16), plus 2^-10 of the weighted sum of |v| for the
-probabilities' rounding to fp16 (half a step is 2^-11, once in the numerator; the
-denominator is not rounded), plus the effect of the scores' error: a score is a sum in fp32 of
-at most 2 * 128 terms, each off by at most a few 2^-24, so it is off by at most dS = 2^-16 times the sum of
-|q| |k| scale (256 * 2^-24), and 2^-18 for the exponential's own error; weights then move by at most 2 dS relative.
+Attention's bound, per output:
+  * its rounding, half a step of the type: 2^-8 relative in bf16, 2^-11 in fp16;
+  * the probabilities' rounding to fp16.  A value is held as v = s c + m = s (c - 8) + (m + 8 s), and its first
+    part is multiplied by fp16(p s): off by 2^-11 p s |c - 8| <= 2^-11 p 8 s a key, so by 2^-11 of the weighted sum
+    of 8 s (not of |v|, which is smaller where s (c - 8) and m + 8 s have opposite signs).  Below the fp16 range
+    p s is off by 2^-25 absolute, where the largest step seen is scaled to over 2^10: 2^-35 of it a key, times
+    |c - 8| <= 8, over a denominator of at least 1: 2^-32 of the keys times the largest step;
+  * the scores' error: a score is a sum in fp32 of at most 2 * 128 terms, each off by at most a few 2^-24, so it
+    is off by at most dS = 2^-16 (256 * 2^-24) times the sum of |q| |k| scale, and 2^-18 for the exponential's own
+    error; weights then move by at most 2 dS relative, and the output by that of the weighted sum of |v| + 8 s
+    (both parts are summed).
 lse moves by at most dS + 2^-20 + 2^-22 |lse|."""
 
 import numpy as np
@@ -82,7 +87,7 @@ class Cache:
         return k, v
 
     def fill(self, lengths, seed=0, layer=0, scale=1.0):
-        """Grow all slots to `lengths` and write random rows; the values they read as, per slot, in float64."""
+        """Grow all slots to `lengths` and write random rows; per slot the values they read as and V's steps, in float64."""
         g = torch.Generator().manual_seed(seed)
         start = self.grow(list(range(len(lengths))), lengths)
         k = torch.randn(sum(lengths), self.heads, self.dim, generator=g) * scale + torch.randn(self.heads, self.dim, generator=g)
@@ -93,8 +98,9 @@ class Cache:
             self.write(kd, vd, rows, "fp32", layer=layer)
         torch.cuda.synchronize()
         kq, vq = (ko.quantise(x.numpy(), self.group).astype(np.float64) for x in (k, v))
+        steps = ko.steps(v.numpy(), self.group)
         at = np.cumsum([0] + list(lengths))
-        return [(kq[a:b], vq[a:b]) for a, b in zip(at, at[1:])]
+        return [(kq[a:b], vq[a:b], steps[a:b]) for a, b in zip(at, at[1:])]
 
     def attend(self, q, rows, dtype, scale=0.125, chunk=0, left=-1, layer=0, max_len=0, lse=True, out=None, **kw):
         heads = q.shape[1]
@@ -106,11 +112,11 @@ class Cache:
 
 
 def check(out, lse, want, dtype):
-    """`want`: (out, lse, size, weight) of ko.attention."""
-    ref, rl, size, weight = want
+    """`want`: what ko.attention returns."""
+    ref, rl, size, weight, coarse, most = want
     out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
     ds = 2.0 ** -16 * size + 2.0 ** -18
-    tol = HALF[dtype] * np.abs(ref) + (2.0 ** -10 + 2 * ds[..., None]) * weight + 2.0 ** -25
+    tol = HALF[dtype] * np.abs(ref) + 2.0 ** -11 * coarse + 2.0 ** -32 * most + 2 * ds[..., None] * (weight + coarse)
     bad = np.abs(out - ref) > tol
     assert np.isfinite(out).all() and not bad.any(), (np.argwhere(bad)[:4], np.abs(out - ref).max())
     none = np.isinf(rl)
@@ -153,7 +159,7 @@ def test_write_read(dim, group, page, dtype):
 def test_layout_is_the_documented_one():
     for dim, group in ((64, 64), (64, 32), (128, 64), (128, 32)):
         c = Cache(n_pages=3, n_seq=1, max_pages=2, heads=2, dim=dim, group=group, page=32)
-        (k, v), = c.fill([45], seed=dim + group)
+        (k, v, _), = c.fill([45], seed=dim + group)
         table = c.table.cpu().numpy()[0]
         data = c.bytes().cpu().numpy()
         for b in range(3):
@@ -318,9 +324,9 @@ def test_attention(case, dtype):
     torch.cuda.synchronize()
     assert c.c.status() == 0
     at = 0
-    for (k, v), n in zip(held, counts):
+    for (k, v, st), n in zip(held, counts):
         pos = [len(k) - n + t for t in range(n)]
-        want = ko.attention(q[at:at + n].double().numpy(), k, v, pos, dim ** -0.5, chunk, left)
+        want = ko.attention(q[at:at + n].double().numpy(), k, v, st, pos, dim ** -0.5, chunk, left)
         check(out[at:at + n], lse[at:at + n], want, dtype)
         at += n
 
@@ -330,9 +336,9 @@ def test_attention(case, dtype):
 def test_attention_long(length, dim, per):
     """One row over growing lengths, with a bound of the length that is right, far too large, or absent."""
     c = Cache(n_pages=300, n_seq=2, max_pages=280, heads=2, dim=dim, group=64, page=16)
-    (k, v), _ = c.fill([length, 0], seed=length)
+    (k, v, st), _ = c.fill([length, 0], seed=length)
     q = torch.randn(1, 2 * per, dim, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
-    want = ko.attention(q.double().numpy(), k, v, [length - 1], 0.1, 1, -1)
+    want = ko.attention(q.double().numpy(), k, v, st, [length - 1], 0.1, 1, -1)
     got = []
     for most in (0, length, 1, 280 * 16):
         out, lse = c.attend(q.cuda(), c.batch([1]), "bf16", scale=0.1, chunk=1, max_len=most)
@@ -360,8 +366,8 @@ def test_attention_options():
     assert (out[8] == 3).all() and (out[:, 0] == 3).all() and (out[:, 5] == 3).all()
     assert (out[:, :, :5] == 3).all() and (out[:, :, 69:] == 3).all()
     for i in range(4):
-        k, v = held[seqs[i]]
-        want = ko.attention(q[2 * i:2 * i + 2].double().cpu().numpy(), k, v, [pos[i], pos[i] + 1], 0.2, 10, 15)
+        k, v, st = held[seqs[i]]
+        want = ko.attention(q[2 * i:2 * i + 2].double().cpu().numpy(), k, v, st, [pos[i], pos[i] + 1], 0.2, 10, 15)
         lse = torch.from_numpy(want[1])
         check(out[2 * i:2 * i + 2, 1:5, 5:69], lse, want, "fp16")
     # entries that were not served, and bad slots: zeros
@@ -375,7 +381,7 @@ def test_attention_values_that_must_not_matter():
     """NaN in keys behind the end, behind the chunk and before the window, and in pages of nobody: no effect; in a key
     that is seen: NaN, in V only in the channels of its group.  Pages outside the pool are not seen."""
     c = Cache(n_pages=12, n_seq=2, max_pages=6, heads=1, dim=64, group=32, fill=0xFF)  # NaN everywhere
-    (k, v), _ = c.fill([70, 0], seed=1)
+    (k, v, st), _ = c.fill([70, 0], seed=1)
     q = torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
     bad = torch.full((1, 1, 64), float("nan"), device="cuda")
     for at in (5, 69):  # one key before the window, one behind the chunk
@@ -383,7 +389,7 @@ def test_attention_values_that_must_not_matter():
     rows = c.batch([3], start=[40])
     out, lse = c.attend(q.cuda(), rows, "bf16", chunk=20, left=25)
     torch.cuda.synchronize()
-    check(out, lse, ko.attention(q.double().numpy(), k, v, [40, 41, 42], 0.125, 20, 25), "bf16")
+    check(out, lse, ko.attention(q.double().numpy(), k, v, st, [40, 41, 42], 0.125, 20, 25), "bf16")
     out, lse = c.attend(q.cuda(), rows, "bf16", chunk=0)
     torch.cuda.synchronize()
     assert torch.isnan(out).all() and torch.isnan(lse).all()
@@ -407,7 +413,7 @@ def test_attention_values_that_must_not_matter():
     c.table.copy_(table)
     got_k, got_v = c.read(c.batch([70], start=[0]), 70)
     kk, vv = got_k.double().cpu().numpy(), got_v.double().cpu().numpy()
-    want = ko.attention(q.double().numpy(), kk, vv, [40, 41, 42], 0.125, 60, 0, seen=seen | (np.arange(70) == 5))
+    want = ko.attention(q.double().numpy(), kk, vv, st, [40, 41, 42], 0.125, 60, 0, seen=seen | (np.arange(70) == 5))
     ok = torch.isfinite(torch.from_numpy(want[0]))
     assert torch.equal(torch.isfinite(out.cpu()), ok)
     check(out[..., :32], lse, tuple(x[..., :32] if x.ndim == 3 else x for x in want), "bf16")
@@ -437,7 +443,7 @@ def test_attention_ranges(dim, count):
         q = (q.float() * size).to(torch.bfloat16)
         out, lse = c.attend(q.cuda(), c.batch([count]), "bf16", scale=0.3 / size, chunk=1)
         torch.cuda.synchronize()
-        check(out, lse, ko.attention(q.double().numpy(), kq, vq, [n - count + t for t in range(count)], 0.3 / size, 1, -1), "bf16")
+        check(out, lse, ko.attention(q.double().numpy(), kq, vq, ko.steps(v.numpy(), 64), [n - count + t for t in range(count)], 0.3 / size, 1, -1), "bf16")
 
 
 def test_attention_beyond_32_bits():
@@ -445,12 +451,12 @@ def test_attention_beyond_32_bits():
     n_pages = (1 << 32) // (16 * 16 * 72) + 2000
     c = Cache(layers=1, n_pages=n_pages, n_seq=1, max_pages=8, heads=16, fill=-1)
     c.refs[: n_pages - 6] = 1
-    (k, v), = c.fill([83], seed=3)
+    (k, v, st), = c.fill([83], seed=3)
     assert int(c.table[0, 0]) == n_pages - 6
     q = torch.randn(2, 16, 64, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
     out, lse = c.attend(q.cuda(), c.batch([2]), "bf16", chunk=1)
     torch.cuda.synchronize()
-    check(out, lse, ko.attention(q.double().numpy(), k, v, [81, 82], 0.125, 1, -1), "bf16")
+    check(out, lse, ko.attention(q.double().numpy(), k, v, st, [81, 82], 0.125, 1, -1), "bf16")
 
 
 def test_calls_on_other_streams_and_in_graphs():
@@ -624,7 +630,8 @@ def test_generation_end_to_end():
             for s, m in zip(seqs, counts):
                 mine[s].append((k[at:at + m].float().numpy(), v[at:at + m].float().numpy()))
                 kk, vv = (ko.quantise(np.concatenate([x[i] for x in mine[s]]), 64).astype(np.float64) for i in (0, 1))
-                want = ko.attention(q[at:at + m].double().numpy(), kk, vv, [len(kk) - m + t for t in range(m)], 0.125, 1, -1)
+                st = ko.steps(np.concatenate([x[1] for x in mine[s]]), 64)
+                want = ko.attention(q[at:at + m].double().numpy(), kk, vv, st, [len(kk) - m + t for t in range(m)], 0.125, 1, -1)
                 check(out[at:at + m], lse[at:at + m], want, "bf16")
                 at += m
 
