@@ -5,29 +5,31 @@
 // number is the subnormal c 2^-24 (16 c 2^-24 four bits further up), which the
 // instruction multiplies exactly, so one AND makes two operands.  The steps and
 // minima stay outside, in fp32: with k = c s + m per group of channels
-//   q . k = s (q . c) + m sum(q)          (a scale per key, on the scores)
-//   sum_j p_j v_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j)  (a scale per key, on P)
-// (The codes are centred for V because p s is rounded to fp16, which must not be
+//   q . k = s (q . c) + m sum(q)                         (a scale per key, on the scores)
+//   sum_j p_j v_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j)   (a scale per key, on P)
+// The codes are centred for V because p s is rounded to fp16, which must not be
 // multiplied by more than half the group's range: the product takes c, and a
 // product with the constant 8 takes off what the centring needs, of the same
-// rounded values.)
-// q is scaled by a power of two so that its largest value is near 2^13 (an
-// fp16 operand: what is lost is below 2^-38 of that); p s is scaled by a power
-// of two F per group of channels that keeps it below 2^15 for the largest
-// step seen so far and the largest p (2^4, see below), so that what fp16
-// rounds away is 2^-11 of each term, or 2^-36 of the largest.
+// rounded values.  q is scaled by a power of two so that the largest value of
+// the rows is near 2^13 (what fp16 loses is below 2^-38 of that).  p is taken times a
+// power of two F that brings the largest step of V so far to 2^11: p s F stays
+// below 2^15, and what fp16 rounds away is 2^-11 of each term, or 2^-36 of
+// the largest.  F cancels in the quotient.
 //
-// A warp holds 16 rows (query rows x heads of one kv head) and walks the keys
-// 32 at a time with a running maximum, sum and output in registers.  The maximum is raised, and the
-// sums rescaled, only when a score exceeds it by 4 (log2 units): p <= 2^4.
-// MW warps of a CTA hold different rows and share the keys' bytes, KW such
-// groups split the CTA's keys, and a cluster of CTAs splits the keys of long
-// sequences; they are joined through shared memory, in a fixed order.  The
-// bytes come through rings of cp.async stages.
+// The maximum is raised, and the sums rescaled, only when a score exceeds it by
+// 4 (log2 units), so p <= 2^4; likewise F only when a step exceeds its bound.
+//
+// Two forms, by the rows (query rows x query heads of one kv head) of an entry:
+// k_kv_few for up to 16, whose warps all split the keys, and k_kv_many, whose warps
+// share the keys' bytes.  In both a cluster of CTAs splits the keys of long
+// sequences, joined through shared memory in a fixed order: no workspace in
+// global memory, so calls may overlap.  The bytes come through rings of
+// cp.async stages.
 #include <cooperative_groups.h>
 
 #include <cmath>
 
+#include "common.cuh"
 #include "kv.cuh"
 
 namespace cg = cooperative_groups;
@@ -38,8 +40,11 @@ namespace {
 
 constexpr int UNIT = 32;  // keys of a step: two blocks
 constexpr uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u;
-constexpr float RAISE = 4.0f;        // log2 units by which a score may exceed the running maximum
-constexpr float P_TOP = 2048.0f;     // F x the largest step: 2^4 x 2^11 stays below 2^15
+constexpr uint32_t EIGHTS = 0x00080008u;
+constexpr float RAISE = 4.0f;         // log2 units by which a score may exceed the running maximum
+constexpr int P_TOP = 11;             // F x the largest step is 2^11 at most: 2^4 x 2^11 stays below 2^15
+constexpr float STEP_MIN = 8.0779357e-28f;  // 2^-90: F stays below 2^101, so that sums of p F do not overflow
+constexpr float STEP_MAX = 8.5070592e37f;   // 2^126
 
 struct Mask {
   int chunk, left;
@@ -48,8 +53,11 @@ struct Mask {
     lo = 0;
     hi = len;
     if (chunk > 0) {
-      int at = p / chunk;
-      if (p < 0 && at * chunk != p) --at;  // rounds down
+      int at = p;
+      if (chunk > 1) {
+        at = p / chunk;
+        if (p < 0 && at * chunk != p) --at;  // rounds down
+      }
       const long long begin = static_cast<long long>(at) * chunk;
       hi = static_cast<int>(max(0ll, min(static_cast<long long>(len), begin + chunk)));
       if (left >= 0) lo = static_cast<int>(max(0ll, begin - left));
@@ -57,11 +65,27 @@ struct Mask {
   }
 };
 
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// d += a b, or d = a b
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// An 8 x 8 matrix of 16-bit elements, row lane / 4, columns 2 (lane % 4) + {0, 1}, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -80,385 +104,510 @@ __device__ __forceinline__ void cp_async_wait() {
 }
 
 __device__ __forceinline__ uint4 lds128(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ uint32_t lds32(const void* p) { return *reinterpret_cast<const uint32_t*>(p); }
 
-// Steps and minima of two neighbouring keys from their parameter words.
-__device__ __forceinline__ float2 steps(uint32_t a, uint32_t b) {
-  return make_float2(__uint_as_float(a << 16), __uint_as_float(b << 16));
-}
-__device__ __forceinline__ float2 minima(uint32_t a, uint32_t b) {
-  return make_float2(__uint_as_float(a & 0xFFFF0000u), __uint_as_float(b & 0xFFFF0000u));
-}
+// Step and minimum of a parameter word.
+__device__ __forceinline__ float step_of(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float low_of(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ uint32_t half_pair(float2 x) {
+  const __half2 h = __float22half2_rn(x);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-template <int DIM, int GROUP, int MW, int KW>
-struct Shape {
-  static constexpr int THREADS = 32 * MW * KW;
+// The power of two at or above a step (its exponent), within the bounds of F.
+__device__ __forceinline__ int step_exponent(float v) {
+  const uint32_t bits = __float_as_uint(fminf(fmaxf(v, STEP_MIN), STEP_MAX)) + 0x7FFFFFu;
+  return static_cast<int>(bits >> 23) - 127;
+}
+
+struct Args {
+  lx_kv_cache c;
+  lx_kv_rows r;
+  int layer, q_heads, per, tiles, split, block_lg;  // block_lg: log2 of the blocks of a page
+  const void* q;
+  int64_t q_row, q_head;
+  bool wide;
+  void* out;
+  int64_t o_row, o_head;
+  float* lse;
+  float scale;
+  Mask mask;
+};
+
+// Eight neighbouring channels of the query.
+template <typename T>
+__device__ __forceinline__ void query8(const T* p, bool wide, float (&x)[8]) {
+  if (wide) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const T* t = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(p[i]);
+  }
+}
+
+// The exponent by which the rows are scaled: 2^e times their largest finite value lies in [2^13, 2^14).
+__device__ __forceinline__ int query_exponent(float top) {
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+  return top > 0.0f ? min(max(13 - e, -110), 110) : 0;
+}
+
+// One CTA's share of an entry's rows and keys.
+struct Share {
+  Entry e;
+  int head, row0, n_rows, rows, len, start, rank;
+  // the rows of the CTA are rows row0 .. row0 + n_rows - 1 of the entry's (query row, query head) pairs
+  __device__ __forceinline__ bool take(const Args& a, int tile_rows) {
+    rank = blockIdx.x % a.split;
+    int item = blockIdx.x / a.split;
+    head = item % a.c.kv_heads;
+    item /= a.c.kv_heads;
+    const int tile = item % a.tiles, entry = item / a.tiles;
+    e = entry_of(a.c, a.r, entry);
+    rows = e.rows * a.per;
+    row0 = tile * tile_rows;
+    if (row0 >= rows) return false;  // for the whole cluster
+    n_rows = min(tile_rows, rows - row0);
+    len = 0;
+    start = LX_KV_REFUSED;
+    if (e.slot >= 0) {
+      len = length_of(a.c, e.slot);
+      start = start_of(a.r, entry, len, e.rows);
+    }
+    return true;
+  }
+  // keys that row `row` (behind the last one: the last one) of the CTA sees
+  __device__ __forceinline__ void range(const Args& a, int row, int& lo, int& hi) const {
+    lo = hi = 0;
+    if (start != LX_KV_REFUSED) a.mask.range(start + (row0 + min(row, n_rows - 1)) / a.per, len, lo, hi);
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* query(const Args& a, int row) const {
+    const int x = row0 + min(row, n_rows - 1), t = x / a.per;
+    return static_cast<const T*>(a.q) + (e.row0 + t) * a.q_row + (head * a.per + (x - t * a.per)) * a.q_head;
+  }
+};
+
+// The ring through which THREADS threads bring the blocks of units unit, unit + STRIDE, ... below
+// the end into shared memory, STAGES - 1 units ahead.
+template <int BB, int STAGES, int STRIDE, int THREADS>
+struct Ring {
+  const int32_t* table;
+  const uint8_t* base;  // of the layer and head, in page 0
+  uint32_t page_bytes;  // from a page to the next, the same layer and head
+  int n_pages, block_lg, tid;
+  uint32_t smem;        // this ring's first stage
+  int next, n_blocks;   // next unit to load; blocks below this one exist
+  int page[2];          // of its blocks, looked up one unit ahead; -2: no such block
+  uint32_t got;         // two bits a loaded unit, the last in the lowest place: which blocks are there
+  int* error;
+
+  __device__ __forceinline__ void look_up() {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) page[b] = 2 * next + b < n_blocks ? table[(2 * next + b) >> block_lg] : -2;
+  }
+  __device__ __forceinline__ void load(int stage) {
+    got <<= 2;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (static_cast<uint32_t>(page[b]) < static_cast<uint32_t>(n_pages)) {
+        got |= 1u << b;
+        const int in_page = (2 * next + b) & ((1 << block_lg) - 1);
+        const uint8_t* src = base + static_cast<uint64_t>(static_cast<uint32_t>(page[b])) * page_bytes +
+                             (in_page * BB + 16 * tid);
+        const uint32_t dst = smem + (2 * stage + b) * BB + 16 * tid;
+#pragma unroll
+        for (int x = 0; x < (BB / 16 + THREADS - 1) / THREADS; ++x)
+          if (BB / 16 >= THREADS * (x + 1) || tid + THREADS * x < BB / 16)
+            cp_async16(dst + 16 * THREADS * x, src + 16 * THREADS * x);
+      } else if (page[b] != -2 && tid == 0) {
+        atomicOr(error, LX_KV_PAGE);
+      }
+    }
+    cp_async_commit();
+    next += STRIDE;
+    look_up();
+  }
+  __device__ __forceinline__ void start(const Args& a, const Share& s, int unit, int unit_end, int hi, uint8_t* stages,
+                                        int thread) {
+    table = a.c.table + static_cast<size_t>(s.e.slot < 0 ? 0 : s.e.slot) * a.c.max_pages;
+    const uint32_t head_bytes = static_cast<uint32_t>(BB) << a.block_lg;
+    page_bytes = head_bytes * a.c.kv_heads;
+    base = static_cast<const uint8_t*>(a.c.pool) +
+           (static_cast<uint64_t>(a.layer) * a.c.n_pages * a.c.kv_heads + s.head) * head_bytes;
+    n_pages = a.c.n_pages;
+    block_lg = a.block_lg;
+    tid = thread;
+    smem = smem_u32(stages);
+    next = unit;
+    n_blocks = min(2 * unit_end, (hi + BLOCK - 1) / BLOCK);
+    got = 0;
+    error = a.c.error;
+    look_up();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) load(i);
+  }
+};
+
+// The units [first, last) of this CTA for keys [lo, hi) of its rows.
+__device__ __forceinline__ void share_units(int lo, int hi, int rank, int split, int& first, int& last) {
+  first = last = 0;
+  if (hi > lo) {
+    const int u = lo / UNIT, count = (hi + UNIT - 1) / UNIT - u;
+    first = u + static_cast<int>(static_cast<long long>(count) * rank / split);
+    last = u + static_cast<int>(static_cast<long long>(count) * (rank + 1) / split);
+  }
+}
+
+// Joins the parts of KW key groups, and of the CTAs of the cluster, and writes
+// the rows.  A part is O [rows][DIM] and, per row, the maximum and the sum.
+template <typename T, int DIM, int KW, int ROWS, int THREADS>
+__device__ __forceinline__ void join(const Args& a, const Share& s, float* part_o, float* part_m, float* part_l) {
+  float* cta_o = part_o + (KW > 1 ? KW * ROWS * DIM : 0);
+  float* cta_m = part_m + (KW > 1 ? KW * ROWS : 0);
+  float* cta_l = part_l + (KW > 1 ? KW * ROWS : 0);
+  if (KW > 1) {
+    for (int x = threadIdx.x; x < s.n_rows * DIM; x += THREADS) {
+      const int row = x / DIM;
+      float top = part_m[row];
+#pragma unroll
+      for (int k = 1; k < KW; ++k) top = fmaxf(top, part_m[k * ROWS + row]);
+      float o = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const float mk = part_m[k * ROWS + row];
+        const float f = mk == top ? 1.0f : ex2(mk - top);
+        o = fmaf(part_o[k * ROWS * DIM + x], f, o);
+        sum = fmaf(part_l[k * ROWS + row], f, sum);
+      }
+      cta_o[x] = o;
+      if (x % DIM == 0) {
+        cta_m[row] = top;
+        cta_l[row] = sum;
+      }
+    }
+  }
+  if (a.split > 1)
+    cg::this_cluster().sync();
+  else
+    __syncthreads();
+  for (int x = threadIdx.x + s.rank * THREADS; x < s.n_rows * DIM; x += a.split * THREADS) {
+    const int row = x / DIM, d = x % DIM;
+    float top = cta_m[row], o = cta_o[x], sum = cta_l[row];
+    if (a.split > 1) {
+      top = -INFINITY;
+      for (int k = 0; k < a.split; ++k) top = fmaxf(top, *cg::this_cluster().map_shared_rank(cta_m + row, k));
+      o = sum = 0.0f;
+      for (int k = 0; k < a.split; ++k) {
+        const float mk = *cg::this_cluster().map_shared_rank(cta_m + row, k);
+        const float f = mk == top ? 1.0f : ex2(mk - top);
+        o = fmaf(*cg::this_cluster().map_shared_rank(cta_o + x, k), f, o);
+        sum = fmaf(*cg::this_cluster().map_shared_rank(cta_l + row, k), f, sum);
+      }
+    }
+    const int t = (s.row0 + row) / a.per, h = s.head * a.per + (s.row0 + row - t * a.per);
+    static_cast<T*>(a.out)[(s.e.row0 + t) * a.o_row + h * a.o_head + d] =
+        static_cast<T>(sum == 0.0f ? 0.0f : o / sum);
+    if (a.lse && d == 0)
+      a.lse[static_cast<int64_t>(s.e.row0 + t) * a.q_heads + h] =
+          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  }
+  if (a.split > 1) cg::this_cluster().sync();  // nobody leaves while its part may be read
+}
+
+// ---------------------------------------------------------------------------
+// few rows: up to 8 NT, the keys on the long side of the matrix instruction
+// ---------------------------------------------------------------------------
+// Both products are turned over: S^T = K q^T takes the codes of 16 keys as the
+// 16-row operand and 8 query rows as the other, O^T = V^T P^T 16 channels
+// and 8 rows.  Against rows on the long side (16, most of them empty in a step of
+// single tokens) this halves the instructions of everything but the codes'
+// unpacking.  P^T is the transpose of what S^T leaves in the registers: one
+// movmatrix for 8 keys.  Lane (n, j) holds the scores of keys n and n + 8 with
+// rows 2 j and 2 j + 1.
+template <int DIM, int GROUP, int NT, int KW>
+struct FewShape {
+  static constexpr int THREADS = 32 * KW, ROWS = 8 * NT;
   static constexpr int BB = block_bytes(DIM, GROUP);
   static constexpr int STAGES = DIM == 64 ? 4 : 3;
   static constexpr int RING = KW * STAGES * 2 * BB;
-  static constexpr int ROWS = 16 * MW;
-  // joining: per key group O [ROWS][DIM], m [ROWS], l [ROWS]; it takes the rings' place
-  static constexpr int PART = ROWS * (DIM + 2) * 4;
-  static constexpr int SMEM = (RING > (KW + 1) * PART ? RING : (KW + 1) * PART) + 16 * KW * STAGES;
+  static constexpr int JOIN = (KW + 1) * ROWS * (DIM + 2) * 4;
+  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 };
 
-template <typename T, int DIM, int GROUP, int MW, int KW>
-__global__ void __launch_bounds__(32 * MW * KW)
-    k_kv_attention(const lx_kv_cache c, int layer, const lx_kv_rows r, int q_heads, int per, int tiles, int split,
-                   const T* __restrict__ q, int64_t q_row, int64_t q_head, bool wide, T* __restrict__ out,
-                   int64_t o_row, int64_t o_head, float* lse, float scale, Mask mask) {
-  using S = Shape<DIM, GROUP, MW, KW>;
-  constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB, STAGES = S::STAGES;
+template <typename T, int DIM, int GROUP, int NT, int KW>
+__global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)) k_kv_few(const __grid_constant__ Args a) {
+  using S = FewShape<DIM, GROUP, NT, KW>;
+  constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB;
   extern __shared__ __align__(128) uint8_t smem[];
-  int* held = reinterpret_cast<int*>(smem + S::SMEM - 16 * KW * STAGES);  // [KW][STAGES][4]: blocks of the stage that exist
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
-  const int mw = warp % MW, kg = warp / MW, gt = threadIdx.x % (32 * MW);
-  const int rank = blockIdx.x % split;
-  int item = blockIdx.x / split;
-  const int head = item % c.kv_heads;
-  item /= c.kv_heads;
-  const int tile = item % tiles, entry = item / tiles;
+  pdl_launch_dependents();
+  pdl_wait();
+  Share s;
+  if (!s.take(a, S::ROWS)) return;
 
-  const Entry e = entry_of(c, r, entry);
-  const int rows = e.rows * per, row0 = tile * S::ROWS;
-  if (row0 >= rows) return;  // the whole cluster
-  const int n_rows = min(S::ROWS, rows - row0);
-  int len = 0, start = LX_KV_REFUSED;
-  if (e.slot >= 0) {
-    len = length_of(c, e.slot);
-    start = start_of(r, entry, len, e.rows);
-  }
-  // keys of this lane's two rows, of the warp's rows (seen by one: [lo, hi), by all: [lo_all, hi_all)), of the CTA's
-  int lo[2] = {0, 0}, hi[2] = {0, 0}, lo_all = 0, hi_all = 0, lo_cta = 0, hi_cta = 0;
-  if (start != LX_KV_REFUSED) {
-    int x;
+  // keys seen by this lane's rows 8 r + 2 j + x, and by every row
+  int lo[NT][2], hi[NT][2], lo_all, hi_all, lo_cta, hi_cta;
+  s.range(a, 0, lo_cta, hi_all);
+  s.range(a, S::ROWS, lo_all, hi_cta);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      mask.range(start + min(row0 + 16 * mw + n + 8 * u, rows - 1) / per, len, lo[u], hi[u]);
-    mask.range(start + min(row0 + 16 * mw, rows - 1) / per, len, x, hi_all);
-    mask.range(start + min(row0 + 16 * mw + 15, rows - 1) / per, len, lo_all, x);
-    mask.range(start + row0 / per, len, lo_cta, x);
-    mask.range(start + (row0 + n_rows - 1) / per, len, x, hi_cta);
-  }
+  for (int r = 0; r < NT; ++r)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) s.range(a, 8 * r + 2 * j + x, lo[r][x], hi[r][x]);
+  int unit, unit_end;
+  share_units(lo_cta, hi_cta, s.rank, a.split, unit, unit_end);
+  unit += warp;
+  Ring<BB, S::STAGES, KW, 32> ring;
+  uint8_t* stages = smem + warp * S::STAGES * 2 * BB;
+  ring.start(a, s, unit, unit_end, hi_cta, stages, lane);
 
-  // the query as A operands; lane (n, j): channels 64 h + 32 w + 8 j + {0..7} of rows n and n + 8
-  uint32_t qa[H][2][2][4];
-  float qs[2][G];
+  // the query: lane (n, j) holds channels 64 h + 32 w + 8 j + {0..7} of row 8 r + n
+  uint32_t qb[NT][H][2][2][2];
+  float2 qs[NT][G];  // sums over a group's channels of rows 2 j, 2 j + 1, times scale log2(e)
   float c1;
   {
-    float x[2][H][2][8], top = 0.0f;
+    float x[NT][H][2][8], top = 0.0f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = min(row0 + 16 * mw + n + 8 * u, rows - 1);
-      const T* p = q + (e.row0 + row / per) * q_row + (head * per + row % per) * q_head + 8 * j;
+    for (int r = 0; r < NT; ++r) {
+      const T* p = s.query<T>(a, 8 * r + n) + 8 * j;
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          if (wide) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p + 64 * h + 32 * w);
-            const T* t = reinterpret_cast<const T*>(&v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[u][h][w][i] = static_cast<float>(t[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[u][h][w][i] = static_cast<float>(p[64 * h + 32 * w + i]);
-          }
+          query8(p + 64 * h + 32 * w, a.wide, x[r][h][w]);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float a = fabsf(x[u][h][w][i]);
-            top = a <= 3.4e38f ? fmaxf(top, a) : top;
+            const float y = fabsf(x[r][h][w][i]);
+            top = y <= 3.4e38f ? fmaxf(top, y) : top;
           }
         }
     }
+    const int up = query_exponent(top);
+    const float f = pow2(up), f16 = f * 0.0625f, l2 = a.scale * 1.4426950408889634f;
+    c1 = l2 * pow2(24) * pow2(-up);
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // 2^up x top lies in [2^13, 2^14)
-    const int up = top > 0.0f ? min(max(13 - ilogbf(top), -110), 110) : 0;
-    const float f = ldexpf(1.0f, up), f16 = f * 0.0625f, l2 = scale * 1.4426950408889634f;
-    c1 = ldexpf(l2, 24 - up);
+    for (int r = 0; r < NT; ++r) {
+      float sum[G];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int g = 0; g < G; ++g) qs[u][g] = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int g = 0; g < G; ++g) sum[g] = 0.0f;
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const float(&y)[8] = x[u][h][w];
-          float sum = 0.0f;
+          const float(&y)[8] = x[r][h][w];
+          sum[(64 * h + 32 * w) / GROUP] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum += y[i];
-          qs[u][(64 * h + 32 * w) / GROUP] += sum;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            __half2 a = __floats2half2_rn(y[4 * s] * f, y[4 * s + 1] * f);
-            qa[h][w][s][u] = *reinterpret_cast<uint32_t*>(&a);
-            a = __floats2half2_rn(y[4 * s + 2] * f16, y[4 * s + 3] * f16);
-            qa[h][w][s][2 + u] = *reinterpret_cast<uint32_t*>(&a);
+          for (int t = 0; t < 2; ++t) {
+            qb[r][h][w][t][0] = half_pair(make_float2(y[4 * t] * f, y[4 * t + 1] * f));
+            qb[r][h][w][t][1] = half_pair(make_float2(y[4 * t + 2] * f16, y[4 * t + 3] * f16));
           }
         }
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
       for (int g = 0; g < G; ++g) {
-        qs[u][g] += __shfl_xor_sync(0xffffffffu, qs[u][g], 1);
-        qs[u][g] += __shfl_xor_sync(0xffffffffu, qs[u][g], 2);
-        qs[u][g] *= l2;
-      }
-  }
-
-  // the units of this key group: unit0, unit0 + KW, ... < unit1
-  int unit0 = 0, unit1 = 0;
-  if (hi_cta > lo_cta) {
-    const int first = lo_cta / UNIT, count = (hi_cta + UNIT - 1) / UNIT - first;
-    unit0 = first + static_cast<int>(static_cast<long long>(count) * rank / split);
-    unit1 = first + static_cast<int>(static_cast<long long>(count) * (rank + 1) / split);
-  }
-  unit0 += kg;
-  const int32_t* table = c.table + static_cast<size_t>(e.slot < 0 ? 0 : e.slot) * c.max_pages;
-  const int per_page = c.page / BLOCK;  // blocks
-  const uint8_t* pool = static_cast<const uint8_t*>(c.pool);
-  uint8_t* ring = smem + kg * STAGES * 2 * BB;
-  int* ring_held = held + kg * STAGES * 4;
-
-  // page ids of the next unit to load, read one step ahead
-  int next = unit0, page[2] = {-1, -1};
-  auto look_up = [&] {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int block = 2 * next + b;
-      page[b] = next < unit1 && block * BLOCK < hi_cta ? table[block / per_page] : -2;
-    }
-  };
-  auto load = [&](int stage) {
-    int got = 0;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if (page[b] >= 0 && page[b] < c.n_pages) {
-        got |= 1 << b;
-        const uint8_t* src = pool + block_at(c, layer, page[b], head, (2 * next + b) % per_page);
-        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring + (2 * stage + b) * BB));
-#pragma unroll
-        for (int x = 0; x < (BB / 16 + 32 * MW - 1) / (32 * MW); ++x) {
-          const int at = gt + 32 * MW * x;
-          if (at < BB / 16) cp_async16(dst + 16 * at, src + 16 * at);
-        }
-      } else if (page[b] != -2 && gt == 0) {
-        flag(c, LX_KV_PAGE);
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+        sum[g] *= l2;
+        qs[r][g].x = __shfl_sync(0xffffffffu, sum[g], 8 * j);
+        qs[r][g].y = __shfl_sync(0xffffffffu, sum[g], 8 * j + 4);
       }
     }
-    if (gt == 0) ring_held[4 * stage] = got;
-    cp_async_commit();
-    next += KW;
-    look_up();
-  };
-  look_up();
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load(i);
+  }
 
-  float o[H][2][4][4], o8[G][4];  // o8: the rounded p s F times 8, the same in every column
+  float o[NT][H][2][2][4], o8[NT][G][4];
+  float2 m[NT], off[NT], l[NT], z[NT][G];  // maxima; what is subtracted (less log2 F); sums of p F, and of p F (m_v + 8 s_v)
+  float step_top = 0.0f;                   // power of two at or above the largest step of V so far
+  int f_exp = 0;                           // F = 2^f_exp
 #pragma unroll
-  for (int g = 0; g < G; ++g) o8[g][0] = o8[g][1] = o8[g][2] = o8[g][3] = 0.0f;
+  for (int r = 0; r < NT; ++r) {
+    m[r] = both(-INFINITY);
+    off[r] = l[r] = both(0.0f);
 #pragma unroll
-  for (int h = 0; h < H; ++h)
+    for (int g = 0; g < G; ++g) {
+      z[r][g] = both(0.0f);
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+      for (int x = 0; x < 4; ++x) o8[r][g][x] = 0.0f;
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[h][w][i][x] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY};    // running maxima
-  float off[2] = {0.0f, 0.0f};            // what is subtracted from the scores: m, 0 while nothing was seen
-  float2 l[2] = {both(0.0f), both(0.0f)}; // sums of p, over this lane's keys
-  float2 z[2][G];                         // sums of p (m_v + 8 s_v)
-  float vtop[G], vf[G];                   // power of two above the largest step of V so far, F
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    z[0][g] = z[1][g] = both(0.0f);
-    vtop[g] = 0.0f;
-    vf[g] = 1.0f;
+    for (int x = 0; x < H * 16; ++x) o[r][x / 16][x / 8 % 2][x / 4 % 2][x % 4] = 0.0f;
   }
 
   int stage = 0;
-  for (int unit = unit0; unit < unit1; unit += KW) {
-    cp_async_wait<STAGES - 2>();
-    if (MW == 1)
-      __syncwarp();
-    else
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + kg), "n"(32 * MW) : "memory");
-    load((stage + STAGES - 1) % STAGES);
-    const uint8_t* data = ring + 2 * stage * BB;
-    const int got = ring_held[4 * stage];
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  const int slot = 16 * (n / 2) + 4 * (n % 2);  // bytes to the parameters of key n; those of n + 8 are 8 further
+#pragma unroll 1
+  for (; unit < unit_end; unit += KW) {
+    cp_async_wait<S::STAGES - 2>();
+    __syncwarp();
+    ring.load(stage == 0 ? S::STAGES - 1 : stage - 1);
+    const uint8_t* data = stages + 2 * stage * BB;
+    const uint32_t got = ring.got >> (2 * (S::STAGES - 1)) & 3u;
+    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
     const int key0 = unit * UNIT;
 
-    // scores, in log2 units: s[block][row][key half]
-    float2 s[2][2][2];
+    // scores in log2 units, of (rows 2 j, 2 j + 1): s2[block][r][key n or n + 8]
+    float2 s2[2][NT][2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const uint8_t* d = data + b * BB;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float raw[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        float raw[NT][4];
 #pragma unroll
         for (int hw = g * GROUP / 32; hw < (g + 1) * GROUP / 32; ++hw) {
-          const uint2 k0 = *reinterpret_cast<const uint2*>(d + 512 * (hw / 2) + 16 * lane);
-          const uint2 k1 = *reinterpret_cast<const uint2*>(d + 512 * (hw / 2) + 16 * lane + 8);
-          const uint32_t w0 = hw % 2 ? k0.y : k0.x, w1 = hw % 2 ? k1.y : k1.x;
-          mma(raw[0], qa[hw / 2][hw % 2][0], w0 & M0, w0 & M1);
-          mma(raw[1], qa[hw / 2][hw % 2][0], w1 & M0, w1 & M1);
-          mma(raw[0], qa[hw / 2][hw % 2][1], w0 >> 8 & M0, w0 >> 8 & M1);
-          mma(raw[1], qa[hw / 2][hw % 2][1], w1 >> 8 & M0, w1 >> 8 & M1);
+          const uint4 k = lds128(d + 512 * (hw / 2) + 16 * lane);
+          const uint32_t k0 = hw % 2 ? k.y : k.x, k1 = hw % 2 ? k.w : k.z;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t x0 = k0 >> (8 * t), x1 = k1 >> (8 * t);
+#pragma unroll
+            for (int r = 0; r < NT; ++r) {
+              const uint32_t(&y)[2] = qb[r][hw / 2][hw % 2][t];
+              if (hw == g * GROUP / 32 && t == 0)
+                mma0(raw[r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
+              else
+                mma(raw[r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
+            }
+          }
         }
-        const uint4 kp = lds128(d + param_offset(DIM) + 64 * g + 16 * j);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint32_t p0 = t ? kp.z : kp.x, p1 = t ? kp.w : kp.y;
-          const float2 ks = __fmul2_rn(steps(p0, p1), both(c1)), km = minima(p0, p1);
+          const uint32_t p = lds32(d + param_offset(DIM) + 64 * g + slot + 8 * t);
+          const float2 ks = both(step_of(p) * c1), km = both(low_of(p));
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float2 base = g == 0 ? __fmul2_rn(both(qs[u][g]), km) : __ffma2_rn(both(qs[u][g]), km, s[b][u][t]);
-            s[b][u][t] = __ffma2_rn(make_float2(raw[t][2 * u], raw[t][2 * u + 1]), ks, base);
+          for (int r = 0; r < NT; ++r) {
+            const float2 base = g == 0 ? __fmul2_rn(qs[r][g], km) : __ffma2_rn(qs[r][g], km, s2[b][r][t]);
+            s2[b][r][t] = __ffma2_rn(make_float2(raw[r][2 * t], raw[r][2 * t + 1]), ks, base);
           }
         }
       }
     }
-    const bool part = got != 3 || key0 < lo_all || key0 + UNIT > hi_all;
-    uint32_t seen = 0xFFFFu;  // bit 8 b + 4 u + 2 t + x
+    // steps and centred minima of V
+    float vs[2][G][2], vm[2][G][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t p = lds32(data + b * BB + param_offset(DIM) + 64 * (G + g) + slot + 8 * t);
+          vs[b][g][t] = step_of(p);
+          vm[b][g][t] = fmaf(vs[b][g][t], 8.0f, low_of(p));
+        }
+    const bool part = got != 3u || key0 < lo_all || key0 + UNIT > hi_all;
+    uint32_t seen = 0xFFFFFFFFu;  // bit 4 NT b + 4 r + 2 t + x
     if (part) {
       seen = 0;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int t = 0; t < 2; ++t) {
+          const int key = (got >> b & 1) ? key0 + 16 * b + 8 * t + n : -1;
+          bool any = false;
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int r = 0; r < NT; ++r)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const int key = key0 + 16 * b + 8 * t + 2 * j + x;
-              const bool in = (got >> b & 1) && key >= lo[u] && key < hi[u];
-              seen |= static_cast<uint32_t>(in) << (8 * b + 4 * u + 2 * t + x);
-              if (!in) (x ? s[b][u][t].y : s[b][u][t].x) = -INFINITY;
+              const bool in = key >= lo[r][x] && key < hi[r][x];
+              any |= in;
+              seen |= static_cast<uint32_t>(in) << (4 * NT * b + 4 * r + 2 * t + x);
+              if (!in) (x ? s2[b][r][t].y : s2[b][r][t].x) = -INFINITY;
             }
+          if (!any)  // a step that none of the rows sees does not count
+#pragma unroll
+            for (int g = 0; g < G; ++g) vs[b][g][t] = vm[b][g][t] = 0.0f;
+        }
     }
-    // steps of V; a step that nobody sees does not count
-    float2 vs[2][G][2], vm[2][G][2];
     bool raise = false;
+    float2 top[NT];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint4 vp = lds128(data + b * BB + param_offset(DIM) + 64 * (G + g) + 16 * j);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t p0 = t ? vp.z : vp.x, p1 = t ? vp.w : vp.y;
-          vs[b][g][t] = steps(p0, p1);
-          vm[b][g][t] = __ffma2_rn(vs[b][g][t], both(8.0f), minima(p0, p1));
-          if (part) {
-            const uint32_t any = seen >> (8 * b + 2 * t) | seen >> (8 * b + 2 * t + 4);
-            if (!(any & 1)) vs[b][g][t].x = vm[b][g][t].x = 0.0f;
-            if (!(any & 2)) vs[b][g][t].y = vm[b][g][t].y = 0.0f;
-          }
-          raise |= fmaxf(vs[b][g][t].x, vs[b][g][t].y) > vtop[g];
-        }
-      }
-    float top[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      top[u] = fmaxf(fmaxf(fmaxf(s[0][u][0].x, s[0][u][0].y), fmaxf(s[0][u][1].x, s[0][u][1].y)),
-                     fmaxf(fmaxf(s[1][u][0].x, s[1][u][0].y), fmaxf(s[1][u][1].x, s[1][u][1].y)));
-      raise |= top[u] > m[u] + RAISE;
+    for (int r = 0; r < NT; ++r) {
+      top[r].x = fmaxf(fmaxf(s2[0][r][0].x, s2[0][r][1].x), fmaxf(s2[1][r][0].x, s2[1][r][1].x));
+      top[r].y = fmaxf(fmaxf(s2[0][r][0].y, s2[0][r][1].y), fmaxf(s2[1][r][0].y, s2[1][r][1].y));
+      raise |= top[r].x > m[r].x + RAISE || top[r].y > m[r].y + RAISE;
     }
+    float v = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) v = fmaxf(v, fmaxf(fmaxf(vs[0][g][0], vs[0][g][1]), fmaxf(vs[1][g][0], vs[1][g][1])));
+    raise |= v > step_top;
     if (__any_sync(0xffffffffu, raise)) {
-      float f[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
-        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
-        const float to = fmaxf(m[u], top[u]);
-        f[u] = to == -INFINITY ? 1.0f : ex2(m[u] - to);
-        m[u] = to;
-        off[u] = to == -INFINITY ? 0.0f : to;
-        l[u] = __fmul2_rn(l[u], both(f[u]));
-#pragma unroll
-        for (int g = 0; g < G; ++g) z[u][g] = __fmul2_rn(z[u][g], both(f[u]));
+      for (int x = 4; x < 32; x *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+      int up = 0;
+      if (v > step_top) {
+        const int e = step_exponent(v), to = P_TOP - e;
+        up = step_top == 0.0f ? 0 : to - f_exp;
+        f_exp = to;
+        step_top = v > STEP_MAX ? INFINITY : pow2(e);
       }
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float v = 0.0f;
+      for (int r = 0; r < NT; ++r) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int x = 4; x < 32; x *= 2) {
+          top[r].x = fmaxf(top[r].x, __shfl_xor_sync(0xffffffffu, top[r].x, x));
+          top[r].y = fmaxf(top[r].y, __shfl_xor_sync(0xffffffffu, top[r].y, x));
+        }
+        const float2 to = make_float2(fmaxf(m[r].x, top[r].x), fmaxf(m[r].y, top[r].y));
+        float2 f;
+        f.x = to.x == -INFINITY ? 1.0f : ex2(m[r].x - to.x + up);
+        f.y = to.y == -INFINITY ? 1.0f : ex2(m[r].y - to.y + up);
+        m[r] = to;
+        off[r].x = (to.x == -INFINITY ? 0.0f : to.x) - f_exp;
+        off[r].y = (to.y == -INFINITY ? 0.0f : to.y) - f_exp;
+        l[r] = __fmul2_rn(l[r], f);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) v = fmaxf(v, fmaxf(vs[b][g][t].x, vs[b][g][t].y));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-        float ratio = 1.0f;
-        if (v > vtop[g]) {  // the power of two at or above v, at least 2^-110
-          const uint32_t bits = (__float_as_uint(v) + 0x7FFFFFu) & 0x7F800000u;
-          const float to = fminf(fmaxf(__uint_as_float(bits), 7.7037198e-34f), 8.5070592e37f);
-          const float nf = P_TOP / to;
-          ratio = vtop[g] == 0.0f ? 1.0f : nf / vf[g];
-          vtop[g] = v > to ? INFINITY : to;
-          vf[g] = nf;
+        for (int g = 0; g < G; ++g) {
+          z[r][g] = __fmul2_rn(z[r][g], f);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o8[r][g][x] *= x % 2 ? f.y : f.x;
         }
 #pragma unroll
-        for (int hw = g * GROUP / 32; hw < (g + 1) * GROUP / 32; ++hw)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[hw / 2][hw % 2][i][x] *= f[x / 2] * ratio;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o8[g][x] *= f[x / 2] * ratio;
+        for (int x = 0; x < H * 16; ++x) o[r][x / 16][x / 8 % 2][x / 4 % 2][x % 4] *= x % 2 ? f.y : f.x;
       }
     }
-    // p, its sums, and O += (p s F) c
+    // p F, its sums, and O += (p F s) c
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const uint8_t* d = data + b * BB + 512 * H;
-      float2 p[2][2];
+      uint32_t pb[NT][G][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float2 y = __fadd2_rn(s[b][u][t], both(-off[u]));
-          p[u][t] = make_float2(ex2(y.x), ex2(y.y));
-          l[u] = __fadd2_rn(l[u], p[u][t]);
-        }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        uint32_t pa[4];
+      for (int r = 0; r < NT; ++r)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float2 f = __fmul2_rn(vs[b][g][t], both(vf[g]));
+          const float2 y = __fadd2_rn(s2[b][r][t], make_float2(-off[r].x, -off[r].y));
+          const float2 p = make_float2(ex2(y.x), ex2(y.y));
+          l[r] = __fadd2_rn(l[r], p);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float2 a = __fmul2_rn(p[u][t], f), add = p[u][t];
-            if (part) {  // a key that this row does not see: not even its NaN counts
-              const uint32_t in = seen >> (8 * b + 4 * u + 2 * t);
-              float2 low = vm[b][g][t];
-              if (!(in & 1)) a.x = low.x = 0.0f;
-              if (!(in & 2)) a.y = low.y = 0.0f;
-              z[u][g] = __ffma2_rn(add, low, z[u][g]);
-            } else {
-              z[u][g] = __ffma2_rn(add, vm[b][g][t], z[u][g]);
+          for (int g = 0; g < G; ++g) {
+            float2 w = __fmul2_rn(p, both(vs[b][g][t])), low = both(vm[b][g][t]);
+            if (part) {  // a key that a row does not see: not even its NaN counts
+              const uint32_t in = seen >> (4 * NT * b + 4 * r + 2 * t);
+              if (!(in & 1)) w.x = low.x = 0.0f;
+              if (!(in & 2)) w.y = low.y = 0.0f;
             }
-            const __half2 hp = __float22half2_rn(a);
-            pa[2 * t + u] = *reinterpret_cast<const uint32_t*>(&hp);
+            z[r][g] = __ffma2_rn(p, low, z[r][g]);
+            pb[r][g][t] = transpose8(half_pair(w));
           }
         }
-        mma(o8[g], pa, 0x00080008u, 0x00080008u);
 #pragma unroll
-        for (int hw = g * GROUP / 32; hw < (g + 1) * GROUP / 32; ++hw) {
-          const uint4 v = lds128(d + 512 * (hw / 2) + 16 * lane);
-          const uint32_t w0 = hw % 2 ? v.y : v.x, w1 = hw % 2 ? v.w : v.z;
-          float(&acc)[4][4] = o[hw / 2][hw % 2];
-          mma(acc[0], pa, w0 & M0, w1 & M0);
-          mma(acc[1], pa, w0 & M1, w1 & M1);
-          mma(acc[2], pa, w0 >> 8 & M0, w1 >> 8 & M0);
-          mma(acc[3], pa, w0 >> 8 & M1, w1 >> 8 & M1);
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int r = 0; r < NT; ++r) mma(o8[r][g], EIGHTS, EIGHTS, EIGHTS, EIGHTS, pb[r][g][0], pb[r][g][1]);
+#pragma unroll
+      for (int hw = 0; hw < 2 * H; ++hw) {
+        const uint4 x = lds128(d + 512 * (hw / 2) + 16 * lane);
+        const uint32_t v0 = hw % 2 ? x.y : x.x, v1 = hw % 2 ? x.w : x.z;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t x0 = v0 >> (8 * i), x1 = v1 >> (8 * i);
+#pragma unroll
+          for (int r = 0; r < NT; ++r)
+            mma(o[r][hw / 2][hw % 2][i], x0 & M0, x0 & M1, x1 & M0, x1 & M1, pb[r][32 * hw / GROUP][0],
+                pb[r][32 * hw / GROUP][1]);
         }
       }
     }
@@ -466,153 +615,454 @@ __global__ void __launch_bounds__(32 * MW * KW)
   cp_async_wait<0>();
   __syncthreads();  // every ring has been read: the joining takes their place
 
-  // this warp's result: O in true units
-  float* part_o = reinterpret_cast<float*>(smem);              // [KW + 1][ROWS][DIM], the last one the CTA's
-  float* part_m = part_o + (KW + 1) * S::ROWS * DIM;           // [KW + 1][ROWS]
+  float* part_o = reinterpret_cast<float*>(smem);  // [KW + 1][ROWS][DIM], the last one the CTA's
+  float* part_m = part_o + (KW + 1) * S::ROWS * DIM;
   float* part_l = part_m + (KW + 1) * S::ROWS;
+  const float back = pow2(-f_exp);
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int row = 16 * mw + n + 8 * u;
-    float sum = l[u].x + l[u].y;
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if (j == 0) {
-      part_m[kg * S::ROWS + row] = m[u];
-      part_l[kg * S::ROWS + row] = sum;
-    }
+  for (int r = 0; r < NT; ++r)
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+    for (int x = 0; x < 2; ++x) {
+      const int row = 8 * r + 2 * j + x;
+      float sum = x ? l[r].y : l[r].x, low[G];
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int g = (64 * h + 32 * w) / GROUP;
-        float low = z[u][g].x + z[u][g].y;
-        low += __shfl_xor_sync(0xffffffffu, low, 1);
-        low += __shfl_xor_sync(0xffffffffu, low, 2);
-        const float f = 1.0f / vf[g];
-        // columns 2 j, 2 j + 1 of product i are channels 8 j + i and 8 j + 4 + i
-        float* dst = part_o + (kg * S::ROWS + row) * DIM + 64 * h + 32 * w + 8 * j;
+      for (int g = 0; g < G; ++g) low[g] = x ? z[r][g].y : z[r][g].x;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+      for (int y = 4; y < 32; y *= 2) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, y);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            dst[4 * x + i] =
-                fmaf((o[h][w][i][2 * u + x] * (i % 2 ? 0.0625f : 1.0f) - o8[g][2 * u + x]) * 16777216.0f, f, low);
+        for (int g = 0; g < G; ++g) low[g] += __shfl_xor_sync(0xffffffffu, low[g], y);
       }
-  }
+      if (row < s.n_rows) {
+        if (n == 0) {
+          part_m[warp * S::ROWS + row] = x ? m[r].y : m[r].x;
+          part_l[warp * S::ROWS + row] = sum * back;
+        }
+        // rows n and n + 8 of product i are channels 4 n + 2 i and 4 n + 2 i + 1, the latter times 16
+#pragma unroll
+        for (int hw = 0; hw < 2 * H; ++hw) {
+          const float(&y)[2][4] = o[r][hw / 2][hw % 2];
+          const float c = o8[r][32 * hw / GROUP][x], w = low[32 * hw / GROUP];
+          float4 out;
+          out.x = fmaf(y[0][x] - c, 16777216.0f, w) * back;
+          out.y = fmaf(fmaf(y[0][2 + x], 0.0625f, -c), 16777216.0f, w) * back;
+          out.z = fmaf(y[1][x] - c, 16777216.0f, w) * back;
+          out.w = fmaf(fmaf(y[1][2 + x], 0.0625f, -c), 16777216.0f, w) * back;
+          *reinterpret_cast<float4*>(part_o + (warp * S::ROWS + row) * DIM + 32 * hw + 4 * n) = out;
+        }
+      }
+    }
   __syncthreads();
-  // join the CTA's key groups
-  float* cta_o = part_o + KW * S::ROWS * DIM;
-  float* cta_m = part_m + KW * S::ROWS;
-  float* cta_l = part_l + KW * S::ROWS;
-  for (int x = threadIdx.x; x < n_rows * DIM; x += S::THREADS) {
-    const int row = x / DIM;
-    float top = part_m[row];
-#pragma unroll
-    for (int k = 1; k < KW; ++k) top = fmaxf(top, part_m[k * S::ROWS + row]);
-    float a = 0.0f, sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      const float mk = part_m[k * S::ROWS + row];
-      const float f = mk == top ? 1.0f : ex2(mk - top);
-      a = fmaf(part_o[k * S::ROWS * DIM + x], f, a);
-      sum = fmaf(part_l[k * S::ROWS + row], f, sum);
-    }
-    cta_o[x] = a;
-    if (x % DIM == 0) {
-      cta_m[row] = top;
-      cta_l[row] = sum;
-    }
-  }
-  if (split > 1)
-    cg::this_cluster().sync();
-  else
-    __syncthreads();
-  // join the cluster's CTAs, each a part of the outputs
-  for (int x = threadIdx.x + rank * S::THREADS; x < n_rows * DIM; x += split * S::THREADS) {
-    const int row = x / DIM, d = x % DIM;
-    float top, a, sum;
-    if (split > 1) {
-      top = -INFINITY;
-      for (int k = 0; k < split; ++k) top = fmaxf(top, *cg::this_cluster().map_shared_rank(cta_m + row, k));
-      a = sum = 0.0f;
-      for (int k = 0; k < split; ++k) {
-        const float mk = *cg::this_cluster().map_shared_rank(cta_m + row, k);
-        const float f = mk == top ? 1.0f : ex2(mk - top);
-        a = fmaf(*cg::this_cluster().map_shared_rank(cta_o + x, k), f, a);
-        sum = fmaf(*cg::this_cluster().map_shared_rank(cta_l + row, k), f, sum);
-      }
-    } else {
-      top = cta_m[row];
-      a = cta_o[x];
-      sum = cta_l[row];
-    }
-    const int t = (row0 + row) / per, h = head * per + (row0 + row) % per;
-    out[(e.row0 + t) * o_row + h * o_head + d] = static_cast<T>(sum == 0.0f ? 0.0f : a / sum);
-    if (lse && d == 0)
-      lse[static_cast<int64_t>(e.row0 + t) * q_heads + h] =
-          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-  }
-  if (split > 1) cg::this_cluster().sync();  // nobody leaves while its part may be read
+  join<T, DIM, KW, S::ROWS, S::THREADS>(a, s, part_o, part_m, part_l);
 }
 
-struct Call {
-  const lx_kv_cache* c;
-  const lx_kv_rows* r;
-  int layer, q_heads;
-  const void* q;
-  int64_t q_row, q_head;
-  void* out;
-  int64_t o_row, o_head;
-  float* lse;
-  float scale;
-  Mask mask;
-  int max_len;
-  cudaStream_t s;
+// ---------------------------------------------------------------------------
+// many rows
+// ---------------------------------------------------------------------------
+// MW warps of 16 MT rows share each unit of keys.  Lane (n, j) holds the scores of rows
+// n and n + 8 of each 16 with keys 2 j + {0, 1, 8, 9}, which is how P enters the second product.
+template <int DIM, int GROUP, int MT, int MW>
+struct ManyShape {
+  static constexpr int THREADS = 32 * MW, ROWS = 16 * MT * MW;
+  static constexpr int BB = block_bytes(DIM, GROUP);
+  static constexpr int STAGES = 4;
+  static constexpr int RING = STAGES * 2 * BB;
+  static constexpr int JOIN = ROWS * (DIM + 2) * 4;
+  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 };
 
-template <typename T, int DIM, int GROUP, int MW, int KW>
-bool run(const Call& a) {
-  using S = Shape<DIM, GROUP, MW, KW>;
-  auto kernel = k_kv_attention<T, DIM, GROUP, MW, KW>;
-  static bool ready[64] = {false};
-  int dev = a.c->device & 63;
-  if (!ready[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess ||
+template <typename T, int DIM, int GROUP, int MT, int MW>
+__global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Args a) {
+  using S = ManyShape<DIM, GROUP, MT, MW>;
+  constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
+  const int warp_row = 16 * MT * warp;
+  pdl_launch_dependents();
+  pdl_wait();
+  Share s;
+  if (!s.take(a, S::ROWS)) return;
+
+  // keys seen by this lane's rows warp_row + 16 r + n + 8 u; by every row of the warp; by one of the warp, the CTA
+  int lo[MT][2], hi[MT][2], lo_all, hi_all, lo_warp, hi_warp, lo_cta, hi_cta, x_;
+  s.range(a, 0, lo_cta, x_);
+  s.range(a, S::ROWS, x_, hi_cta);
+  s.range(a, warp_row, lo_warp, hi_all);
+  s.range(a, warp_row + 16 * MT - 1, lo_all, hi_warp);
+#pragma unroll
+  for (int r = 0; r < MT; ++r)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s.range(a, warp_row + 16 * r + n + 8 * u, lo[r][u], hi[r][u]);
+  int unit, unit_end;
+  share_units(lo_cta, hi_cta, s.rank, a.split, unit, unit_end);
+  Ring<BB, S::STAGES, 1, 32 * MW> ring;
+  ring.start(a, s, unit, unit_end, hi_cta, smem, threadIdx.x);
+
+  // the query: lane (n, j) holds channels 64 h + 32 w + 8 j + {0..7} of rows n and n + 8 of each 16
+  uint32_t qa[MT][H][2][2][4];
+  float qs[MT][2][G];
+  float c1;
+  {
+    float x[MT][2][H][2][8], top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const T* p = s.query<T>(a, warp_row + 16 * r + n + 8 * u) + 8 * j;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            query8(p + 64 * h + 32 * w, a.wide, x[r][u][h][w]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float y = fabsf(x[r][u][h][w][i]);
+              top = y <= 3.4e38f ? fmaxf(top, y) : top;
+            }
+          }
+      }
+    const int up = query_exponent(top);
+    const float f = pow2(up), f16 = f * 0.0625f, l2 = a.scale * 1.4426950408889634f;
+    c1 = l2 * pow2(24) * pow2(-up);
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) qs[r][u][g] = 0.0f;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const float(&y)[8] = x[r][u][h][w];
+            qs[r][u][(64 * h + 32 * w) / GROUP] +=
+                ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              qa[r][h][w][t][u] = half_pair(make_float2(y[4 * t] * f, y[4 * t + 1] * f));
+              qa[r][h][w][t][2 + u] = half_pair(make_float2(y[4 * t + 2] * f16, y[4 * t + 3] * f16));
+            }
+          }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          qs[r][u][g] += __shfl_xor_sync(0xffffffffu, qs[r][u][g], 1);
+          qs[r][u][g] += __shfl_xor_sync(0xffffffffu, qs[r][u][g], 2);
+          qs[r][u][g] *= l2;
+        }
+      }
+  }
+
+  float o[MT][H][2][4][4], o8[MT][G][4];
+  float m[MT][2], off[MT][2];        // maxima; what is subtracted (less log2 F)
+  float2 l[MT][2], z[MT][2][G];      // sums of p F, and of p F (m_v + 8 s_v), over this lane's keys
+  float step_top = 0.0f;
+  int f_exp = 0;
+#pragma unroll
+  for (int r = 0; r < MT; ++r) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      m[r][u] = -INFINITY;
+      off[r][u] = 0.0f;
+      l[r][u] = both(0.0f);
+#pragma unroll
+      for (int g = 0; g < G; ++g) z[r][u][g] = both(0.0f);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o8[r][g][x] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < H * 32; ++x) o[r][x / 32][x / 16 % 2][x / 4 % 4][x % 4] = 0.0f;
+  }
+
+  int stage = 0;
+#pragma unroll 1
+  for (; unit < unit_end; ++unit) {
+    cp_async_wait<S::STAGES - 2>();
+    __syncthreads();
+    ring.load(stage == 0 ? S::STAGES - 1 : stage - 1);
+    const uint8_t* data = smem + 2 * stage * BB;
+    const uint32_t got = ring.got >> (2 * (S::STAGES - 1)) & 3u;
+    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+#pragma unroll 1
+    for (int b = 0; b < 2; ++b) {
+      const int key0 = unit * UNIT + 16 * b;
+      if (key0 >= hi_warp || key0 + 16 <= lo_warp || !(got >> b & 1)) continue;
+      const uint8_t* d = data + b * BB;
+      float2 s2[MT][2][2];  // scores in log2 units: [rows 16 r + n, + 8][keys 2 j + {0, 1}, {8, 9}]
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float raw[MT][2][4];
+#pragma unroll
+        for (int hw = g * GROUP / 32; hw < (g + 1) * GROUP / 32; ++hw) {
+          const uint4 k = lds128(d + 512 * (hw / 2) + 16 * lane);
+          const uint32_t kw[2] = {hw % 2 ? k.y : k.x, hw % 2 ? k.w : k.z};
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const uint32_t y = kw[t] >> (8 * x);
+#pragma unroll
+              for (int r = 0; r < MT; ++r) {
+                const uint32_t(&q)[4] = qa[r][hw / 2][hw % 2][x];
+                if (hw == g * GROUP / 32 && x == 0)
+                  mma0(raw[r][t], q[0], q[1], q[2], q[3], y & M0, y & M1);
+                else
+                  mma(raw[r][t], q[0], q[1], q[2], q[3], y & M0, y & M1);
+              }
+            }
+        }
+        const uint4 kp = lds128(d + param_offset(DIM) + 64 * g + 16 * j);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t p0 = t ? kp.z : kp.x, p1 = t ? kp.w : kp.y;
+          const float2 ks = __fmul2_rn(make_float2(step_of(p0), step_of(p1)), both(c1));
+          const float2 km = make_float2(low_of(p0), low_of(p1));
+#pragma unroll
+          for (int r = 0; r < MT; ++r)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float2 base =
+                  g == 0 ? __fmul2_rn(both(qs[r][u][g]), km) : __ffma2_rn(both(qs[r][u][g]), km, s2[r][u][t]);
+              s2[r][u][t] = __ffma2_rn(make_float2(raw[r][t][2 * u], raw[r][t][2 * u + 1]), ks, base);
+            }
+        }
+      }
+      float2 vs[G][2], vm[G][2];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint4 vp = lds128(d + param_offset(DIM) + 64 * (G + g) + 16 * j);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t p0 = t ? vp.z : vp.x, p1 = t ? vp.w : vp.y;
+          vs[g][t] = make_float2(step_of(p0), step_of(p1));
+          vm[g][t] = __ffma2_rn(vs[g][t], both(8.0f), make_float2(low_of(p0), low_of(p1)));
+        }
+      }
+      const bool part = key0 < lo_all || key0 + 16 > hi_all;
+      uint32_t seen = 0xFFFFFFFFu;  // bit 8 r + 4 u + 2 t + x
+      if (part) {
+        seen = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int key = key0 + 8 * t + 2 * j + x;
+            bool any = false;
+#pragma unroll
+            for (int r = 0; r < MT; ++r)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const bool in = key >= lo[r][u] && key < hi[r][u];
+                any |= in;
+                seen |= static_cast<uint32_t>(in) << (8 * r + 4 * u + 2 * t + x);
+                if (!in) (x ? s2[r][u][t].y : s2[r][u][t].x) = -INFINITY;
+              }
+            if (!any)
+#pragma unroll
+              for (int g = 0; g < G; ++g) (x ? vs[g][t].y : vs[g][t].x) = (x ? vm[g][t].y : vm[g][t].x) = 0.0f;
+          }
+      }
+      bool raise = false;
+      float top[MT][2], v = 0.0f;
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          top[r][u] = fmaxf(fmaxf(s2[r][u][0].x, s2[r][u][0].y), fmaxf(s2[r][u][1].x, s2[r][u][1].y));
+          raise |= top[r][u] > m[r][u] + RAISE;
+        }
+#pragma unroll
+      for (int g = 0; g < G; ++g) v = fmaxf(v, fmaxf(fmaxf(vs[g][0].x, vs[g][0].y), fmaxf(vs[g][1].x, vs[g][1].y)));
+      raise |= v > step_top;
+      if (__any_sync(0xffffffffu, raise)) {
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+        int up = 0;
+        if (v > step_top) {
+          const int e = step_exponent(v), to = P_TOP - e;
+          up = step_top == 0.0f ? 0 : to - f_exp;
+          f_exp = to;
+          step_top = v > STEP_MAX ? INFINITY : pow2(e);
+        }
+#pragma unroll
+        for (int r = 0; r < MT; ++r) {
+          float f[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(0xffffffffu, top[r][u], 1));
+            top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(0xffffffffu, top[r][u], 2));
+            const float to = fmaxf(m[r][u], top[r][u]);
+            f[u] = to == -INFINITY ? 1.0f : ex2(m[r][u] - to + up);
+            m[r][u] = to;
+            off[r][u] = (to == -INFINITY ? 0.0f : to) - f_exp;
+            l[r][u] = __fmul2_rn(l[r][u], both(f[u]));
+#pragma unroll
+            for (int g = 0; g < G; ++g) z[r][u][g] = __fmul2_rn(z[r][u][g], both(f[u]));
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o8[r][g][x] *= f[x / 2];
+#pragma unroll
+          for (int x = 0; x < H * 32; ++x) o[r][x / 32][x / 16 % 2][x / 4 % 4][x % 4] *= f[x / 2 % 2];
+        }
+      }
+      // p F, its sums, and O += (p F s) c
+      uint32_t pa[MT][G][4];
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float2 y = __fadd2_rn(s2[r][u][t], both(-off[r][u]));
+            const float2 p = make_float2(ex2(y.x), ex2(y.y));
+            l[r][u] = __fadd2_rn(l[r][u], p);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              float2 w = __fmul2_rn(p, vs[g][t]), low = vm[g][t];
+              if (part) {  // a key that a row does not see: not even its NaN counts
+                const uint32_t in = seen >> (8 * r + 4 * u + 2 * t);
+                if (!(in & 1)) w.x = low.x = 0.0f;
+                if (!(in & 2)) w.y = low.y = 0.0f;
+              }
+              z[r][u][g] = __ffma2_rn(p, low, z[r][u][g]);
+              pa[r][g][2 * t + u] = half_pair(w);
+            }
+          }
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          mma(o8[r][g], pa[r][g][0], pa[r][g][1], pa[r][g][2], pa[r][g][3], EIGHTS, EIGHTS);
+#pragma unroll
+      for (int hw = 0; hw < 2 * H; ++hw) {
+        const uint4 x = lds128(d + 512 * H + 512 * (hw / 2) + 16 * lane);
+        const uint32_t v0 = hw % 2 ? x.y : x.x, v1 = hw % 2 ? x.w : x.z;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t y0 = v0 >> (8 * i), y1 = v1 >> (8 * i);
+#pragma unroll
+          for (int r = 0; r < MT; ++r) {
+            const uint32_t(&p)[4] = pa[r][32 * hw / GROUP];
+            mma(o[r][hw / 2][hw % 2][2 * i], p[0], p[1], p[2], p[3], y0 & M0, y1 & M0);
+            mma(o[r][hw / 2][hw % 2][2 * i + 1], p[0], p[1], p[2], p[3], y0 & M1, y1 & M1);
+          }
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  float* part_o = reinterpret_cast<float*>(smem);  // [ROWS][DIM]
+  float* part_m = part_o + S::ROWS * DIM;
+  float* part_l = part_m + S::ROWS;
+  const float back = pow2(-f_exp);
+#pragma unroll
+  for (int r = 0; r < MT; ++r)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = warp_row + 16 * r + n + 8 * u;
+      float sum = l[r][u].x + l[r][u].y, low[G];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        low[g] = z[r][u][g].x + z[r][u][g].y;
+        low[g] += __shfl_xor_sync(0xffffffffu, low[g], 1);
+        low[g] += __shfl_xor_sync(0xffffffffu, low[g], 2);
+      }
+      if (row < s.n_rows) {
+        if (j == 0) {
+          part_m[row] = m[r][u];
+          part_l[row] = sum * back;
+        }
+        // columns 2 j, 2 j + 1 of product i are channels 8 j + i and 8 j + 4 + i, times 16 for odd i
+#pragma unroll
+        for (int hw = 0; hw < 2 * H; ++hw)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float(&y)[4][4] = o[r][hw / 2][hw % 2];
+            const float c = o8[r][32 * hw / GROUP][2 * u], w = low[32 * hw / GROUP];
+            float4 out;
+            out.x = fmaf(y[0][2 * u + x] - c, 16777216.0f, w) * back;
+            out.y = fmaf(fmaf(y[1][2 * u + x], 0.0625f, -c), 16777216.0f, w) * back;
+            out.z = fmaf(y[2][2 * u + x] - c, 16777216.0f, w) * back;
+            out.w = fmaf(fmaf(y[3][2 * u + x], 0.0625f, -c), 16777216.0f, w) * back;
+            *reinterpret_cast<float4*>(part_o + row * DIM + 32 * hw + 8 * j + 4 * x) = out;
+          }
+      }
+    }
+  __syncthreads();
+  join<T, DIM, 1, S::ROWS, S::THREADS>(a, s, part_o, part_m, part_l);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// Launches over tiles of `tile_rows` rows, the keys of each split over a cluster.
+template <typename K>
+bool start(K kernel, Args& a, bool* ready, int threads, int smem, int tile_rows, int max_len, int split,
+           cudaStream_t s) {
+  bool& done = ready[a.c.device & 63];
+  if (!done) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return false;
-    ready[dev] = true;
+    done = true;
   }
-  const int per = a.q_heads / a.c->kv_heads;
-  const long long tiles = (static_cast<long long>(a.r->max_rows) * per + S::ROWS - 1) / S::ROWS;
-  const long long items = tiles * a.r->n * a.c->kv_heads;
-  // split the keys over a cluster until the GPU is full, leaving each key group two steps
-  const int most = a.max_len > 0 ? a.max_len : a.c->max_pages * a.c->page;
-  int split = 1;
-  while (split < 16 && items * split < 2 * num_sms() && most / UNIT >= 2 * KW * 2 * split) split *= 2;
-  if (items * split > 0x7fffffff) return false;
-  const bool wide = aligned(a.q, 16) && a.q_row % 8 == 0 && a.q_head % 8 == 0;
+  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per + tile_rows - 1) / tile_rows;
+  const long long ctas = tiles * a.r.n * a.c.kv_heads * split;
+  if (ctas > 0x7fffffff) return false;
+  a.tiles = static_cast<int>(tiles);
+  a.split = split;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * split));
-  cfg.blockDim = dim3(S::THREADS);
-  cfg.dynamicSmemBytes = S::SMEM;
-  cfg.stream = a.s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, *a.c, a.layer, *a.r, a.q_heads, per, static_cast<int>(tiles), split,
-                            static_cast<const T*>(a.q), a.q_row, a.q_head, wide, static_cast<T*>(a.out), a.o_row,
-                            a.o_head, a.lse, a.scale, a.mask) == cudaSuccess;
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess;
+}
+
+template <typename T, int DIM, int GROUP, int NT, int KW>
+bool few(Args& a, int max_len, int split, cudaStream_t s) {
+  using S = FewShape<DIM, GROUP, NT, KW>;
+  static bool ready[64] = {false};
+  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, ready, S::THREADS, S::SMEM, S::ROWS, max_len, split, s);
+}
+template <typename T, int DIM, int GROUP, int MT, int MW>
+bool many(Args& a, int max_len, int split, cudaStream_t s) {
+  using S = ManyShape<DIM, GROUP, MT, MW>;
+  static bool ready[64] = {false};
+  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, ready, S::THREADS, S::SMEM, S::ROWS, max_len, split, s);
 }
 
 template <typename T, int DIM, int GROUP>
-bool go(const Call& a) {
-  const long long rows = static_cast<long long>(a.r->max_rows) * (a.q_heads / a.c->kv_heads);
-  if (rows <= 16) return run<T, DIM, GROUP, 1, 4>(a);
-  if (rows <= 32) return run<T, DIM, GROUP, 2, 2>(a);
-  return run<T, DIM, GROUP, 4, 1>(a);
+bool go(Args& a, int max_len, cudaStream_t s) {
+  const long long rows = static_cast<long long>(a.r.max_rows) * a.per;
+  const long long items = static_cast<long long>(a.r.n) * a.c.kv_heads;
+  const int units = (max_len + UNIT - 1) / UNIT;
+  int split = 1;
+  if (rows <= 16) {
+    // as many CTAs as make four rounds of the GPU, as long as every warp has two units
+    while (split < 16 && items * split < 4 * num_sms() * (DIM == 64 ? 4 : 3) && units >= 2 * 4 * 2 * split) split *= 2;
+    return rows <= 8 ? few<T, DIM, GROUP, 1, 4>(a, max_len, split, s) : few<T, DIM, GROUP, 2, 4>(a, max_len, split, s);
+  }
+  constexpr int MT = DIM == 64 ? 2 : 1;
+  const int mw = rows <= 32 * MT ? 2 : 4;
+  const long long ctas = items * ((rows + 16 * MT * mw - 1) / (16 * MT * mw));
+  while (split < 8 && ctas * split < 2 * num_sms() && units >= 8 * split) split *= 2;
+  return mw == 2 ? many<T, DIM, GROUP, MT, 2>(a, max_len, split, s) : many<T, DIM, GROUP, MT, 4>(a, max_len, split, s);
 }
 
 }  // namespace
@@ -633,18 +1083,35 @@ extern "C" int lx_kv_attention(const lx_kv_cache* c, int32_t layer, const lx_kv_
   if (rows->max_rows == 0 || rows->total == 0) return LX_OK;
   OnDevice on(c->device);
   if (!on.ok()) return LX_ERR_CUDA;
-  const Call a{c,   rows, layer,  q_heads, q,       q_row, q_head, out,
-               o_row, o_head, lse, scale, Mask{chunk, left}, max_len, static_cast<cudaStream_t>(stream)};
+  Args a;
+  a.c = *c;
+  a.r = *rows;
+  a.layer = layer;
+  a.q_heads = q_heads;
+  a.per = q_heads / c->kv_heads;
+  a.block_lg = c->page == 16 ? 0 : c->page == 32 ? 1 : c->page == 64 ? 2 : 3;
+  a.q = q;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.wide = aligned(q, 16) && q_row % 8 == 0 && q_head % 8 == 0;
+  a.out = out;
+  a.o_row = o_row;
+  a.o_head = o_head;
+  a.lse = lse;
+  a.scale = scale;
+  a.mask = Mask{chunk, left};
+  const int most = max_len > 0 && max_len < c->max_pages * c->page ? max_len : c->max_pages * c->page;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   bool ok = false;
   switch ((dtype == LX_KV_FP16) * 4 + (c->head_dim == 128) * 2 + (c->group == 64)) {
-    case 0: ok = go<lx::bf16, 64, 32>(a); break;
-    case 1: ok = go<lx::bf16, 64, 64>(a); break;
-    case 2: ok = go<lx::bf16, 128, 32>(a); break;
-    case 3: ok = go<lx::bf16, 128, 64>(a); break;
-    case 4: ok = go<__half, 64, 32>(a); break;
-    case 5: ok = go<__half, 64, 64>(a); break;
-    case 6: ok = go<__half, 128, 32>(a); break;
-    case 7: ok = go<__half, 128, 64>(a); break;
+    case 0: ok = go<lx::bf16, 64, 32>(a, most, s); break;
+    case 1: ok = go<lx::bf16, 64, 64>(a, most, s); break;
+    case 2: ok = go<lx::bf16, 128, 32>(a, most, s); break;
+    case 3: ok = go<lx::bf16, 128, 64>(a, most, s); break;
+    case 4: ok = go<__half, 64, 32>(a, most, s); break;
+    case 5: ok = go<__half, 64, 64>(a, most, s); break;
+    case 6: ok = go<__half, 128, 32>(a, most, s); break;
+    case 7: ok = go<__half, 128, 64>(a, most, s); break;
   }
   return ok ? LX_OK : LX_ERR_CUDA;
 }
