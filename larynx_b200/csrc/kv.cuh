@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "../../include/larynx_kv.h"
+#include "common.cuh"
 #include "kernels.h"
 
 namespace lx {
@@ -35,11 +36,11 @@ __device__ __forceinline__ size_t block_at(const lx_kv_cache& c, int layer, int 
 
 __device__ __forceinline__ void flag(const lx_kv_cache& c, int bit) { atomicOr(c.error, bit); }
 
-// Length of a slot, clamped to what its table can hold.
-__device__ __forceinline__ int length_of(const lx_kv_cache& c, int slot) {
-  const int len = c.lengths[slot], most = c.max_pages * c.page;
-  return len < 0 ? 0 : len > most ? most : len;
+// A length, clamped to what a slot's table can hold.
+__device__ __forceinline__ int clamp_length(const lx_kv_cache& c, int len) {
+  return min(max(len, 0), c.max_pages * c.page);
 }
+__device__ __forceinline__ int length_of(const lx_kv_cache& c, int slot) { return clamp_length(c, c.lengths[slot]); }
 
 __device__ __forceinline__ int pages_of(const lx_kv_cache& c, int tokens) { return (tokens + c.page - 1) / c.page; }
 
@@ -47,15 +48,17 @@ __device__ __forceinline__ int pages_of(const lx_kv_cache& c, int tokens) { retu
 struct Entry {
   int slot, row0, rows;
 };
-__device__ __forceinline__ Entry entry_of(const lx_kv_cache& c, const lx_kv_rows& r, int i) {
+// (`slot`, and `from`, `to` where row0 is given: the words that entry i has in memory.)
+__device__ __forceinline__ Entry entry_of(const lx_kv_cache& c, const lx_kv_rows& r, int slot, int from, int to,
+                                          int i) {
   Entry e;
-  e.slot = r.seqs ? r.seqs[i] : i;
-  if (e.slot < 0 || e.slot >= c.n_seq) {
+  e.slot = slot;
+  if (slot < 0 || slot >= c.n_seq) {
     e.slot = -1;
     flag(c, LX_KV_SLOT);
   }
-  long long first = r.row0 ? r.row0[i] : static_cast<long long>(i) * r.max_rows;
-  long long end = r.row0 ? r.row0[i + 1] : first + r.max_rows;
+  long long first = r.row0 ? from : static_cast<long long>(i) * r.max_rows;
+  long long end = r.row0 ? to : first + r.max_rows;
   if (first < 0 || end < first || end > r.total || end - first > r.max_rows) {
     flag(c, LX_KV_ROWS);
     first = first < 0 ? 0 : first;
@@ -67,11 +70,17 @@ __device__ __forceinline__ Entry entry_of(const lx_kv_cache& c, const lx_kv_rows
   return e;
 }
 
+__device__ __forceinline__ Entry entry_of(const lx_kv_cache& c, const lx_kv_rows& r, int i) {
+  return entry_of(c, r, r.seqs ? r.seqs[i] : i, r.row0 ? r.row0[i] : 0, r.row0 ? r.row0[i + 1] : 0, i);
+}
+
 // Position of the first row of entry i, or LX_KV_REFUSED.  (Clamped so that sums
 // with row counts stay in 32 bits; no sequence reaches that far.)
-__device__ __forceinline__ int start_of(const lx_kv_rows& r, int i, int len, int rows) {
-  const int s = r.start ? r.start[i] : len - rows;
+__device__ __forceinline__ int clamp_start(int s) {
   return s == LX_KV_REFUSED ? s : min(max(s, -MAX_ROWS), MAX_TOKENS);
+}
+__device__ __forceinline__ int start_of(const lx_kv_rows& r, int i, int len, int rows) {
+  return clamp_start(r.start ? r.start[i] : len - rows);
 }
 
 // ---- host side ---------------------------------------------------------------
@@ -118,8 +127,10 @@ class OnDevice {
   bool ok_ = false, changed_ = false;
 };
 
-// A plain launch with its own status (not the thread's last error, which may
-// be another call's).
+// A launch with its own status (not the thread's last error, which may be another
+// call's), with programmatic serialization: every kernel of the cache calls
+// pdl_launch_dependents and pdl_wait (common.cuh) before it reads memory, so that
+// its launch overlaps the end of the one before.
 template <typename... KArgs, typename... Args>
 inline bool launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
@@ -127,6 +138,11 @@ inline bool launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) == cudaSuccess;
 }
 

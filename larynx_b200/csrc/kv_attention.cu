@@ -12,12 +12,12 @@
 // product with the constant 8 takes off what the centring needs, of the same
 // rounded values.  q is scaled by a power of two so that the largest value of
 // the rows is near 2^13 (what fp16 loses is below 2^-38 of that).  p is taken times a
-// power of two F that brings the largest step of V so far to 2^11: p s F stays
-// below 2^15, and what fp16 rounds away is 2^-11 of each term, or 2^-36 of
+// power of two F that brings the largest step of V so far to 2^7: p s F stays
+// below 2^15, and what fp16 rounds away is 2^-11 of each term, or 2^-32 of
 // the largest.  F cancels in the quotient.
 //
 // The maximum is raised, and the sums rescaled, only when a score exceeds it by
-// 4 (log2 units), so p <= 2^4; likewise F only when a step exceeds its bound.
+// 8 (log2 units), so p <= 2^8; likewise F only when a step exceeds its bound.
 //
 // Two forms, by the rows (query rows x query heads of one kv head) of an entry:
 // k_kv_few for up to 16, whose warps all split the keys, and k_kv_many, whose warps
@@ -28,6 +28,7 @@
 #include <cooperative_groups.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv.cuh"
@@ -41,8 +42,8 @@ namespace {
 constexpr int UNIT = 32;  // keys of a step: two blocks
 constexpr uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u;
 constexpr uint32_t EIGHTS = 0x00080008u;
-constexpr float RAISE = 4.0f;         // log2 units by which a score may exceed the running maximum
-constexpr int P_TOP = 11;             // F x the largest step is 2^11 at most: 2^4 x 2^11 stays below 2^15
+constexpr float RAISE = 8.0f;         // log2 units by which a score may exceed the running maximum
+constexpr int P_TOP = 7;              // F x the largest step is 2^7 at most: 2^8 x 2^7 does not exceed 2^15
 constexpr float STEP_MIN = 8.0779357e-28f;  // 2^-90: F stays below 2^101, so that sums of p F do not overflow
 constexpr float STEP_MAX = 8.5070592e37f;   // 2^126
 
@@ -136,19 +137,25 @@ struct Args {
   Mask mask;
 };
 
-// Eight neighbouring channels of the query.
+// Eight neighbouring channels of the query, loaded and converted in two steps.
 template <typename T>
-__device__ __forceinline__ void query8(const T* p, bool wide, float (&x)[8]) {
-  if (wide) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
+struct Raw8 {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p, bool wide) {
+    if (wide) {
+      v = *reinterpret_cast<const uint4*>(p);
+    } else {
+      T* t = reinterpret_cast<T*>(&v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
     const T* t = reinterpret_cast<const T*>(&v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(t[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(p[i]);
   }
-}
+};
 
 // The exponent by which the rows are scaled: 2^e times their largest finite value lies in [2^13, 2^14).
 __device__ __forceinline__ int query_exponent(float top) {
@@ -169,16 +176,21 @@ struct Share {
     head = item % a.c.kv_heads;
     item /= a.c.kv_heads;
     const int tile = item % a.tiles, entry = item / a.tiles;
-    e = entry_of(a.c, a.r, entry);
+    // the entry's words in flight together
+    const int slot = a.r.seqs ? a.r.seqs[entry] : entry;
+    const bool ok = slot >= 0 && slot < a.c.n_seq;
+    const int length = a.c.lengths[ok ? slot : 0], given = a.r.start ? a.r.start[entry] : 0;
+    const int first = a.r.row0 ? a.r.row0[entry] : 0, end = a.r.row0 ? a.r.row0[entry + 1] : 0;
+    e = entry_of(a.c, a.r, slot, first, end, entry);
     rows = e.rows * a.per;
     row0 = tile * tile_rows;
     if (row0 >= rows) return false;  // for the whole cluster
     n_rows = min(tile_rows, rows - row0);
     len = 0;
     start = LX_KV_REFUSED;
-    if (e.slot >= 0) {
-      len = length_of(a.c, e.slot);
-      start = start_of(a.r, entry, len, e.rows);
+    if (ok) {
+      len = clamp_length(a.c, length);
+      start = clamp_start(a.r.start ? given : len - e.rows);
     }
     return true;
   }
@@ -205,14 +217,19 @@ struct Ring {
   uint32_t smem;        // this ring's first stage
   int next, n_blocks;   // next unit to load; blocks below this one exist
   int page[2];          // of its blocks, looked up one unit ahead; -2: no such block
+  int first[STAGES - 1][2];  // the same of the first units, looked up at once
   uint32_t got;         // two bits a loaded unit, the last in the lowest place: which blocks are there
   int* error;
 
-  __device__ __forceinline__ void look_up() {
+  __device__ __forceinline__ void look_up(int unit, int (&page)[2]) const {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) page[b] = 2 * next + b < n_blocks ? table[(2 * next + b) >> block_lg] : -2;
+    for (int b = 0; b < 2; ++b) page[b] = 2 * unit + b < n_blocks ? table[(2 * unit + b) >> block_lg] : -2;
   }
   __device__ __forceinline__ void load(int stage) {
+    bring(stage, page);
+    look_up(next, page);
+  }
+  __device__ __forceinline__ void bring(int stage, const int (&page)[2]) {
     got <<= 2;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -232,7 +249,6 @@ struct Ring {
     }
     cp_async_commit();
     next += STRIDE;
-    look_up();
   }
   __device__ __forceinline__ void start(const Args& a, const Share& s, int unit, int unit_end, int hi, uint8_t* stages,
                                         int thread) {
@@ -249,9 +265,13 @@ struct Ring {
     n_blocks = min(2 * unit_end, (hi + BLOCK - 1) / BLOCK);
     got = 0;
     error = a.c.error;
-    look_up();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(i);
+    for (int i = 0; i < STAGES - 1; ++i) look_up(unit + i * STRIDE, first[i]);
+    look_up(unit + (STAGES - 1) * STRIDE, page);
+  }
+  __device__ __forceinline__ void fill() {
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) bring(i, first[i]);
   }
 };
 
@@ -342,7 +362,7 @@ struct FewShape {
 };
 
 template <typename T, int DIM, int GROUP, int NT, int KW>
-__global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)) k_kv_few(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / KW - (NT - 1)) k_kv_few(const __grid_constant__ Args a) {
   using S = FewShape<DIM, GROUP, NT, KW>;
   constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -372,15 +392,22 @@ __global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)
   float2 qs[NT][G];  // sums over a group's channels of rows 2 j, 2 j + 1, times scale log2(e)
   float c1;
   {
-    float x[NT][H][2][8], top = 0.0f;
+    Raw8<T> raw[NT][H][2];
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
       const T* p = s.query<T>(a, 8 * r + n) + 8 * j;
 #pragma unroll
+      for (int hw = 0; hw < 2 * H; ++hw) raw[r][hw / 2][hw % 2].load(p + 32 * hw, a.wide);
+    }
+    ring.fill();
+    float x[NT][H][2][8], top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < NT; ++r) {
+#pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          query8(p + 64 * h + 32 * w, a.wide, x[r][h][w]);
+          raw[r][h][w].get(x[r][h][w]);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float y = fabsf(x[r][h][w][i]);
@@ -449,6 +476,9 @@ __global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)
     stage = stage + 1 == S::STAGES ? 0 : stage + 1;
     const int key0 = unit * UNIT;
 
+    // PART: not every row sees every key of the unit (a body of its own, so that the others carry no selects)
+    auto body = [&](auto tag) {
+    constexpr bool PART = decltype(tag)::value;
     // scores in log2 units, of (rows 2 j, 2 j + 1): s2[block][r][key n or n + 8]
     float2 s2[2][NT][2];
 #pragma unroll
@@ -477,11 +507,12 @@ __global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const uint32_t p = lds32(d + param_offset(DIM) + 64 * g + slot + 8 * t);
-          const float2 ks = both(step_of(p) * c1), km = both(low_of(p));
+          const float ks = step_of(p) * c1, km = low_of(p);
 #pragma unroll
           for (int r = 0; r < NT; ++r) {
-            const float2 base = g == 0 ? __fmul2_rn(qs[r][g], km) : __ffma2_rn(qs[r][g], km, s2[b][r][t]);
-            s2[b][r][t] = __ffma2_rn(make_float2(raw[r][2 * t], raw[r][2 * t + 1]), ks, base);
+            float2& y = s2[b][r][t];
+            y.x = fmaf(raw[r][2 * t], ks, g == 0 ? qs[r][g].x * km : fmaf(qs[r][g].x, km, y.x));
+            y.y = fmaf(raw[r][2 * t + 1], ks, g == 0 ? qs[r][g].y * km : fmaf(qs[r][g].y, km, y.y));
           }
         }
       }
@@ -498,10 +529,8 @@ __global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)
           vs[b][g][t] = step_of(p);
           vm[b][g][t] = fmaf(vs[b][g][t], 8.0f, low_of(p));
         }
-    const bool part = got != 3u || key0 < lo_all || key0 + UNIT > hi_all;
-    uint32_t seen = 0xFFFFFFFFu;  // bit 4 NT b + 4 r + 2 t + x
-    if (part) {
-      seen = 0;
+    uint32_t seen = 0;  // bit 4 NT b + 4 r + 2 t + x
+    if (PART) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -583,13 +612,14 @@ __global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)
           l[r] = __fadd2_rn(l[r], p);
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            float2 w = __fmul2_rn(p, both(vs[b][g][t])), low = both(vm[b][g][t]);
-            if (part) {  // a key that a row does not see: not even its NaN counts
+            float2 w = make_float2(p.x * vs[b][g][t], p.y * vs[b][g][t]), low = both(vm[b][g][t]);
+            if (PART) {  // a key that a row does not see: not even its NaN counts
               const uint32_t in = seen >> (4 * NT * b + 4 * r + 2 * t);
               if (!(in & 1)) w.x = low.x = 0.0f;
               if (!(in & 2)) w.y = low.y = 0.0f;
             }
-            z[r][g] = __ffma2_rn(p, low, z[r][g]);
+            z[r][g].x = fmaf(p.x, low.x, z[r][g].x);
+            z[r][g].y = fmaf(p.y, low.y, z[r][g].y);
             pb[r][g][t] = transpose8(half_pair(w));
           }
         }
@@ -611,6 +641,11 @@ __global__ void __launch_bounds__(32 * KW, (DIM == 64 ? 16 : 12) / KW - (NT - 1)
         }
       }
     }
+    };
+    if (got != 3u || key0 < lo_all || key0 + UNIT > hi_all)
+      body(std::true_type());
+    else
+      body(std::false_type());
   }
   cp_async_wait<0>();
   __syncthreads();  // every ring has been read: the joining takes their place
@@ -672,7 +707,7 @@ struct ManyShape {
 };
 
 template <typename T, int DIM, int GROUP, int MT, int MW>
-__global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_kv_many(const __grid_constant__ Args a) {
   using S = ManyShape<DIM, GROUP, MT, MW>;
   constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -703,17 +738,26 @@ __global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Arg
   float qs[MT][2][G];
   float c1;
   {
-    float x[MT][2][H][2][8], top = 0.0f;
+    Raw8<T> raw[MT][2][H][2];
 #pragma unroll
     for (int r = 0; r < MT; ++r)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const T* p = s.query<T>(a, warp_row + 16 * r + n + 8 * u) + 8 * j;
 #pragma unroll
+        for (int hw = 0; hw < 2 * H; ++hw) raw[r][u][hw / 2][hw % 2].load(p + 32 * hw, a.wide);
+      }
+    ring.fill();
+    float x[MT][2][H][2][8], top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            query8(p + 64 * h + 32 * w, a.wide, x[r][u][h][w]);
+            raw[r][u][h][w].get(x[r][u][h][w]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float y = fabsf(x[r][u][h][w][i]);
@@ -788,6 +832,8 @@ __global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Arg
     for (int b = 0; b < 2; ++b) {
       const int key0 = unit * UNIT + 16 * b;
       if (key0 >= hi_warp || key0 + 16 <= lo_warp || !(got >> b & 1)) continue;
+      auto body = [&](auto tag) {
+      constexpr bool PART = decltype(tag)::value;  // not every row of the warp sees every key
       const uint8_t* d = data + b * BB;
       float2 s2[MT][2][2];  // scores in log2 units: [rows 16 r + n, + 8][keys 2 j + {0, 1}, {8, 9}]
 #pragma unroll
@@ -839,10 +885,8 @@ __global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Arg
           vm[g][t] = __ffma2_rn(vs[g][t], both(8.0f), make_float2(low_of(p0), low_of(p1)));
         }
       }
-      const bool part = key0 < lo_all || key0 + 16 > hi_all;
-      uint32_t seen = 0xFFFFFFFFu;  // bit 8 r + 4 u + 2 t + x
-      if (part) {
-        seen = 0;
+      uint32_t seen = 0;  // bit 8 r + 4 u + 2 t + x
+      if (PART) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -922,7 +966,7 @@ __global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Arg
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               float2 w = __fmul2_rn(p, vs[g][t]), low = vm[g][t];
-              if (part) {  // a key that a row does not see: not even its NaN counts
+              if (PART) {  // a key that a row does not see: not even its NaN counts
                 const uint32_t in = seen >> (8 * r + 4 * u + 2 * t);
                 if (!(in & 1)) w.x = low.x = 0.0f;
                 if (!(in & 2)) w.y = low.y = 0.0f;
@@ -951,6 +995,11 @@ __global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Arg
           }
         }
       }
+      };
+      if (key0 < lo_all || key0 + 16 > hi_all)
+        body(std::true_type());
+      else
+        body(std::false_type());
     }
   }
   cp_async_wait<0>();
@@ -1002,49 +1051,83 @@ __global__ void __launch_bounds__(32 * MW) k_kv_many(const __grid_constant__ Arg
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Launches over tiles of `tile_rows` rows, the keys of each split over a cluster.
+// What a kernel needs to be launched on one device: set up at its first call.
+struct Launch {
+  bool ready = false;
+  int active[17];  // clusters of 1 .. 16 CTAs that the GPU holds at once
+};
+
 template <typename K>
-bool start(K kernel, Args& a, bool* ready, int threads, int smem, int tile_rows, int max_len, int split,
-           cudaStream_t s) {
-  bool& done = ready[a.c.device & 63];
-  if (!done) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return false;
-    done = true;
-  }
-  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per + tile_rows - 1) / tile_rows;
-  const long long ctas = tiles * a.r.n * a.c.kv_heads * split;
-  if (ctas > 0x7fffffff) return false;
-  a.tiles = static_cast<int>(tiles);
-  a.split = split;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+void set_up(K kernel, Launch& l, int threads, int smem, cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr) {
+  cfg = cudaLaunchConfig_t{};
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = split;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 2 : 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  if (l.ready) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return;
+  for (int k = 1; k <= 16; ++k) {
+    cfg.gridDim = dim3(k);
+    attr[0].val.clusterDim.x = k;
+    cfg.numAttrs = 1;
+    l.active[k] = 0;
+    if (cudaOccupancyMaxActiveClusters(&l.active[k], kernel, &cfg) != cudaSuccess) {
+      l.active[k] = 0;
+      cudaGetLastError();
+    }
+  }
+  l.ready = l.active[1] > 0;
+}
+
+// Launches `items` (tiles of rows x kv heads) with the keys of each split over a
+// cluster: as finely as all items still run at once and each key group has a
+// unit (`groups` a CTA); where even whole items do not all run at once, into twice as many
+// CTAs as do, so that the last ones leave little of the GPU idle.
+template <typename K>
+bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_rows, int groups, int units,
+           cudaStream_t s) {
+  Launch& l = launches[a.c.device & 63];
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  set_up(kernel, l, threads, smem, cfg, attr);
+  if (!l.ready) return false;
+  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per + tile_rows - 1) / tile_rows;
+  const long long items = tiles * a.r.n * a.c.kv_heads;
+  const int most = min(16, (units + groups - 1) / groups);
+  int split = 1;
+  for (int k = 2; k <= most; ++k)
+    if (l.active[k] >= items) split = k;
+  if (split == 1 && items > l.active[1] / 2 && items < 2 * l.active[1] && most >= 8) split = 2;
+  if (items * split > 0x7fffffff) return false;
+  a.tiles = static_cast<int>(tiles);
+  a.split = split;
+  cfg.gridDim = dim3(static_cast<unsigned>(items * split));
+  cfg.stream = s;
+  attr[0].val.clusterDim.x = split;
+  cfg.numAttrs = 2;
+  if (split == 1) {
+    cfg.attrs = attr + 1;
+    cfg.numAttrs = 1;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess;
 }
 
 template <typename T, int DIM, int GROUP, int NT, int KW>
-bool few(Args& a, int max_len, int split, cudaStream_t s) {
+bool few(Args& a, int units, cudaStream_t s) {
   using S = FewShape<DIM, GROUP, NT, KW>;
-  static bool ready[64] = {false};
-  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, ready, S::THREADS, S::SMEM, S::ROWS, max_len, split, s);
+  static Launch launches[64];
+  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, s);
 }
 template <typename T, int DIM, int GROUP, int MT, int MW>
-bool many(Args& a, int max_len, int split, cudaStream_t s) {
+bool many(Args& a, int units, cudaStream_t s) {
   using S = ManyShape<DIM, GROUP, MT, MW>;
-  static bool ready[64] = {false};
-  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, ready, S::THREADS, S::SMEM, S::ROWS, max_len, split, s);
+  static Launch launches[64];
+  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 4, units, s);
 }
 
 template <typename T, int DIM, int GROUP>
@@ -1052,17 +1135,14 @@ bool go(Args& a, int max_len, cudaStream_t s) {
   const long long rows = static_cast<long long>(a.r.max_rows) * a.per;
   const long long items = static_cast<long long>(a.r.n) * a.c.kv_heads;
   const int units = (max_len + UNIT - 1) / UNIT;
-  int split = 1;
   if (rows <= 16) {
-    // as many CTAs as make four rounds of the GPU, as long as every warp has two units
-    while (split < 16 && items * split < 4 * num_sms() * (DIM == 64 ? 4 : 3) && units >= 2 * 4 * 2 * split) split *= 2;
-    return rows <= 8 ? few<T, DIM, GROUP, 1, 4>(a, max_len, split, s) : few<T, DIM, GROUP, 2, 4>(a, max_len, split, s);
+    // CTAs of four warps, or where clusters of sixteen of them leave the GPU empty, of as many as an SM holds
+    constexpr int WIDE = DIM == 64 ? 16 : 12;
+    const bool wide = items * 16 * 4 < num_sms() * 8 && units > 4 * 16;
+    if (rows <= 8) return wide ? few<T, DIM, GROUP, 1, WIDE>(a, units, s) : few<T, DIM, GROUP, 1, 4>(a, units, s);
+    return wide ? few<T, DIM, GROUP, 2, 8>(a, units, s) : few<T, DIM, GROUP, 2, 4>(a, units, s);
   }
-  constexpr int MT = DIM == 64 ? 2 : 1;
-  const int mw = rows <= 32 * MT ? 2 : 4;
-  const long long ctas = items * ((rows + 16 * MT * mw - 1) / (16 * MT * mw));
-  while (split < 8 && ctas * split < 2 * num_sms() && units >= 8 * split) split *= 2;
-  return mw == 2 ? many<T, DIM, GROUP, MT, 2>(a, max_len, split, s) : many<T, DIM, GROUP, MT, 4>(a, max_len, split, s);
+  return rows <= 32 ? many<T, DIM, GROUP, 1, 2>(a, units, s) : many<T, DIM, GROUP, 1, 4>(a, units, s);
 }
 
 }  // namespace

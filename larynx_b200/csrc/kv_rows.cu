@@ -1,15 +1,16 @@
 // Writing rows into the 4-bit cache and reading them back.
 //
-// A warp takes one block (16 tokens) of one head, K and V.  Lane (n, j),
-// n = lane / 4, j = lane % 4, works on tokens n and n + 8 and on channels
+// A warp takes one block (16 tokens) of one head, K or V.  In writing, lane
+// (n, j), n = lane / 4, j = lane % 4, works on tokens n and n + 8 and on channels
 // 64 h + 32 w + 8 j + {0..7}: the codes that the lane holds of the K fragment,
-// so K needs no exchange; V's codes pass through shared memory.  Both sides of
-// memory move in pieces of 8 to 32 bytes a lane.
+// so K needs no exchange; V's codes pass through shared memory.  In reading, V is
+// taken as it lies: lane (n, j) holds tokens 2 j + {0, 1, 8, 9} and channels
+// 64 h + 32 w + 4 n + {0..3}.  All of a lane's loads are in flight before the first is used.
 //
 // Quantising, per token and group (include/larynx_kv.h): the codes are those
 // of exact arithmetic.  x - m is taken with its rounding error (two-sum), the
-// quotient from the reciprocal of s, and where the remainder d - c s comes
-// within a hair of s / 2 the decision is made on the exact remainder.
+// quotient from the reciprocal of s, and where one of eight remainders d - c s comes
+// within a hair of s / 2 the decisions are made again on the exact remainders.
 #include <cfloat>
 
 #include "kv.cuh"
@@ -26,10 +27,20 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
   return c;
 }
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float c;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
   return c;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // The rounding error of d = fl(a - b).
@@ -83,24 +94,41 @@ __device__ __forceinline__ Params params_of(float lo, float hi) {
   return p;
 }
 
-// The code of x: rint((x - m) / s) in exact arithmetic, ties to even.  With
-// c = rint(fl(x - m) / s), the remainder e = fl(x - m) - c s is exact (a multiple of the
-// smaller ulp, at most about s / 2); only where |e| reaches s / 2 can the
-// rounding of the quotient, or of x - m, have decided wrongly.
-__device__ __forceinline__ uint32_t code_of(float x, const Params& p) {
-  const float d = x - p.m;
-  float t = fmaf(d, p.inv, MAGIC);
+// rint((x - m) / s) + MAGIC in exact arithmetic, ties to even, given d = fl(x - m) and t, the same from the rounded quotient.
+__device__ __noinline__ float exact_code(float x, float d, float t, float m, float s) {
   float c = t - MAGIC;
-  const float e = fmaf(-c, p.s, d);
-  if (2.0f * fabsf(e) >= 0.99999f * p.s) {
-    const float rest = diff_error(x, p.m, d), h = 0.5f * p.s;
-    const bool odd = __float_as_uint(t) & 1u;
-    if (e > h || (e == h && (rest > 0.0f || (rest == 0.0f && odd)))) c += 1.0f;
-    if (e < -h || (e == -h && (rest < 0.0f || (rest == 0.0f && odd)))) c -= 1.0f;
-    c = fminf(fmaxf(c, 0.0f), 15.0f);
-    t = c + MAGIC;
+  const float e = fmaf(-c, s, d), rest = diff_error(x, m, d), h = 0.5f * s;
+  const bool odd = __float_as_uint(t) & 1u;
+  if (e > h || (e == h && (rest > 0.0f || (rest == 0.0f && odd)))) c += 1.0f;
+  if (e < -h || (e == -h && (rest < 0.0f || (rest == 0.0f && odd)))) c -= 1.0f;
+  return fminf(fmaxf(c, 0.0f), 15.0f) + MAGIC;
+}
+
+// The codes of eight values, code i at bit K ? 4 (i / 2) + 16 (i % 2) : 4 i.  With c = rint(fl(x - m) / s), the
+// remainder e = fl(x - m) - c s is exact (a multiple of the smaller ulp, at most about s / 2); only where |e| reaches
+// s / 2 can the rounding of the quotient, or of x - m, have decided wrongly.  MAGIC + c has c in its low bits, so a sum
+// of products with powers of 16 packs the codes; what MAGIC adds is taken off at the end.
+template <bool K>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], const Params& p) {
+  float d[8], t[8], far = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    d[i] = x[i] - p.m;
+    t[i] = fmaf(d[i], p.inv, MAGIC);
+    far = fmaxf(far, fabsf(fmaf(MAGIC - t[i], p.s, d[i])));
   }
-  return __float_as_uint(t) & 15u;
+  if (2.0f * far >= 0.99999f * p.s) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = exact_code(x[i], d[i], t[i], p.m, p.s);
+  }
+  uint32_t bits = 0, magic = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t by = 1u << (K ? 4 * (i / 2) + 16 * (i % 2) : 4 * i);
+    bits += __float_as_uint(t[i]) * by;
+    magic += 0x4B400000u * by;
+  }
+  return bits - magic;
 }
 
 template <typename T>
@@ -132,34 +160,51 @@ __device__ __forceinline__ float from_f32(float x) {
   return x;
 }
 
-// Eight neighbouring elements; `wide`: 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool wide, float (&x)[8]) {
-  if (wide) {
-    constexpr int N = sizeof(T) / 2;
-    uint4 u[N];
+// N neighbouring elements, N sizeof(T) a multiple of 8 bytes; `wide`: the address is as aligned as the widest access.
+template <typename T, int N>
+struct Pack {
+  static constexpr int BYTES = N * static_cast<int>(sizeof(T));
+  __align__(16) T e[BYTES >= 16 ? N : 16 / sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, bool wide) {
+    if (wide) {
+      if (BYTES == 8) {
+        *reinterpret_cast<uint2*>(e) = __ldg(reinterpret_cast<const uint2*>(p));
+      } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const T* e = reinterpret_cast<const T*>(u);
+        for (int i = 0; i < BYTES / 16; ++i)
+          reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+      for (int i = 0; i < N; ++i) e[i] = p[i];
+    }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, bool wide, const float (&x)[8]) {
-  if (wide) {
-    constexpr int N = sizeof(T) / 2;
-    __align__(16) T e[8];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+    for (int i = 0; i < N; ++i) e[i] = from_f32<T>(0.0f);
+  }
+  __device__ __forceinline__ void store(T* p, bool wide) const {
+    if (wide) {
+      if (BYTES == 8) {
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+      } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
-  } else {
+        for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(x[i]);
+      for (int i = 0; i < N; ++i) p[i] = e[i];
+    }
+  }
+};
+
+// Codes 0..3 of a 16-bit field (the low half of `word`) as floats: with the exponent of 2^(23 - 4 i) above it, code i
+// stands at the units of the float's mantissa.
+__device__ __forceinline__ void codes_f32(uint32_t word, float (&c)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t one = static_cast<uint32_t>(127 + 23 - 4 * i) << 23;
+    c[i] = __uint_as_float((word & (15u << (4 * i))) | one) - __uint_as_float(one);
   }
 }
 
@@ -173,16 +218,22 @@ struct Span {
 // The b-th block that entry i touches; false when there is none.
 __device__ __forceinline__ bool span_of(const lx_kv_cache& c, const lx_kv_rows& r, int layer, int i, int b, int head,
                                         bool writes, Span& s) {
-  s.e = entry_of(c, r, i);
-  if (s.e.slot < 0 || s.e.rows == 0) return false;
-  s.len = length_of(c, s.e.slot);
-  s.start = start_of(r, i, s.len, s.e.rows);
+  // the entry's words in flight together
+  const int slot = r.seqs ? r.seqs[i] : i;
+  const bool ok = slot >= 0 && slot < c.n_seq;
+  const int length = c.lengths[ok ? slot : 0], given = r.start ? r.start[i] : 0;
+  const int from = r.row0 ? r.row0[i] : 0, to = r.row0 ? r.row0[i + 1] : 0;
+  s.e = entry_of(c, r, slot, from, to, i);
+  s.start = 0;
+  if (!ok || s.e.rows == 0) return false;
+  s.len = clamp_length(c, length);
+  s.start = clamp_start(r.start ? given : s.len - s.e.rows);
   if (s.start == LX_KV_REFUSED) return false;  // an entry that was not served
   s.pos0 = (s.start & ~(BLOCK - 1)) + b * BLOCK;
   if (s.pos0 >= s.start + s.e.rows) return false;
   s.page = -1;
   if (s.pos0 >= 0 && s.pos0 < s.len) {
-    s.page = c.table[static_cast<size_t>(s.e.slot) * c.max_pages + s.pos0 / c.page];
+    s.page = c.table[static_cast<size_t>(slot) * c.max_pages + s.pos0 / c.page];
     if (s.page < 0 || s.page >= c.n_pages) {
       flag(c, LX_KV_PAGE);
       s.page = -1;
@@ -197,115 +248,123 @@ __device__ __forceinline__ bool span_of(const lx_kv_cache& c, const lx_kv_rows& 
   return true;
 }
 
+// The block, head and side (K or V) of this warp.
+struct Work {
+  int entry, b, head, kv;
+  bool any;
+};
+__device__ __forceinline__ Work work_of(const lx_kv_rows& r, int blocks) {
+  Work w;
+  const unsigned item = blockIdx.x * (WARPS / 2) + threadIdx.x / 64;
+  w.entry = item / blocks;
+  w.b = item - w.entry * blocks;
+  w.head = blockIdx.y;
+  w.kv = threadIdx.x / 32 % 2;
+  w.any = w.entry < r.n;
+  return w;
+}
+
 template <typename T, int DIM, int GROUP>
 __global__ void __launch_bounds__(32 * WARPS)
     k_kv_write(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, const T* __restrict__ k, int64_t k_row,
                int64_t k_head, const T* __restrict__ v, int64_t v_row, int64_t v_head, bool wide) {
   constexpr int H = DIM / 64, G = DIM / GROUP;
-  __shared__ __align__(16) uint16_t sv[WARPS][H * 256];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4, head = blockIdx.y;
-  const long long item = static_cast<long long>(blockIdx.x) * WARPS + warp;
-  if (item >= static_cast<long long>(r.n) * blocks) return;
+  __shared__ __align__(16) uint16_t sv[WARPS / 2][H * 256];
+  const int pair = threadIdx.x / 64, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Work w = work_of(r, blocks);
   Span s;
-  if (!span_of(c, r, layer, static_cast<int>(item / blocks), static_cast<int>(item % blocks), head, true, s)) return;
+  if (!w.any || !span_of(c, r, layer, w.entry, w.b, w.head, true, s)) return;
   // tokens of the block that this entry writes (and that lie in the sequence)
   const int first = max(s.start - s.pos0, 0), past = min(min(s.start + s.e.rows, s.len) - s.pos0, BLOCK);
   if ((s.start < 0 || s.start + s.e.rows > s.len) && lane == 0) flag(c, LX_KV_ROWS);
   if (s.page < 0 || past <= first) return;
   uint8_t* block = static_cast<uint8_t*>(c.pool) + s.at;
   const bool full = first == 0 && past == BLOCK;
+  const T* src = w.kv ? v + w.head * v_head : k + w.head * k_head;
+  const int64_t row = w.kv ? v_row : k_row;
+  Pack<T, 8> raw[2][2 * H];  // tokens n, n + 8
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const T* src = kv ? v : k;
-    const int64_t row_stride = kv ? v_row : k_row, head_stride = kv ? v_head : k_head;
+  for (int u = 0; u < 2; ++u) {
+    const int t = n + 8 * u;
+    const T* p = src + (s.e.row0 + (s.pos0 + t - s.start)) * row + 8 * j;
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      uint32_t word[2][2];  // [token n, n + 8][w]
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int t = n + 8 * u;
-        const bool mine = t >= first && t < past;
-        float x[2][8];
-        const T* p = src + (s.e.row0 + (s.pos0 + t - s.start)) * row_stride + head * head_stride + 64 * h + 8 * j;
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if (mine)
-            load8(p + 32 * w, wide, x[w]);
-          else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[w][i] = 0.0f;
-        }
-        float lo[2], hi[2];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          lo[w] = hi[w] = x[w][0];
-#pragma unroll
-          for (int i = 1; i < 8; ++i) {
-            lo[w] = min_nan(lo[w], x[w][i]);
-            hi[w] = max_nan(hi[w], x[w][i]);
-          }
-        }
-        if (GROUP == 64) {
-          lo[0] = lo[1] = min_nan(lo[0], lo[1]);
-          hi[0] = hi[1] = max_nan(hi[0], hi[1]);
-        }
-#pragma unroll
-        for (int w = 0; w < 64 / GROUP; ++w) {
-#pragma unroll
-          for (int o = 1; o < 4; o *= 2) {
-            lo[w] = min_nan(lo[w], __shfl_xor_sync(0xffffffffu, lo[w], o));
-            hi[w] = max_nan(hi[w], __shfl_xor_sync(0xffffffffu, hi[w], o));
-          }
-          const Params q = params_of(lo[w], hi[w]);
-          const int g = 64 * h / GROUP + w;
-          if (mine && j == 0)
-            *reinterpret_cast<uint32_t*>(block + param_offset(DIM) + 64 * (kv * G + g) + 4 * param_slot(t)) = q.packed;
-#pragma unroll
-          for (int w2 = w; w2 < (GROUP == 64 ? 2 : w + 1); ++w2) {
-            uint32_t bits = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t code = code_of(x[w2][i], q);
-              bits |= code << (kv ? 4 * i : 4 * (i / 2) + 16 * (i % 2));
-            }
-            word[u][w2] = bits;
-          }
-        }
-      }
-      if (!kv) {
-        uint8_t* dst = block + 512 * h + 16 * lane;
-        if (full) {
-          *reinterpret_cast<uint4*>(dst) = make_uint4(word[0][0], word[0][1], word[1][0], word[1][1]);
-        } else {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (n + 8 * u >= first && n + 8 * u < past)
-              *reinterpret_cast<uint2*>(dst + 8 * u) = make_uint2(word[u][0], word[u][1]);
-        }
-      } else {
-        // V: lane (n', j') of the fragment takes tokens 2 j' + {0, 1, 8, 9}, channels 32 w + 4 n' + {0..3}
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-              sv[warp][256 * h + ((2 * j + q) * 4 + n / 2) * 8 + 4 * u + 2 * w + n % 2] =
-                  static_cast<uint16_t>(word[u][w] >> (16 * q));
-      }
+    for (int hw = 0; hw < 2 * H; ++hw) {
+      if (t >= first && t < past)
+        raw[u][hw].load(p + 32 * hw, wide);
+      else
+        raw[u][hw].clear();
     }
   }
+  uint32_t word[2][2 * H];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = n + 8 * u;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      constexpr int PARTS = GROUP / 32;
+      float x[PARTS][8], lo = 0.0f, hi = 0.0f;
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[q][i] = to_f32(raw[u][PARTS * g + q].e[i]);
+        if (q == 0) lo = hi = x[0][0];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          lo = min_nan(lo, x[q][i], x[q][i + 1]);
+          hi = max_nan(hi, x[q][i], x[q][i + 1]);
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o *= 2) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      const Params p = params_of(lo, hi);
+      if (j == 0 && t >= first && t < past)
+        *reinterpret_cast<uint32_t*>(block + param_offset(DIM) + 64 * (w.kv * G + g) + 4 * param_slot(t)) = p.packed;
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q)
+        word[u][PARTS * g + q] = w.kv ? codes_of<false>(x[q], p) : codes_of<true>(x[q], p);
+    }
+  }
+  if (!w.kv) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      uint8_t* dst = block + 512 * h + 16 * lane;
+      if (full) {
+        *reinterpret_cast<uint4*>(dst) =
+            make_uint4(word[0][2 * h], word[0][2 * h + 1], word[1][2 * h], word[1][2 * h + 1]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (n + 8 * u >= first && n + 8 * u < past)
+            *reinterpret_cast<uint2*>(dst + 8 * u) = make_uint2(word[u][2 * h], word[u][2 * h + 1]);
+      }
+    }
+    return;
+  }
+  // V: lane (n', j') of the fragment takes tokens 2 j' + {0, 1, 8, 9}, channels 32 w + 4 n' + {0..3}
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int hw = 0; hw < 2 * H; ++hw)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        sv[pair][256 * (hw / 2) + ((2 * j + q) * 4 + n / 2) * 8 + 4 * u + 2 * (hw % 2) + n % 2] =
+            static_cast<uint16_t>(word[u][hw] >> (16 * q));
   __syncwarp();
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     uint8_t* dst = block + 512 * (H + h) + 16 * lane;
-    const uint16_t* from = &sv[warp][256 * h + 8 * lane];
+    const uint16_t* from = &sv[pair][256 * h + 8 * lane];
     if (full) {
       *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(from);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int t = 8 * (i / 4) + 2 * (lane % 4) + i % 2;
+        const int t = 8 * (i / 4) + 2 * j + i % 2;
         if (t >= first && t < past) reinterpret_cast<uint16_t*>(dst)[i] = from[i];
       }
     }
@@ -317,67 +376,82 @@ __global__ void __launch_bounds__(32 * WARPS)
     k_kv_read(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, T* __restrict__ k, int64_t k_row,
               int64_t k_head, T* __restrict__ v, int64_t v_row, int64_t v_head, bool wide) {
   constexpr int H = DIM / 64, G = DIM / GROUP;
-  __shared__ __align__(16) uint16_t sv[WARPS][H * 256];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4, head = blockIdx.y;
-  const long long item = static_cast<long long>(blockIdx.x) * WARPS + warp;
-  if (item >= static_cast<long long>(r.n) * blocks) return;
+  const int lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Work w = work_of(r, blocks);
+  if (!w.any) return;
   Span s;
-  const int entry = static_cast<int>(item / blocks), b = static_cast<int>(item % blocks);
-  if (!span_of(c, r, layer, entry, b, head, false, s)) {
+  if (!span_of(c, r, layer, w.entry, w.b, w.head, false, s)) {
     // a slot or an entry that does not exist: its rows read as 0
-    if (s.e.rows == 0 || b * BLOCK >= s.e.rows || (s.e.slot >= 0 && s.start != LX_KV_REFUSED)) return;
+    if (s.e.rows == 0 || w.b * BLOCK >= s.e.rows || (s.e.slot >= 0 && s.start != LX_KV_REFUSED)) return;
     s.start = 0;
-    s.pos0 = b * BLOCK;
+    s.pos0 = w.b * BLOCK;
     s.len = 0;
     s.page = -1;
   }
   const int first = max(s.start - s.pos0, 0), past = min(s.start + s.e.rows - s.pos0, BLOCK);
   const int held = s.page < 0 ? 0 : min(s.len - s.pos0, BLOCK);
   const uint8_t* block = static_cast<const uint8_t*>(c.pool) + (s.page < 0 ? 0 : s.at);
-  uint4 kw[H];
+  uint4 code[H];
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    kw[h] = make_uint4(0, 0, 0, 0);
-    if (held > 0) {
-      kw[h] = *reinterpret_cast<const uint4*>(block + 512 * h + 16 * lane);
-      *reinterpret_cast<uint4*>(&sv[warp][256 * h + 8 * lane]) =
-          *reinterpret_cast<const uint4*>(block + 512 * (H + h) + 16 * lane);
-    }
-  }
-  __syncwarp();
+  for (int h = 0; h < H; ++h)
+    code[h] = held > 0 ? __ldcg(reinterpret_cast<const uint4*>(block + 512 * (w.kv * H + h) + 16 * lane))
+                       : make_uint4(0, 0, 0, 0);
+  T* dst = w.kv ? v + w.head * v_head : k + w.head * k_head;
+  const int64_t row = w.kv ? v_row : k_row;
+  const uint8_t* par = block + param_offset(DIM) + 64 * G * w.kv;
+  if (!w.kv) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int t = n + 8 * u;
-    if (t < first || t >= past) continue;
-    const int64_t row = s.e.row0 + (s.pos0 + t - s.start);
+    for (int u = 0; u < 2; ++u) {
+      const int t = n + 8 * u;
+      if (t < first || t >= past) continue;
+      T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 8 * j;
+      uint32_t p[G];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv)
+      for (int g = 0; g < G; ++g)
+        p[g] = t < held ? __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(t))) : 0u;
 #pragma unroll
-      for (int h = 0; h < H; ++h)
+      for (int hw = 0; hw < 2 * H; ++hw) {
+        const uint4 x = code[hw / 2];
+        const uint32_t word = u ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
+        const float step = bf16_value(p[32 * hw / GROUP] & 0xFFFFu), low = __uint_as_float(p[32 * hw / GROUP] & 0xFFFF0000u);
+        float even[4], odd[4];
+        codes_f32(word, even);
+        codes_f32(word >> 16, odd);
+        Pack<T, 8> y;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          if (t < held) {
-            const int g = (64 * h + 32 * w) / GROUP;
-            const uint32_t p = *reinterpret_cast<const uint32_t*>(block + param_offset(DIM) + 64 * (kv * G + g) +
-                                                                  4 * param_slot(t));
-            const float step = bf16_value(p & 0xFFFFu), low = __uint_as_float(p & 0xFFFF0000u);
-            uint32_t word;
-            if (kv) {
-              const uint16_t* from = &sv[warp][256 * h + (2 * j * 4 + n / 2) * 8 + 4 * u + 2 * w + n % 2];
-              word = from[0] | static_cast<uint32_t>(from[32]) << 16;
-            } else {
-              word = u ? (w ? kw[h].w : kw[h].z) : (w ? kw[h].y : kw[h].x);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t code = word >> (kv ? 4 * i : 4 * (i / 2) + 16 * (i % 2)) & 15u;
-              x[i] = fmaf(static_cast<float>(code), step, low);
-            }
-          }
-          T* dst = kv ? v + row * v_row + head * v_head : k + row * k_row + head * k_head;
-          store8(dst + 64 * h + 32 * w + 8 * j, wide, x);
+        for (int i = 0; i < 4; ++i) {
+          y.e[2 * i] = from_f32<T>(fmaf(even[i], step, low));
+          y.e[2 * i + 1] = from_f32<T>(fmaf(odd[i], step, low));
         }
+        if (t >= held) y.clear();
+        y.store(out + 32 * hw, wide);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 2 * j + 8 * (i / 2) + i % 2;
+    if (t < first || t >= past) continue;
+    T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 4 * n;
+    uint32_t p[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      p[g] = t < held ? __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(t))) : 0u;
+#pragma unroll
+    for (int hw = 0; hw < 2 * H; ++hw) {
+      const uint4 x = code[hw / 2];
+      const uint32_t word = i / 2 ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
+      const float step = bf16_value(p[32 * hw / GROUP] & 0xFFFFu), low = __uint_as_float(p[32 * hw / GROUP] & 0xFFFF0000u);
+      float e[4];
+      codes_f32(i % 2 ? word >> 16 : word, e);
+      Pack<T, 4> y;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) y.e[q] = from_f32<T>(t < held ? fmaf(e[q], step, low) : 0.0f);
+      y.store(out + 32 * hw, wide);
+    }
   }
 }
 
@@ -391,9 +465,9 @@ bool wide_rows(const void* k, int64_t k_row, int64_t k_head, const void* v, int6
 template <typename T, int DIM, int GROUP>
 bool go(bool writes, const lx_kv_cache& c, int layer, const lx_kv_rows& r, void* k, int64_t k_row, int64_t k_head,
         void* v, int64_t v_row, int64_t v_head, cudaStream_t s) {
-  const int blocks = (r.max_rows + BLOCK - 1) / BLOCK + 1;  // rows may begin inside a block
+  const int blocks = (r.max_rows + BLOCK - 2) / BLOCK + 1;  // rows may begin inside a block
   const long long items = static_cast<long long>(r.n) * blocks;
-  const dim3 grid(static_cast<unsigned>((items + WARPS - 1) / WARPS), c.kv_heads);
+  const dim3 grid(static_cast<unsigned>((items + WARPS / 2 - 1) / (WARPS / 2)), c.kv_heads);
   const bool wide = wide_rows<T>(k, k_row, k_head, v, v_row, v_head);
   if (writes)
     return launch(k_kv_write<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks,
@@ -408,7 +482,7 @@ int rows_call(bool writes, const lx_kv_cache* c, int layer, const lx_kv_rows* r,
   if (dtype != LX_KV_BF16 && dtype != LX_KV_FP16 && dtype != LX_KV_FP32) return LX_ERR_ARG;
   const size_t size = dtype == LX_KV_FP32 ? 4 : 2;
   if (!aligned(k, size) || !aligned(v, size)) return LX_ERR_ARG;
-  const long long blocks = (static_cast<long long>(r->max_rows) + BLOCK - 1) / BLOCK + 1;
+  const long long blocks = (static_cast<long long>(r->max_rows) + BLOCK - 2) / BLOCK + 1;
   if (blocks * r->n > (static_cast<long long>(0x7fffffff) - WARPS)) return LX_ERR_ARG;
   if (r->max_rows == 0 || r->total == 0) return LX_OK;
   OnDevice on(c->device);
