@@ -367,8 +367,8 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
   constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   Share s;
   if (!s.take(a, S::ROWS)) return;
 
@@ -713,8 +713,8 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
   const int warp_row = 16 * MT * warp;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   Share s;
   if (!s.take(a, S::ROWS)) return;
 

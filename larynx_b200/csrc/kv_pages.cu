@@ -92,8 +92,8 @@ inline int hash_slots(int n) {
 template <bool COPY>
 __global__ void __launch_bounds__(PLAN_THREADS)
     k_kv_grow(const lx_kv_cache c, int n, int hash, const int* __restrict__ a, const int* __restrict__ b, int* start) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   extern __shared__ int sm[];
   int* before = sm;          // [n + 1] pages that earlier entries need
   int* slot = before + n + 1;  // [n] the sequence that grows, -1: refused
@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
 
 __global__ void __launch_bounds__(PLAN_THREADS)
     k_kv_fork(const lx_kv_cache c, int n, int hash, const int* __restrict__ src, const int* __restrict__ dst) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   extern __shared__ int sm[];
   int* len = sm;  // [n] tokens to share, -1: refused
   FirstNamed named{len + n, len + n + hash, hash - 1};
@@ -273,8 +273,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
 // One warp an entry.  Entries may name a slot twice: each table entry is taken
 // off by whoever exchanges it first, and the length takes the least keep.
 __global__ void k_kv_free(const lx_kv_cache c, int n, const int* __restrict__ seqs, const int* __restrict__ keep) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int i = (blockIdx.x * blockDim.x + threadIdx.x) / 32, lane = threadIdx.x % 32;
   if (i >= n) return;
   const int s = seqs[i], k0 = keep[i];
@@ -299,8 +299,8 @@ __global__ void k_kv_free(const lx_kv_cache c, int n, const int* __restrict__ se
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) k_kv_compact(const lx_kv_cache c, int* used) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int tid = threadIdx.x;
   int count = 0, u;
   for (int p = tid; p < c.n_pages; p += PLAN_THREADS) count += c.refs[p] != 0;
@@ -349,8 +349,8 @@ constexpr int PIECE = 16 * MOVE_THREADS * 4;  // bytes that a block copies at on
 // Copies the listed pages in every layer; REMAP: also renames them in the tables.
 template <bool REMAP>
 __global__ void __launch_bounds__(MOVE_THREADS) k_kv_move(const lx_kv_cache c) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int moves = c.scratch[MOVES];
   if (moves == 0) return;
   const size_t bytes = static_cast<size_t>(c.kv_heads) * (c.page / BLOCK) * block_bytes(c.head_dim, c.group);

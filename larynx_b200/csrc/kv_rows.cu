@@ -8,10 +8,10 @@
 // 64 h + 32 w + 4 n + {0..3}.  All of a lane's loads are in flight before the first is used.
 //
 // Quantising, per token and group (include/larynx_kv.h): the codes are those
-// of exact arithmetic.  x - m is taken with its rounding error (two-sum), the
-// quotient from the reciprocal of s, and where one of eight remainders d - c s comes
-// within a hair of s / 2 the decisions are made again on the exact remainders.
+// of exact arithmetic, without branches (16-bit values meet ties in every other warp; a
+// second look at those cost four times the instructions).
 #include <cfloat>
+#include <cmath>
 
 #include "kv.cuh"
 
@@ -61,11 +61,12 @@ __device__ __forceinline__ float bf16_value(uint32_t u) { return __uint_as_float
 struct Params {
   float s, m, inv;
   uint32_t packed;  // bf16 s in the low half, bf16 m in the high half
+  bool small;       // a step so small that products with it lose bits (and not all values equal)
 };
 
 // Step and minimum of a group with smallest and largest value lo, hi (NaN where
 // the group holds one).  s is the least bf16 value with 15 s >= hi - m: the
-// rounded quotient is at most one bf16 step off, and 15 s is exact in fp32.
+// product with 1 / 15 is at most one bf16 step off, and 15 s is exact in fp32.
 __device__ __forceinline__ Params params_of(float lo, float hi) {
   Params p;
   const uint32_t mb = bf16_floor(lo);
@@ -75,10 +76,11 @@ __device__ __forceinline__ Params params_of(float lo, float hi) {
     p.s = p.m = __uint_as_float(0x7fc00000u);
     p.inv = 0.0f;
     p.packed = 0x7fc07fc0u;
+    p.small = false;
     return p;
   }
   constexpr uint32_t least = 0x00800000u;  // 2^-126
-  uint32_t sb = (__float_as_uint(__fdiv_rn(range, 15.0f)) + 0xFFFFu) & 0xFFFF0000u;
+  uint32_t sb = (__float_as_uint(range * (1.0f / 15.0f)) + 0xFFFFu) & 0xFFFF0000u;
   sb = sb < least ? least : sb;
   float top = 15.0f * __uint_as_float(sb);
   if (top < range || (top == range && rest > 0.0f)) {
@@ -89,37 +91,68 @@ __device__ __forceinline__ Params params_of(float lo, float hi) {
   }
   p.s = __uint_as_float(sb);
   p.m = m;
-  p.inv = __frcp_rn(p.s);
+  asm("rcp.approx.f32 %0, %1;" : "=f"(p.inv) : "f"(p.s));  // to an ulp, which is enough (codes_of)
   p.packed = (sb >> 16) | (mb << 16);
+  p.small = p.s < 7.8886091e-31f && range > 0.0f;  // 2^-100
   return p;
 }
 
-// rint((x - m) / s) + MAGIC in exact arithmetic, ties to even, given d = fl(x - m) and t, the same from the rounded quotient.
-__device__ __noinline__ float exact_code(float x, float d, float t, float m, float s) {
-  float c = t - MAGIC;
+// Packed sums rounded down and up.
+__device__ __forceinline__ float2 add2_rm(float2 a, float2 b) {
+  float2 c;
+  asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rm.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 add2_rp(float2 a, float2 b) {
+  float2 c;
+  asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rp.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+
+// rint((x - m) / s) + MAGIC in exact arithmetic, ties to even, for steps near the end of the range, where the remainder
+// below would underflow: the decision on the remainder d - c s, which is exact, and on what d = x - m lost.
+__device__ __noinline__ float small_code(float x, float m, float s) {
+  const float d = x - m;
+  float c = fminf(rintf(__fdiv_rn(d, s)), 15.0f);
   const float e = fmaf(-c, s, d), rest = diff_error(x, m, d), h = 0.5f * s;
-  const bool odd = __float_as_uint(t) & 1u;
+  const bool odd = static_cast<int>(c) & 1;
   if (e > h || (e == h && (rest > 0.0f || (rest == 0.0f && odd)))) c += 1.0f;
   if (e < -h || (e == -h && (rest < 0.0f || (rest == 0.0f && odd)))) c -= 1.0f;
   return fminf(fmaxf(c, 0.0f), 15.0f) + MAGIC;
 }
 
-// The codes of eight values, code i at bit K ? 4 (i / 2) + 16 (i % 2) : 4 i.  With c = rint(fl(x - m) / s), the
-// remainder e = fl(x - m) - c s is exact (a multiple of the smaller ulp, at most about s / 2); only where |e| reaches
-// s / 2 can the rounding of the quotient, or of x - m, have decided wrongly.  MAGIC + c has c in its low bits, so a sum
-// of products with powers of 16 packs the codes; what MAGIC adds is taken off at the end.
+// The codes of eight values, code i at bit K ? 4 (i / 2) + 16 (i % 2) : 4 i: rint((x - m) / s) in exact arithmetic, ties
+// to even.
+//  * d = x - m is rounded to odd (the last bit set where something was cut off).  A tie (c + 1/2) s has at most 13
+//    bits, so d is a tie only where x - m is, and is on its side of every tie otherwise.
+//  * The quotient y is corrected once by its remainder, which is exact; it is then the rounded d / s (off by less
+//    than 2^-24 of an ulp before rounding).  A quotient that is no tie is at least 0.502 ulp away from one (an ulp of
+//    d, over s with 8 bits), so it is not rounded onto one, and a tie is met exactly.
+//  * MAGIC + c has c in its low bits: a sum of products with powers of 16 packs the codes.
 template <bool K>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], const Params& p) {
-  float d[8], t[8], far = 0.0f;
+  float t[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    d[i] = x[i] - p.m;
-    t[i] = fmaf(d[i], p.inv, MAGIC);
-    far = fmaxf(far, fabsf(fmaf(MAGIC - t[i], p.s, d[i])));
+  for (int i = 0; i < 8; i += 2) {
+    const float2 v = make_float2(x[i], x[i + 1]), low = make_float2(-p.m, -p.m);
+    const float2 down = add2_rm(v, low), up = add2_rp(v, low);
+    float2 d;
+    d.x = __uint_as_float(__float_as_uint(down.x) | (__float_as_uint(up.x) - __float_as_uint(down.x)));
+    d.y = __uint_as_float(__float_as_uint(down.y) | (__float_as_uint(up.y) - __float_as_uint(down.y)));
+    const float2 inv = make_float2(p.inv, p.inv);
+    const float2 y = __fmul2_rn(d, inv);
+    const float2 e = __ffma2_rn(make_float2(-y.x, -y.y), make_float2(p.s, p.s), d);
+    const float2 r = __fadd2_rn(__ffma2_rn(e, inv, y), make_float2(MAGIC, MAGIC));
+    t[i] = r.x;
+    t[i + 1] = r.y;
   }
-  if (2.0f * far >= 0.99999f * p.s) {
+  if (p.small) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = exact_code(x[i], d[i], t[i], p.m, p.s);
+    for (int i = 0; i < 8; ++i) t[i] = small_code(x[i], p.m, p.s);
   }
   uint32_t bits = 0, magic = 0;
 #pragma unroll
@@ -158,6 +191,23 @@ __device__ __forceinline__ __half from_f32(float x) {
 template <>
 __device__ __forceinline__ float from_f32(float x) {
   return x;
+}
+
+// Two values side by side, rounded together.
+template <typename T>
+__device__ __forceinline__ void put2(T* e, float a, float b);
+template <>
+__device__ __forceinline__ void put2(bf16* e, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(e) = __floats2bfloat162_rn(a, b);
+}
+template <>
+__device__ __forceinline__ void put2(__half* e, float a, float b) {
+  *reinterpret_cast<__half2*>(e) = __floats2half2_rn(a, b);
+}
+template <>
+__device__ __forceinline__ void put2(float* e, float a, float b) {
+  e[0] = a;
+  e[1] = b;
 }
 
 // N neighbouring elements, N sizeof(T) a multiple of 8 bytes; `wide`: the address is as aligned as the widest access.
@@ -216,8 +266,7 @@ struct Span {
 };
 
 // The b-th block that entry i touches; false when there is none.
-__device__ __forceinline__ bool span_of(const lx_kv_cache& c, const lx_kv_rows& r, int layer, int i, int b, int head,
-                                        bool writes, Span& s) {
+__device__ __forceinline__ bool span_of(const lx_kv_cache& c, const lx_kv_rows& r, int i, int b, Span& s) {
   // the entry's words in flight together
   const int slot = r.seqs ? r.seqs[i] : i;
   const bool ok = slot >= 0 && slot < c.n_seq;
@@ -231,34 +280,38 @@ __device__ __forceinline__ bool span_of(const lx_kv_cache& c, const lx_kv_rows& 
   if (s.start == LX_KV_REFUSED) return false;  // an entry that was not served
   s.pos0 = (s.start & ~(BLOCK - 1)) + b * BLOCK;
   if (s.pos0 >= s.start + s.e.rows) return false;
-  s.page = -1;
-  if (s.pos0 >= 0 && s.pos0 < s.len) {
-    s.page = c.table[static_cast<size_t>(slot) * c.max_pages + s.pos0 / c.page];
-    if (s.page < 0 || s.page >= c.n_pages) {
-      flag(c, LX_KV_PAGE);
-      s.page = -1;
-    } else {
-      s.at = block_at(c, layer, s.page, head, s.pos0 % c.page / BLOCK);
-      if (writes && c.refs[s.page] > 1) {  // held by a fork as well: lx_kv_extend gives a copy first
-        flag(c, LX_KV_ROWS);
-        s.page = -1;
-      }
-    }
-  }
+  s.page = s.pos0 >= 0 && s.pos0 < s.len
+               ? c.table[static_cast<size_t>(slot) * c.max_pages + (s.pos0 >> page_shift(c.page))]
+               : -2;
   return true;
 }
 
-// The block, head and side (K or V) of this warp.
+// Whether the block's page, whose id is under way, can be used; its first byte.
+__device__ __forceinline__ void find_block(const lx_kv_cache& c, int layer, int head, bool writes, Span& s) {
+  if (s.page >= 0 && s.page < c.n_pages) {
+    s.at = block_at(c, layer, s.page, head, (s.pos0 & (c.page - 1)) / BLOCK);
+    if (writes && c.refs[s.page] > 1) {  // held by a fork as well: lx_kv_extend gives a copy first
+      flag(c, LX_KV_ROWS);
+      s.page = -1;
+    }
+  } else {
+    if (s.page != -2) flag(c, LX_KV_PAGE);
+    s.page = -1;
+  }
+}
+
+// The block, side (K or V) and heads of this warp.
 struct Work {
-  int entry, b, head, kv;
+  int entry, b, head, heads, kv;
   bool any;
 };
-__device__ __forceinline__ Work work_of(const lx_kv_rows& r, int blocks) {
+__device__ __forceinline__ Work work_of(const lx_kv_cache& c, const lx_kv_rows& r, int blocks, int heads) {
   Work w;
   const unsigned item = blockIdx.x * (WARPS / 2) + threadIdx.x / 64;
   w.entry = item / blocks;
   w.b = item - w.entry * blocks;
-  w.head = blockIdx.y;
+  w.head = blockIdx.y * heads;
+  w.heads = min(heads, c.kv_heads - w.head);
   w.kv = threadIdx.x / 32 % 2;
   w.any = w.entry < r.n;
   return w;
@@ -266,37 +319,57 @@ __device__ __forceinline__ Work work_of(const lx_kv_rows& r, int blocks) {
 
 template <typename T, int DIM, int GROUP>
 __global__ void __launch_bounds__(32 * WARPS)
-    k_kv_write(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, const T* __restrict__ k, int64_t k_row,
+    k_kv_write(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, int heads, const T* __restrict__ k, int64_t k_row,
                int64_t k_head, const T* __restrict__ v, int64_t v_row, int64_t v_head, bool wide) {
   constexpr int H = DIM / 64, G = DIM / GROUP;
   __shared__ __align__(16) uint16_t sv[WARPS / 2][H * 256];
   const int pair = threadIdx.x / 64, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
-  pdl_launch_dependents();
   pdl_wait();
-  const Work w = work_of(r, blocks);
+  pdl_launch_dependents();
+  const Work w = work_of(c, r, blocks, heads);
   Span s;
-  if (!w.any || !span_of(c, r, layer, w.entry, w.b, w.head, true, s)) return;
+  if (!w.any || !span_of(c, r, w.entry, w.b, s)) return;
   // tokens of the block that this entry writes (and that lie in the sequence)
   const int first = max(s.start - s.pos0, 0), past = min(min(s.start + s.e.rows, s.len) - s.pos0, BLOCK);
   if ((s.start < 0 || s.start + s.e.rows > s.len) && lane == 0) flag(c, LX_KV_ROWS);
-  if (s.page < 0 || past <= first) return;
-  uint8_t* block = static_cast<uint8_t*>(c.pool) + s.at;
+  if (past <= first) return;
   const bool full = first == 0 && past == BLOCK;
-  const T* src = w.kv ? v + w.head * v_head : k + w.head * k_head;
-  const int64_t row = w.kv ? v_row : k_row;
-  Pack<T, 8> raw[2][2 * H];  // tokens n, n + 8
+  const int64_t row = w.kv ? v_row : k_row, head_stride = w.kv ? v_head : k_head;
+  const T* src = (w.kv ? v : k) + w.head * head_stride + (s.e.row0 + (s.pos0 + n - s.start)) * row + 8 * j;
+  const int head_bytes = c.page / BLOCK * block_bytes(DIM, GROUP);
+  Pack<T, 8> raw[2][2 * H], next[2][2 * H];  // tokens n, n + 8
+  auto bring = [&](const T* from, Pack<T, 8> (&to)[2][2 * H]) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int t = n + 8 * u;
-    const T* p = src + (s.e.row0 + (s.pos0 + t - s.start)) * row + 8 * j;
+    for (int u = 0; u < 2; ++u) {
+      const int t = n + 8 * u;
 #pragma unroll
-    for (int hw = 0; hw < 2 * H; ++hw) {
-      if (t >= first && t < past)
-        raw[u][hw].load(p + 32 * hw, wide);
-      else
-        raw[u][hw].clear();
+      for (int hw = 0; hw < 2 * H; ++hw) {
+        if (t >= first && t < past)
+          to[u][hw].load(from + 8 * u * row + 32 * hw, wide);
+        else
+          to[u][hw].clear();
+      }
     }
-  }
+  };
+  // the next head's values are under way while one is worked on, where the registers allow it
+  constexpr bool AHEAD = sizeof(T) * DIM <= 256;
+  bring(src, raw);
+  find_block(c, layer, w.head, true, s);
+  if (s.page < 0) return;
+  uint8_t* block = static_cast<uint8_t*>(c.pool) + s.at;
+#pragma unroll 1
+  for (int head = 0; head < w.heads; ++head, src += head_stride, block += head_bytes) {
+    if (AHEAD) {
+      if (head > 0) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int hw = 0; hw < 2 * H; ++hw) raw[u][hw] = next[u][hw];
+      }
+      if (head + 1 < w.heads) bring(src + head_stride, next);
+    } else if (head > 0) {
+      bring(src, raw);
+    }
   uint32_t word[2][2 * H];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -343,7 +416,7 @@ __global__ void __launch_bounds__(32 * WARPS)
             *reinterpret_cast<uint2*>(dst + 8 * u) = make_uint2(word[u][2 * h], word[u][2 * h + 1]);
       }
     }
-    return;
+    continue;
   }
   // V: lane (n', j') of the fragment takes tokens 2 j' + {0, 1, 8, 9}, channels 32 w + 4 n' + {0..3}
 #pragma unroll
@@ -369,89 +442,100 @@ __global__ void __launch_bounds__(32 * WARPS)
       }
     }
   }
+  __syncwarp();  // before the next head's codes
+  }
 }
 
 template <typename T, int DIM, int GROUP>
 __global__ void __launch_bounds__(32 * WARPS)
-    k_kv_read(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, T* __restrict__ k, int64_t k_row,
+    k_kv_read(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, int heads, T* __restrict__ k, int64_t k_row,
               int64_t k_head, T* __restrict__ v, int64_t v_row, int64_t v_head, bool wide) {
   constexpr int H = DIM / 64, G = DIM / GROUP;
   const int lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
-  pdl_launch_dependents();
   pdl_wait();
-  const Work w = work_of(r, blocks);
+  pdl_launch_dependents();
+  const Work w = work_of(c, r, blocks, heads);
   if (!w.any) return;
   Span s;
-  if (!span_of(c, r, layer, w.entry, w.b, w.head, false, s)) {
+  if (!span_of(c, r, w.entry, w.b, s)) {
     // a slot or an entry that does not exist: its rows read as 0
     if (s.e.rows == 0 || w.b * BLOCK >= s.e.rows || (s.e.slot >= 0 && s.start != LX_KV_REFUSED)) return;
     s.start = 0;
     s.pos0 = w.b * BLOCK;
     s.len = 0;
-    s.page = -1;
+    s.page = -2;
   }
+  find_block(c, layer, w.head, false, s);
   const int first = max(s.start - s.pos0, 0), past = min(s.start + s.e.rows - s.pos0, BLOCK);
   const int held = s.page < 0 ? 0 : min(s.len - s.pos0, BLOCK);
   const uint8_t* block = static_cast<const uint8_t*>(c.pool) + (s.page < 0 ? 0 : s.at);
+  const int head_bytes = c.page / BLOCK * block_bytes(DIM, GROUP);
+  const int64_t row = w.kv ? v_row : k_row, head_stride = w.kv ? v_head : k_head;
+  T* dst = (w.kv ? v : k) + w.head * head_stride;
+#pragma unroll 1
+  for (int head = 0; head < w.heads; ++head, dst += head_stride, block += head_bytes) {
   uint4 code[H];
 #pragma unroll
   for (int h = 0; h < H; ++h)
     code[h] = held > 0 ? __ldcg(reinterpret_cast<const uint4*>(block + 512 * (w.kv * H + h) + 16 * lane))
                        : make_uint4(0, 0, 0, 0);
-  T* dst = w.kv ? v + w.head * v_head : k + w.head * k_head;
-  const int64_t row = w.kv ? v_row : k_row;
+  // the parameters of this lane's tokens: n and n + 8 (K), 2 j + {0, 1, 8, 9} (V)
   const uint8_t* par = block + param_offset(DIM) + 64 * G * w.kv;
+  uint32_t p[G][4];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+    if (held > 0) {
+      if (w.kv) {
+        *reinterpret_cast<uint4*>(p[g]) = __ldcg(reinterpret_cast<const uint4*>(par + 64 * g + 16 * j));
+      } else {
+        p[g][0] = __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(n)));
+        p[g][1] = __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(n + 8)));
+      }
+    }
   if (!w.kv) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int t = n + 8 * u;
       if (t < first || t >= past) continue;
       T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 8 * j;
-      uint32_t p[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-        p[g] = t < held ? __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(t))) : 0u;
 #pragma unroll
       for (int hw = 0; hw < 2 * H; ++hw) {
         const uint4 x = code[hw / 2];
         const uint32_t word = u ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
-        const float step = bf16_value(p[32 * hw / GROUP] & 0xFFFFu), low = __uint_as_float(p[32 * hw / GROUP] & 0xFFFF0000u);
+        const uint32_t q = p[32 * hw / GROUP][u];
+        const float step = bf16_value(q & 0xFFFFu), low = __uint_as_float(q & 0xFFFF0000u);
         float even[4], odd[4];
         codes_f32(word, even);
         codes_f32(word >> 16, odd);
         Pack<T, 8> y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y.e[2 * i] = from_f32<T>(fmaf(even[i], step, low));
-          y.e[2 * i + 1] = from_f32<T>(fmaf(odd[i], step, low));
-        }
+        for (int i = 0; i < 4; ++i) put2(y.e + 2 * i, fmaf(even[i], step, low), fmaf(odd[i], step, low));
         if (t >= held) y.clear();
         y.store(out + 32 * hw, wide);
       }
     }
-    return;
+    continue;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 2 * j + 8 * (i / 2) + i % 2;
     if (t < first || t >= past) continue;
     T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 4 * n;
-    uint32_t p[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-      p[g] = t < held ? __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(t))) : 0u;
 #pragma unroll
     for (int hw = 0; hw < 2 * H; ++hw) {
       const uint4 x = code[hw / 2];
       const uint32_t word = i / 2 ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
-      const float step = bf16_value(p[32 * hw / GROUP] & 0xFFFFu), low = __uint_as_float(p[32 * hw / GROUP] & 0xFFFF0000u);
+      const uint32_t x4 = p[32 * hw / GROUP][i];
+      const float step = bf16_value(x4 & 0xFFFFu), low = __uint_as_float(x4 & 0xFFFF0000u);
       float e[4];
       codes_f32(i % 2 ? word >> 16 : word, e);
       Pack<T, 4> y;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) y.e[q] = from_f32<T>(t < held ? fmaf(e[q], step, low) : 0.0f);
+      for (int q = 0; q < 2; ++q) put2(y.e + 2 * q, fmaf(e[2 * q], step, low), fmaf(e[2 * q + 1], step, low));
+      if (t >= held) y.clear();
       y.store(out + 32 * hw, wide);
     }
+  }
   }
 }
 
@@ -467,12 +551,23 @@ bool go(bool writes, const lx_kv_cache& c, int layer, const lx_kv_rows& r, void*
         void* v, int64_t v_row, int64_t v_head, cudaStream_t s) {
   const int blocks = (r.max_rows + BLOCK - 2) / BLOCK + 1;  // rows may begin inside a block
   const long long items = static_cast<long long>(r.n) * blocks;
-  const dim3 grid(static_cast<unsigned>((items + WARPS / 2 - 1) / (WARPS / 2)), c.kv_heads);
+  // Heads a warp: finding the block costs as long as two heads of it, and about twenty warps run on an SM at once.
+  int heads = 1;
+  double best = 0.0;
+  for (int h = 1; h <= 8 && h <= c.kv_heads; ++h) {
+    const double warps = 2.0 * static_cast<double>(items) * ((c.kv_heads + h - 1) / h);
+    const double cost = std::ceil(warps / (20.0 * num_sms())) * (2 + h);
+    if (h == 1 || cost < best) {
+      best = cost;
+      heads = h;
+    }
+  }
+  const dim3 grid(static_cast<unsigned>((items + WARPS / 2 - 1) / (WARPS / 2)), (c.kv_heads + heads - 1) / heads);
   const bool wide = wide_rows<T>(k, k_row, k_head, v, v_row, v_head);
   if (writes)
-    return launch(k_kv_write<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks,
+    return launch(k_kv_write<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks, heads,
                   static_cast<const T*>(k), k_row, k_head, static_cast<const T*>(v), v_row, v_head, wide);
-  return launch(k_kv_read<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks, static_cast<T*>(k), k_row,
+  return launch(k_kv_read<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks, heads, static_cast<T*>(k), k_row,
                 k_head, static_cast<T*>(v), v_row, v_head, wide);
 }
 
