@@ -49,6 +49,7 @@ extern "C" {
 #define LX_KV_WIDTH 4 /* the sequence would need more than max_pages pages     */
 #define LX_KV_PAGE 8  /* a table holds a page id outside [0, n_pages)          */
 #define LX_KV_ROWS 16 /* row offsets out of range, or rows outside a sequence  */
+#define LX_KV_STUCK 32 /* a device-side wait exceeded its bound: no result     */
 
 /* The start that lx_kv_extend gives an entry it did not serve. */
 #define LX_KV_REFUSED INT32_MIN

@@ -129,7 +129,7 @@ struct Args {
   int layer, q_heads, per, tiles, split, block_lg;  // block_lg: log2 of the blocks of a page
   const void* q;
   int64_t q_row, q_head;
-  bool wide;
+  bool wide, out_wide;  // 16-byte accesses
   void* out;
   int64_t o_row, o_head;
   float* lse;
@@ -172,10 +172,11 @@ struct Share {
   // the rows of the CTA are rows row0 .. row0 + n_rows - 1 of the entry's (query row, query head) pairs
   __device__ __forceinline__ bool take(const Args& a, int tile_rows) {
     rank = blockIdx.x % a.split;
-    int item = blockIdx.x / a.split;
-    head = item % a.c.kv_heads;
-    item /= a.c.kv_heads;
-    const int tile = item % a.tiles, entry = item / a.tiles;
+    const int item = blockIdx.x / a.split, x = item / a.c.kv_heads;
+    return take_at(a, x / a.tiles, item % a.c.kv_heads, x % a.tiles, tile_rows);
+  }
+  __device__ __forceinline__ bool take_at(const Args& a, int entry, int kv_head, int tile, int tile_rows) {
+    head = kv_head;
     // the entry's words in flight together
     const int slot = a.r.seqs ? a.r.seqs[entry] : entry;
     const bool ok = slot >= 0 && slot < a.c.n_seq;
@@ -1049,6 +1050,511 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 }
 
 // ---------------------------------------------------------------------------
+// tiles of 128 rows on tcgen05
+// ---------------------------------------------------------------------------
+// One CTA takes 128 rows and walks their keys 64 at a time.  Four warps unpack:
+// codes go from global memory through registers into operand tiles in shared memory (K
+// as they are, V less 8, so that no further product is needed), a code being an fp16 subnormal as above, steps and minima
+// into fp32 arrays.  One thread issues the matrix instructions: S = Q K^T (a
+// sum for every group of channels, in tensor memory), one unit ahead of the softmax, and O += P V.
+// Four warps do the softmax, a thread a row: nothing is exchanged between
+// lanes, and what a key's step and minimum cost is shared with nobody but
+// also needs no unpacking, against eight rows and unpacking in every warp in the forms above.
+//   V's tile holds the channels of 32 in the order 8 i + n for channel 4 n + i,
+// which is how the unpacking warps write it without bank conflicts; the rows
+// are put in order when they are written out.
+constexpr int TILE_ROWS = 128;
+constexpr int TILE_KEYS = 64;
+
+template <int DIM, int GROUP>
+struct TileShape {
+  static constexpr int THREADS = 256;  // 4 warps that unpack (a thread of the first issues), 4 of softmax
+  static constexpr int H = DIM / 64, G = DIM / GROUP;
+  static constexpr int CTAS = DIM == 64 ? 2 : 1;  // an SM
+  // tensor memory: S (G sums a buffer), P, O
+  static constexpr int S_BUFS = G == 1 || DIM == 128 ? 2 : 1;
+  static constexpr int P_BUFS = G == 1 ? 2 : 1;
+  static constexpr int P_COL = S_BUFS * G * TILE_KEYS;
+  static constexpr int O_COL = P_COL + P_BUFS * G * TILE_KEYS / 2;
+  static constexpr int COLS = DIM == 64 ? 256 : 512;
+  // two CTAs an SM: the softmax takes registers from the unpacking (128 a thread at launch)
+  static constexpr bool SPLIT = CTAS == 2;
+  static constexpr int LAUNCH_REGS = 128, UNPACK_REGS = 72, SOFTMAX_REGS = 184;
+  static_assert(UNPACK_REGS + SOFTMAX_REGS <= 2 * LAUNCH_REGS, "register split");
+  static_assert(O_COL + DIM <= COLS, "tensor memory");
+  // shared memory
+  static constexpr int Q_BYTES = H * TILE_ROWS * 128;
+  static constexpr int K_BYTES = H * TILE_KEYS * 128;
+  static constexpr int V_BYTES = DIM * 128;
+  static constexpr int PAR = 4 * G * TILE_KEYS * 4;  // ks, km, vs, vm
+  static constexpr int SLOT = K_BYTES + V_BYTES;
+  static constexpr int SMEM = 1024 + Q_BYTES + 2 * SLOT + 2 * PAR + 256;
+};
+
+__device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ uint32_t less(uint32_t x, uint32_t by) {
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&by));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+template <typename T, int DIM, int GROUP>
+__global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(const __grid_constant__ Args a) {
+  using S = TileShape<DIM, GROUP>;
+  constexpr int H = S::H, G = S::G, BB = block_bytes(DIM, GROUP);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;
+  uint8_t* slots = sq + S::Q_BYTES;
+  float* par = reinterpret_cast<float*>(slots + 2 * S::SLOT);  // [slot][ks, km, vs, vm][G][64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(par) + 2 * S::PAR);
+  // Each pair alternates by unit, and the next completion of a barrier always needs the waiter of the one before: no
+  // waiter is ever two phases behind.  empty[t & 1]: the product of unit t is done.
+  uint64_t *q_full = bars, *full = bars + 1, *empty = bars + 3, *s_full = bars + 5, *s_empty = bars + 7, *p_full = bars + 9;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* have = reinterpret_cast<int*>(tmem_slot + 2);    // [slot][4] blocks that exist
+  float* v_top = reinterpret_cast<float*>(have + 8);    // [slot][2][G] largest step of V
+  static_assert(11 * 8 + 8 + 32 + 2 * 2 * 2 * 4 <= 256, "barriers");
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full[i], 128);
+      mbar_init(&empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_full[i], 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, S::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // the last tiles of rows, which see the most keys, first
+  Share s;
+  bool any;
+  {
+    const int per_tile = a.r.n * a.c.kv_heads, tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per_tile;
+    const int x = blockIdx.x % per_tile;
+    any = s.take_at(a, x / a.c.kv_heads, x % a.c.kv_heads, tile, TILE_ROWS);
+  }
+  int lo_cta = 0, hi_cta = 0, x_;
+  if (any) {
+    s.range(a, 0, lo_cta, x_);
+    s.range(a, TILE_ROWS, x_, hi_cta);
+  }
+  const int tile0 = lo_cta / TILE_KEYS;
+  const int n_tiles = any && hi_cta > lo_cta ? (hi_cta + TILE_KEYS - 1) / TILE_KEYS - tile0 : 0;
+  auto wait = [&](uint64_t* bar, int use) {  // for the use-th completion of a barrier
+    return mbar_wait(bar, static_cast<uint32_t>(use & 1), nullptr, abort_flag, 0);
+  };
+
+  // issue, by one thread: the product O += P V of unit t
+  constexpr int PV_N = G == 1 ? DIM : GROUP;
+  auto issue_pv = [&](int t) {
+    if (!wait(&p_full[t & 1], t / 2)) return false;
+    tc_fence_after();
+    const uint64_t dv = sdesc_sw128(smem_u32(slots + (t & 1) * S::SLOT + S::K_BYTES));
+    const uint32_t p = tmem + S::P_COL + (t % S::P_BUFS) * (G * TILE_KEYS / 2);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        umma_ts(tmem + S::O_COL + g * PV_N, p + g * (TILE_KEYS / 2) + 8 * k,
+                dv + static_cast<uint64_t>((g * PV_N * 128) >> 4) + 2 * k, idesc_f16_f32(128, PV_N),
+                t > 0 || k > 0 ? 1u : 0u);
+    umma_commit(&empty[t & 1]);
+    return true;
+  };
+  // the scores of unit t, then the product of the unit before (the softmax of that one is under way meanwhile)
+  auto issue = [&](int t) {
+    if (t == 0 && !wait(q_full, 0)) return false;
+    if (!wait(&full[t & 1], t / 2)) return false;
+    if (t >= S::S_BUFS && !wait(&s_empty[t % S::S_BUFS], t / S::S_BUFS - 1)) return false;
+    tc_fence_after();
+    const uint64_t dq = sdesc_sw128(smem_u32(sq)), dk = sdesc_sw128(smem_u32(slots + (t & 1) * S::SLOT));
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int k = 0; k < GROUP / 16; ++k) {
+        const int c = g * GROUP / 16 + k, h = c / 4;  // 16 channels c of half h
+        umma_ss(tmem + ((t % S::S_BUFS) * G + g) * TILE_KEYS,
+                dq + static_cast<uint64_t>((h * TILE_ROWS * 128) >> 4) + 2 * (c % 4),
+                dk + static_cast<uint64_t>((h * TILE_KEYS * 128) >> 4) + 2 * (c % 4), idesc_f16_f32(128, TILE_KEYS),
+                k > 0 ? 1u : 0u);
+      }
+    umma_commit(&s_full[t % S::S_BUFS]);
+    return t == 0 || issue_pv(t - 1);
+  };
+
+  if (!any) {
+    // no such rows
+  } else if (warp < 4) {
+    if (S::SPLIT) regs_dec<S::UNPACK_REGS>();
+    // ---- unpack: warp w block w of each unit; thread x < 64 K's parameters of key x, the others V's of key x - 64
+    const int n = lane / 4, j = lane % 4, key = threadIdx.x % 64, side = threadIdx.x / 64;
+    const int32_t* table = a.c.table + static_cast<size_t>(s.e.slot < 0 ? 0 : s.e.slot) * a.c.max_pages;
+    const size_t head_bytes = static_cast<size_t>(BB) << a.block_lg;
+    const uint8_t* base = static_cast<const uint8_t*>(a.c.pool) +
+                          (static_cast<size_t>(a.layer) * a.c.n_pages * a.c.kv_heads + s.head) * head_bytes;
+    const int n_blocks = (hi_cta + BLOCK - 1) / BLOCK, mask = (1 << a.block_lg) - 1;
+    // first byte of block b of page p, or null
+    auto at = [&](int p, int b) -> const uint8_t* {
+      if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.c.n_pages)) return nullptr;
+      return base + static_cast<size_t>(p) * a.c.kv_heads * head_bytes + (b & mask) * BB;
+    };
+    auto look = [&](int b) { return b < n_blocks ? table[b >> a.block_lg] : -2; };
+    uint4 code[2][H];
+    uint32_t word[G];
+    bool here = false, key_here = false;
+    auto bring = [&](int t, int page, int key_page) {  // unit t
+      const int b = 4 * (tile0 + t) + warp, kb = 4 * (tile0 + t) + key / 16;
+      const uint8_t *p = at(page, b), *kp = at(key_page, kb);
+      here = p != nullptr;
+      key_here = kp != nullptr && (tile0 + t) * TILE_KEYS + key < s.len;
+      if (!here && page != -2 && lane == 0) flag(a.c, LX_KV_PAGE);
+#pragma unroll
+      for (int x = 0; x < 2 * H; ++x)
+        code[x / H][x % H] =
+            here ? *reinterpret_cast<const uint4*>(p + 512 * x + 16 * lane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        word[g] = key_here ? *reinterpret_cast<const uint32_t*>(kp + param_offset(DIM) + 64 * (side * G + g) +
+                                                                4 * param_slot(key % 16))
+                           : 0u;
+    };
+    int page = look(4 * tile0 + warp), key_page = look(4 * tile0 + key / 16);
+    if (n_tiles > 0) bring(0, page, key_page);
+    page = look(4 * (tile0 + 1) + warp);
+    key_page = look(4 * (tile0 + 1) + key / 16);
+    for (int t = 0; t < n_tiles; ++t) {
+      const int slot = t & 1;
+      if (t >= 2 && !__all_sync(0xffffffffu, wait(&empty[slot], t / 2 - 1))) break;
+      uint8_t* sk = slots + slot * S::SLOT;
+      uint8_t* sv = sk + S::K_BYTES;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // K: word x is w = x % 2 of key n + 8 (x / 2)
+          const uint32_t k = x == 0 ? code[0][h].x : x == 1 ? code[0][h].y : x == 2 ? code[0][h].z : code[0][h].w;
+          const int row = 16 * warp + n + 8 * (x / 2);
+          *reinterpret_cast<uint4*>(sk + h * (TILE_KEYS * 128) + row * 128 + (((4 * (x % 2) + j) ^ (row & 7)) << 4)) =
+              make_uint4(k & M0, k & M1, k >> 8 & M0, k >> 8 & M1);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // V: word x is w = x % 2 of keys 2 j, 2 j + 1 (+ 8 (x / 2))
+          const uint32_t v = x == 0 ? code[1][h].x : x == 1 ? code[1][h].y : x == 2 ? code[1][h].z : code[1][h].w;
+          uint8_t* row = sv + (64 * h + 32 * (x % 2) + n) * 128 + (((2 * warp + x / 2) ^ n) << 4) + 4 * j;
+          *reinterpret_cast<uint32_t*>(row) = less(v & M0, EIGHTS);
+          *reinterpret_cast<uint32_t*>(row + 8 * 128) = less(v & M1, EIGHTS << 4);
+          *reinterpret_cast<uint32_t*>(row + 16 * 128) = less(v >> 8 & M0, EIGHTS);
+          *reinterpret_cast<uint32_t*>(row + 24 * 128) = less(v >> 8 & M1, EIGHTS << 4);
+        }
+      }
+      float* p = par + slot * (S::PAR / 4) + side * 2 * G * TILE_KEYS + key;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float step = step_of(word[g]), low = low_of(word[g]);
+        p[g * TILE_KEYS] = step;
+        p[(G + g) * TILE_KEYS] = side ? fmaf(step, 8.0f, low) : low;
+        if (side) {
+          const float v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(step, 0.0f))));
+          if (lane == 0) v_top[(slot * 2 + warp - 2) * G + g] = v;
+        }
+      }
+      if (lane == 0) have[slot * 4 + warp] = here;
+      if (t + 1 < n_tiles) {
+        bring(t + 1, page, key_page);
+        page = look(4 * (tile0 + t + 2) + warp);
+        key_page = look(4 * (tile0 + t + 2) + key / 16);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&full[slot]);
+      if (warp == 0) {
+        bool ok = lane != 0 || issue(t);
+        if (lane == 0 && ok && t + 1 == n_tiles) ok = issue_pv(t);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+    }
+  } else {
+    // ---- softmax: a thread a row
+    if (S::SPLIT) regs_inc<S::SOFTMAX_REGS>();
+    const int quarter = warp - 4, row = 32 * quarter + lane;
+    const bool live = 32 * quarter < s.n_rows;  // a warp without rows only keeps the barriers going
+    int lo = 0, hi = 0, lo_all = 0, hi_all = 0;
+    float qs[G], c1 = 0.0f;
+    if (live) {
+      s.range(a, row, lo, hi);
+      s.range(a, 32 * quarter, x_, hi_all);
+      s.range(a, 32 * quarter + 31, lo_all, x_);
+      const T* q = s.query<T>(a, row);
+      Raw8<T> raw[DIM / 8];
+      float top = 0.0f;
+#pragma unroll
+      for (int x = 0; x < DIM / 8; ++x) raw[x].load(q + 8 * x, a.wide);
+#pragma unroll
+      for (int x = 0; x < DIM / 8; ++x) {
+        float y[8];
+        raw[x].get(y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fabsf(y[i]) <= 3.4e38f ? fmaxf(top, fabsf(y[i])) : top;
+      }
+      // the row times 2^up (and the sign of scale): its largest value lies in [2^13, 2^14)
+      const int up = top > 0.0f ? min(max(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -110), 110) : 0;
+      const float f = a.scale < 0.0f ? -pow2(up) : pow2(up), f16 = f * 0.0625f;
+      c1 = fabsf(a.scale) * 1.4426950408889634f * pow2(24) * pow2(-up);
+#pragma unroll
+      for (int g = 0; g < G; ++g) qs[g] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < DIM / 8; ++x) {
+        float y[8];
+        raw[x].get(y);
+        qs[8 * x / GROUP] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+        *reinterpret_cast<uint4*>(sq + (x / 8) * (TILE_ROWS * 128) + row * 128 + (((x % 8) ^ (row & 7)) << 4)) =
+            make_uint4(half_pair(make_float2(y[0] * f, y[1] * f)), half_pair(make_float2(y[2] * f16, y[3] * f16)),
+                       half_pair(make_float2(y[4] * f, y[5] * f)), half_pair(make_float2(y[6] * f16, y[7] * f16)));
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) qs[g] *= f * 5.9604645e-8f;  // in the units of the products: 2^-24
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    float limit = -INFINITY, off = 0.0f;  // the score above which the maximum is raised; log2 F less the maximum
+    float2 l = both(0.0f), z[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) z[g] = both(0.0f);
+    float step_top = 0.0f;
+    int f_exp = 0;
+    bool ok = true;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int slot = t & 1, key0 = (tile0 + t) * TILE_KEYS;
+      ok = wait(&full[slot], t / 2) && wait(&s_full[t % S::S_BUFS], t / S::S_BUFS);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      float2 x[TILE_KEYS / 2];
+      const float4* ks = reinterpret_cast<const float4*>(par + slot * (S::PAR / 4));
+      if (live) {
+        // scores over c1
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            float raw[32];
+            tmem_ld32(t_lane + ((t % S::S_BUFS) * G + g) * TILE_KEYS + 32 * c, raw);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 st = ks[g * 16 + 8 * c + i], mi = ks[(G + g) * 16 + 8 * c + i];
+              float2 &u = x[16 * c + 2 * i], &v = x[16 * c + 2 * i + 1];
+              u = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.x, mi.y))
+                         : __ffma2_rn(both(qs[g]), make_float2(mi.x, mi.y), u);
+              v = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.z, mi.w))
+                         : __ffma2_rn(both(qs[g]), make_float2(mi.z, mi.w), v);
+              u = __ffma2_rn(make_float2(raw[4 * i], raw[4 * i + 1]), make_float2(st.x, st.y), u);
+              v = __ffma2_rn(make_float2(raw[4 * i + 2], raw[4 * i + 3]), make_float2(st.z, st.w), v);
+            }
+          }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[t % S::S_BUFS]);
+      // P may be written once the product that read its buffer is done
+      auto p_free = [&](bool last) {
+        const int before = last ? t - 1 : t - S::P_BUFS;
+        if (before < 0) return true;
+        const bool w = __all_sync(0xffffffffu, wait(&empty[before & 1], before / 2));
+        tc_fence_after();
+        return w;
+      };
+      if (!live) {
+        if (!(ok = p_free(true))) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t & 1]);
+        continue;
+      }
+      const int4 got = *reinterpret_cast<const int4*>(have + 4 * slot);
+      const bool part = key0 < lo_all || key0 + TILE_KEYS > hi_all || !(got.x & got.y & got.z & got.w);
+      uint64_t seen = ~0ull;
+      if (part) {
+        const int first = min(max(lo - key0, 0), 64), past = min(max(hi - key0, 0), 64);
+        seen = past > first ? (past == 64 ? ~0ull : (1ull << past) - 1) & (~0ull << first) : 0ull;
+        seen &= (got.x ? 0xFFFFull : 0) | (got.y ? 0xFFFFull << 16 : 0) | (got.z ? 0xFFFFull << 32 : 0) |
+                (got.w ? 0xFFFFull << 48 : 0);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (!(seen >> (2 * i) & 1)) x[i].x = -INFINITY;
+          if (!(seen >> (2 * i + 1) & 1)) x[i].y = -INFINITY;
+        }
+      }
+      float top = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        top = fmaxf(fmaxf(top, x[i].x), x[i].y);
+        top1 = fmaxf(fmaxf(top1, x[i + 1].x), x[i + 1].y);
+      }
+      top = fmaxf(top, top1) * c1;
+      float v = 0.0f;
+#pragma unroll
+      for (int g = 0; g < 2 * G; ++g) v = fmaxf(v, v_top[slot * 2 * G + g]);
+      bool waited = false;
+      if (__any_sync(0xffffffffu, top > limit || v > step_top)) {
+        int up = 0;
+        if (v > step_top) {
+          const int e = step_exponent(v), to = P_TOP - e;
+          up = step_top == 0.0f ? 0 : to - f_exp;
+          f_exp = to;
+          step_top = v > STEP_MAX ? INFINITY : pow2(e);
+        }
+        const float m = limit - RAISE, to = top > limit ? top : m;
+        const float f = to == -INFINITY ? 1.0f : ex2(m - to + up);
+        limit = to + RAISE;
+        off = f_exp - (to == -INFINITY ? 0.0f : to);
+        l = __fmul2_rn(l, both(f));
+#pragma unroll
+        for (int g = 0; g < G; ++g) z[g] = __fmul2_rn(z[g], both(f));
+        if (t > 0) {
+          if (!(ok = p_free(true))) break;  // the last product into O is done
+          waited = true;
+#pragma unroll 1
+          for (int c = 0; c < DIM / 32; ++c) {
+            float y[32];
+            tmem_ld32(t_lane + S::O_COL + 32 * c, y);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(y[8 * i + k] * f);
+              tmem_st8u(t_lane + S::O_COL + 32 * c + 8 * i, w);
+            }
+          }
+          tmem_st_wait();
+        }
+      }
+      if (!waited && !(ok = p_free(false))) break;
+      // p F, its sums, and P = p F s
+      auto probabilities = [&](auto tag) {
+        constexpr bool PART = decltype(tag)::value;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // 16 keys
+          uint32_t w[G][8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float2 p[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float2 y = __ffma2_rn(x[8 * c + 2 * i + k], both(c1), both(off));
+              p[k] = make_float2(ex2(y.x), ex2(y.y));
+              l = __fadd2_rn(l, p[k]);
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const float4 st = ks[(2 * G + g) * 16 + 4 * c + i], mi = ks[(3 * G + g) * 16 + 4 * c + i];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                float2 y = __fmul2_rn(p[k], k ? make_float2(st.z, st.w) : make_float2(st.x, st.y));
+                float2 low = k ? make_float2(mi.z, mi.w) : make_float2(mi.x, mi.y);
+                if (PART) {  // a key that the row does not see: not even its NaN counts
+                  const uint32_t in = static_cast<uint32_t>(seen >> (16 * c + 4 * i + 2 * k));
+                  if (!(in & 1)) y.x = low.x = 0.0f;
+                  if (!(in & 2)) y.y = low.y = 0.0f;
+                }
+                z[g] = __ffma2_rn(p[k], low, z[g]);
+                w[g][2 * i + k] = half_pair(y);
+              }
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            tmem_st8u(t_lane + S::P_COL + ((t % S::P_BUFS) * G + g) * (TILE_KEYS / 2) + 8 * c, w[g]);
+        }
+      };
+      if (part)
+        probabilities(std::true_type());
+      else
+        probabilities(std::false_type());
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t & 1]);
+    }
+    if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, wait(&empty[(n_tiles - 1) & 1], (n_tiles - 1) / 2));
+    if (ok && live) {
+      tc_fence_after();
+      const float sum = l.x + l.y;
+      const int r = s.row0 + row, q_row = r / a.per, h = s.head * a.per + (r - q_row * a.per);
+      T* out = static_cast<T*>(a.out) + (s.e.row0 + q_row) * a.o_row + h * a.o_head;
+#pragma unroll 1
+      for (int c = 0; c < DIM / 32; ++c) {
+        float y[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y[i] = 0.0f;
+        if (n_tiles > 0) {
+          tmem_ld32(t_lane + S::O_COL + 32 * c, y);
+          tmem_ld_wait();
+        }
+        const float2 zg = G == 1 ? z[0] : z[32 * c / GROUP % G];
+        const float low = zg.x + zg.y;
+        if (row < s.n_rows) {
+          __align__(16) T e[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {  // column 8 i + n is channel 4 n + i, times 16 for odd i
+            const float b = fmaf(y[i], (i / 8) % 2 ? 1048576.0f : 16777216.0f, low);
+            e[4 * (i % 8) + i / 8] = static_cast<T>(sum == 0.0f ? 0.0f : b / sum);
+          }
+          if (a.out_wide) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = reinterpret_cast<const uint4*>(e)[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) out[32 * c + i] = e[i];
+          }
+        }
+      }
+      if (a.lse && row < s.n_rows)
+        a.lse[static_cast<int64_t>(s.e.row0 + q_row) * a.q_heads + h] =
+            sum == 0.0f ? -INFINITY : (limit - RAISE - f_exp + log2f(sum)) * 0.6931471805599453f;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) flag(a.c, LX_KV_STUCK);
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 // What a kernel needs to be launched on one device: set up at its first call.
@@ -1131,6 +1637,28 @@ bool many(Args& a, int units, cudaStream_t s) {
 }
 
 template <typename T, int DIM, int GROUP>
+bool tile(Args& a, cudaStream_t s) {
+  using S = TileShape<DIM, GROUP>;
+  static bool ready[64] = {false};
+  auto kernel = k_kv_tile<T, DIM, GROUP>;
+  bool& done = ready[a.c.device & 63];
+  if (!done) {
+    // setmaxnreg.inc waits for registers that the block was launched with: no launch unless they cover the split
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || (S::SPLIT && fa.numRegs < S::LAUNCH_REGS) ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess)
+      return false;
+    done = true;
+  }
+  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per + TILE_ROWS - 1) / TILE_ROWS;
+  const long long ctas = tiles * a.r.n * a.c.kv_heads;
+  if (ctas > 0x7fffffff) return false;
+  a.tiles = static_cast<int>(tiles);
+  a.split = 1;
+  return launch(kernel, dim3(static_cast<unsigned>(ctas)), dim3(S::THREADS), S::SMEM, s, a);
+}
+
+template <typename T, int DIM, int GROUP>
 bool go(Args& a, int max_len, cudaStream_t s) {
   const long long rows = static_cast<long long>(a.r.max_rows) * a.per;
   const long long items = static_cast<long long>(a.r.n) * a.c.kv_heads;
@@ -1142,6 +1670,7 @@ bool go(Args& a, int max_len, cudaStream_t s) {
     if (rows <= 8) return wide ? few<T, DIM, GROUP, 1, WIDE>(a, units, s) : few<T, DIM, GROUP, 1, 4>(a, units, s);
     return wide ? few<T, DIM, GROUP, 2, 8>(a, units, s) : few<T, DIM, GROUP, 2, 4>(a, units, s);
   }
+  if (getenv("KV_TILE") && DIM / GROUP <= 2) return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, s);
   return rows <= 32 ? many<T, DIM, GROUP, 1, 2>(a, units, s) : many<T, DIM, GROUP, 1, 4>(a, units, s);
 }
 
@@ -1175,6 +1704,7 @@ extern "C" int lx_kv_attention(const lx_kv_cache* c, int32_t layer, const lx_kv_
   a.q_head = q_head;
   a.wide = aligned(q, 16) && q_row % 8 == 0 && q_head % 8 == 0;
   a.out = out;
+  a.out_wide = aligned(out, 16) && o_row % 8 == 0 && o_head % 8 == 0;
   a.o_row = o_row;
   a.o_head = o_head;
   a.lse = lse;

@@ -21,7 +21,7 @@ KV_EXPORTS = ("lx_kv_pool_bytes", "lx_kv_scratch_ints", "lx_kv_reset", "lx_kv_st
 
 DTYPES = {"bf16": 0, "fp16": 1, "fp32": 2}
 
-FULL, SLOT, WIDTH, PAGE, ROWS = 1, 2, 4, 8, 16  # bits of the error word
+FULL, SLOT, WIDTH, PAGE, ROWS, STUCK = 1, 2, 4, 8, 16, 32  # bits of the error word
 REFUSED = -2 ** 31  # start of an entry that extend did not serve
 
 
@@ -105,7 +105,7 @@ class KVCache:
         self._check(self._lib.lx_kv_reset(self._ref, stream or None), "reset")
 
     def status(self, stream: int = 0) -> int:
-        """Wait for the stream; the error bits since the last call (FULL, SLOT, WIDTH, PAGE, ROWS)."""
+        """Wait for the stream; the error bits since the last call (FULL, SLOT, WIDTH, PAGE, ROWS, STUCK)."""
         bits = ctypes.c_int32(0)
         self._check(self._lib.lx_kv_status(self._ref, ctypes.byref(bits), stream or None), "status")
         return bits.value
