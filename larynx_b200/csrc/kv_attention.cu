@@ -1052,8 +1052,8 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 // ---------------------------------------------------------------------------
 // tiles of 128 rows on tcgen05
 // ---------------------------------------------------------------------------
-// One CTA takes 128 rows and walks their keys 64 at a time.  Four warps unpack:
-// codes go from global memory through registers into operand tiles in shared memory (K
+// One CTA takes 128 rows and walks their keys 64 at a time.  Three warps unpack, a
+// block each in turn: codes go from global memory through registers into operand tiles in shared memory (K
 // as they are, V less 8, so that no further product is needed), a code being an fp16 subnormal as above, steps and minima
 // into fp32 arrays.  One thread issues the matrix instructions: S = Q K^T (a
 // sum for every group of channels, in tensor memory), one unit ahead of the softmax, and O += P V.
@@ -1068,7 +1068,8 @@ constexpr int TILE_KEYS = 64;
 
 template <int DIM, int GROUP>
 struct TileShape {
-  static constexpr int THREADS = 256;  // 4 warps that unpack (a thread of the first issues), 4 of softmax
+  static constexpr int THREADS = 256;  // a warp that issues, 3 that unpack, 4 of softmax
+  static constexpr int SLOTS = 4;      // units of unpacked keys
   static constexpr int H = DIM / 64, G = DIM / GROUP;
   static constexpr int CTAS = DIM == 64 ? 2 : 1;  // an SM
   // tensor memory: S (G sums a buffer), P, O
@@ -1088,8 +1089,14 @@ struct TileShape {
   static constexpr int V_BYTES = DIM * 128;
   static constexpr int PAR = 4 * G * TILE_KEYS * 4;  // ks, km, vs, vm
   static constexpr int SLOT = K_BYTES + V_BYTES;
-  static constexpr int SMEM = 1024 + Q_BYTES + 2 * SLOT + 2 * PAR + 256;
+  static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * (SLOT + PAR) + 512;
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 __device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
@@ -1116,27 +1123,30 @@ template <typename T, int DIM, int GROUP>
 __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(const __grid_constant__ Args a) {
   using S = TileShape<DIM, GROUP>;
   constexpr int H = S::H, G = S::G, BB = block_bytes(DIM, GROUP);
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that accesses stay known as shared)
   uint8_t* sq = smem;
   uint8_t* slots = sq + S::Q_BYTES;
-  float* par = reinterpret_cast<float*>(slots + 2 * S::SLOT);  // [slot][ks, km, vs, vm][G][64]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(par) + 2 * S::PAR);
-  // Each pair alternates by unit, and the next completion of a barrier always needs the waiter of the one before: no
-  // waiter is ever two phases behind.  empty[t & 1]: the product of unit t is done.
-  uint64_t *q_full = bars, *full = bars + 1, *empty = bars + 3, *s_full = bars + 5, *s_empty = bars + 7, *p_full = bars + 9;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
+  float* par = reinterpret_cast<float*>(slots + S::SLOTS * S::SLOT);  // [slot][ks, km, vs, vm][G][64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(par) + S::SLOTS * S::PAR);
+  // The next completion of each barrier needs the waiter of the one before: no waiter is ever two phases behind.
+  // empty[t % SLOTS]: the product of unit t is done.
+  uint64_t *q_full = bars, *full = bars + 1, *empty = full + S::SLOTS, *s_full = empty + S::SLOTS,
+           *s_empty = s_full + 2, *p_full = s_empty + 2;
+  float* v_top = reinterpret_cast<float*>(bars + 16);       // [slot][G][4] largest step of V in each block
+  int* have = reinterpret_cast<int*>(v_top + S::SLOTS * G * 4);  // [slot][4] blocks that exist
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(have + S::SLOTS * 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* have = reinterpret_cast<int*>(tmem_slot + 2);    // [slot][4] blocks that exist
-  float* v_top = reinterpret_cast<float*>(have + 8);    // [slot][2][G] largest step of V
-  static_assert(11 * 8 + 8 + 32 + 2 * 2 * 2 * 4 <= 256, "barriers");
+  static_assert(7 + 2 * S::SLOTS <= 16 && 16 * 8 + (G + 1) * S::SLOTS * 16 + 8 <= 512, "barriers");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 128);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&full[i], 128);
+    for (int i = 0; i < S::SLOTS; ++i) {
+      mbar_init(&full[i], 4);
       mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 4);
       mbar_init(&p_full[i], 4);
@@ -1179,7 +1189,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
   auto issue_pv = [&](int t) {
     if (!wait(&p_full[t & 1], t / 2)) return false;
     tc_fence_after();
-    const uint64_t dv = sdesc_sw128(smem_u32(slots + (t & 1) * S::SLOT + S::K_BYTES));
+    const uint64_t dv = sdesc_sw128(smem_u32(slots + t % S::SLOTS * S::SLOT + S::K_BYTES));
     const uint32_t p = tmem + S::P_COL + (t % S::P_BUFS) * (G * TILE_KEYS / 2);
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -1188,16 +1198,16 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
         umma_ts(tmem + S::O_COL + g * PV_N, p + g * (TILE_KEYS / 2) + 8 * k,
                 dv + static_cast<uint64_t>((g * PV_N * 128) >> 4) + 2 * k, idesc_f16_f32(128, PV_N),
                 t > 0 || k > 0 ? 1u : 0u);
-    umma_commit(&empty[t & 1]);
+    umma_commit(&empty[t % S::SLOTS]);
     return true;
   };
   // the scores of unit t, then the product of the unit before (the softmax of that one is under way meanwhile)
   auto issue = [&](int t) {
     if (t == 0 && !wait(q_full, 0)) return false;
-    if (!wait(&full[t & 1], t / 2)) return false;
+    if (!wait(&full[t % S::SLOTS], t / S::SLOTS)) return false;
     if (t >= S::S_BUFS && !wait(&s_empty[t % S::S_BUFS], t / S::S_BUFS - 1)) return false;
     tc_fence_after();
-    const uint64_t dq = sdesc_sw128(smem_u32(sq)), dk = sdesc_sw128(smem_u32(slots + (t & 1) * S::SLOT));
+    const uint64_t dq = sdesc_sw128(smem_u32(sq)), dk = sdesc_sw128(smem_u32(slots + t % S::SLOTS * S::SLOT));
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -1216,89 +1226,87 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
     // no such rows
   } else if (warp < 4) {
     if (S::SPLIT) regs_dec<S::UNPACK_REGS>();
-    // ---- unpack: warp w block w of each unit; thread x < 64 K's parameters of key x, the others V's of key x - 64
-    const int n = lane / 4, j = lane % 4, key = threadIdx.x % 64, side = threadIdx.x / 64;
-    const int32_t* table = a.c.table + static_cast<size_t>(s.e.slot < 0 ? 0 : s.e.slot) * a.c.max_pages;
-    const size_t head_bytes = static_cast<size_t>(BB) << a.block_lg;
-    const uint8_t* base = static_cast<const uint8_t*>(a.c.pool) +
-                          (static_cast<size_t>(a.layer) * a.c.n_pages * a.c.kv_heads + s.head) * head_bytes;
-    const int n_blocks = (hi_cta + BLOCK - 1) / BLOCK, mask = (1 << a.block_lg) - 1;
-    // first byte of block b of page p, or null
-    auto at = [&](int p, int b) -> const uint8_t* {
-      if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.c.n_pages)) return nullptr;
-      return base + static_cast<size_t>(p) * a.c.kv_heads * head_bytes + (b & mask) * BB;
-    };
-    auto look = [&](int b) { return b < n_blocks ? table[b >> a.block_lg] : -2; };
-    uint4 code[2][H];
-    uint32_t word[G];
-    bool here = false, key_here = false;
-    auto bring = [&](int t, int page, int key_page) {  // unit t
-      const int b = 4 * (tile0 + t) + warp, kb = 4 * (tile0 + t) + key / 16;
-      const uint8_t *p = at(page, b), *kp = at(key_page, kb);
-      here = p != nullptr;
-      key_here = kp != nullptr && (tile0 + t) * TILE_KEYS + key < s.len;
-      if (!here && page != -2 && lane == 0) flag(a.c, LX_KV_PAGE);
-#pragma unroll
-      for (int x = 0; x < 2 * H; ++x)
-        code[x / H][x % H] =
-            here ? *reinterpret_cast<const uint4*>(p + 512 * x + 16 * lane) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-        word[g] = key_here ? *reinterpret_cast<const uint32_t*>(kp + param_offset(DIM) + 64 * (side * G + g) +
-                                                                4 * param_slot(key % 16))
-                           : 0u;
-    };
-    int page = look(4 * tile0 + warp), key_page = look(4 * tile0 + key / 16);
-    if (n_tiles > 0) bring(0, page, key_page);
-    page = look(4 * (tile0 + 1) + warp);
-    key_page = look(4 * (tile0 + 1) + key / 16);
-    for (int t = 0; t < n_tiles; ++t) {
-      const int slot = t & 1;
-      if (t >= 2 && !__all_sync(0xffffffffu, wait(&empty[slot], t / 2 - 1))) break;
-      uint8_t* sk = slots + slot * S::SLOT;
-      uint8_t* sv = sk + S::K_BYTES;
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {  // K: word x is w = x % 2 of key n + 8 (x / 2)
-          const uint32_t k = x == 0 ? code[0][h].x : x == 1 ? code[0][h].y : x == 2 ? code[0][h].z : code[0][h].w;
-          const int row = 16 * warp + n + 8 * (x / 2);
-          *reinterpret_cast<uint4*>(sk + h * (TILE_KEYS * 128) + row * 128 + (((4 * (x % 2) + j) ^ (row & 7)) << 4)) =
-              make_uint4(k & M0, k & M1, k >> 8 & M0, k >> 8 & M1);
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {  // V: word x is w = x % 2 of keys 2 j, 2 j + 1 (+ 8 (x / 2))
-          const uint32_t v = x == 0 ? code[1][h].x : x == 1 ? code[1][h].y : x == 2 ? code[1][h].z : code[1][h].w;
-          uint8_t* row = sv + (64 * h + 32 * (x % 2) + n) * 128 + (((2 * warp + x / 2) ^ n) << 4) + 4 * j;
-          *reinterpret_cast<uint32_t*>(row) = less(v & M0, EIGHTS);
-          *reinterpret_cast<uint32_t*>(row + 8 * 128) = less(v & M1, EIGHTS << 4);
-          *reinterpret_cast<uint32_t*>(row + 16 * 128) = less(v >> 8 & M0, EIGHTS);
-          *reinterpret_cast<uint32_t*>(row + 24 * 128) = less(v >> 8 & M1, EIGHTS << 4);
-        }
+    if (warp == 0) {
+      if (lane == 0) {
+        bool ok = true;
+        for (int t = 0; ok && t < n_tiles; ++t) ok = issue(t);
+        if (ok && n_tiles > 0) issue_pv(n_tiles - 1);
       }
-      float* p = par + slot * (S::PAR / 4) + side * 2 * G * TILE_KEYS + key;
+    } else {
+      // ---- unpack: blocks warp - 1, warp + 2, ... of the CTA's keys.  Lane (n, j) has the codes of its place in the
+      // fragments, lane x the parameters at slot x % 16 of K (x < 16) or V.
+      const int n = lane / 4, j = lane % 4, side = lane / 16, sl = lane % 16;
+      const int token = sl / 4 * 2 + sl % 2 + sl % 4 / 2 * 8;
+      const int32_t* table = a.c.table + static_cast<size_t>(s.e.slot < 0 ? 0 : s.e.slot) * a.c.max_pages;
+      const uint32_t head_bytes = static_cast<uint32_t>(BB) << a.block_lg, page_bytes = head_bytes * a.c.kv_heads;
+      const uint8_t* base = static_cast<const uint8_t*>(a.c.pool) +
+                            (static_cast<uint64_t>(a.layer) * a.c.n_pages * a.c.kv_heads + s.head) * head_bytes;
+      const int first = 4 * tile0, n_blocks = (hi_cta + BLOCK - 1) / BLOCK - first, all = 4 * n_tiles;
+      const int in_page = (1 << a.block_lg) - 1;
+      auto look = [&](int b) { return b < n_blocks ? table[(first + b) >> a.block_lg] : -2; };
+      uint4 code[2][H];
+      uint32_t word[G];
+      bool here = false;
+      auto bring = [&](int b, int page) {
+        here = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.c.n_pages);
+        if (!here && page != -2 && lane == 0) flag(a.c, LX_KV_PAGE);
+        const uint8_t* p = base + static_cast<uint64_t>(static_cast<uint32_t>(here ? page : 0)) * page_bytes +
+                           (((first + b) & in_page) * BB);
+        const bool key = here && (first + b) * BLOCK + token < s.len;
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float step = step_of(word[g]), low = low_of(word[g]);
-        p[g * TILE_KEYS] = step;
-        p[(G + g) * TILE_KEYS] = side ? fmaf(step, 8.0f, low) : low;
-        if (side) {
-          const float v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(step, 0.0f))));
-          if (lane == 0) v_top[(slot * 2 + warp - 2) * G + g] = v;
+        for (int x = 0; x < 2 * H; ++x)
+          code[x / H][x % H] =
+              here ? *reinterpret_cast<const uint4*>(p + 512 * x + 16 * lane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          word[g] = key ? *reinterpret_cast<const uint32_t*>(p + param_offset(DIM) + 64 * (side * G + g) + 4 * sl) : 0u;
+      };
+      // places of this lane's stores in a slot, less what the block in it adds
+      const int k_at = n * 128 + ((j ^ n) << 4), v_at = n * 128 + 4 * j;
+      bring(warp - 1, look(warp - 1));
+      int page = look(warp + 2);
+      for (int b = warp - 1; b < all; b += 3) {
+        const int t = b / 4, block = b % 4, slot = t % S::SLOTS;
+        if (t >= S::SLOTS && !__all_sync(0xffffffffu, wait(&empty[slot], t / S::SLOTS - 1))) break;
+        uint8_t* sk = slots + slot * S::SLOT + block * (16 * 128) + k_at;
+        uint8_t* sv = slots + slot * S::SLOT + S::K_BYTES + v_at;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {  // K: word x is w = x % 2 of key n + 8 (x / 2)
+            const uint32_t k = x == 0 ? code[0][h].x : x == 1 ? code[0][h].y : x == 2 ? code[0][h].z : code[0][h].w;
+            uint8_t* to = x % 2 ? sk + (n & 4 ? -64 : 64) : sk;  // 16-byte piece (4 w + j) ^ n of the row
+            *reinterpret_cast<uint4*>(to + h * (TILE_KEYS * 128) + x / 2 * (8 * 128)) =
+                make_uint4(k & M0, k & M1, k >> 8 & M0, k >> 8 & M1);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {  // V: word x is w = x % 2 of keys 2 j, 2 j + 1 (+ 8 (x / 2))
+            const uint32_t v = x == 0 ? code[1][h].x : x == 1 ? code[1][h].y : x == 2 ? code[1][h].z : code[1][h].w;
+            uint8_t* to = sv + (((2 * block + x / 2) ^ n) << 4) + (64 * h + 32 * (x % 2)) * 128;
+            *reinterpret_cast<uint32_t*>(to) = less(v & M0, EIGHTS);
+            *reinterpret_cast<uint32_t*>(to + 8 * 128) = less(v & M1, EIGHTS << 4);
+            *reinterpret_cast<uint32_t*>(to + 16 * 128) = less(v >> 8 & M0, EIGHTS);
+            *reinterpret_cast<uint32_t*>(to + 24 * 128) = less(v >> 8 & M1, EIGHTS << 4);
+          }
         }
-      }
-      if (lane == 0) have[slot * 4 + warp] = here;
-      if (t + 1 < n_tiles) {
-        bring(t + 1, page, key_page);
-        page = look(4 * (tile0 + t + 2) + warp);
-        key_page = look(4 * (tile0 + t + 2) + key / 16);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&full[slot]);
-      if (warp == 0) {
-        bool ok = lane != 0 || issue(t);
-        if (lane == 0 && ok && t + 1 == n_tiles) ok = issue_pv(t);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        float* p = par + slot * (S::PAR / 4) + side * (2 * G * TILE_KEYS) + 16 * block + token;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float step = step_of(word[g]), low = low_of(word[g]);
+          p[g * TILE_KEYS] = step;
+          p[(G + g) * TILE_KEYS] = side ? fmaf(step, 8.0f, low) : low;
+          // (as whole numbers positive floats keep their order; a NaN or K's step counts as 0)
+          const uint32_t top = __reduce_max_sync(0xffffffffu, side ? __float_as_uint(fmaxf(step, 0.0f)) : 0u);
+          if (lane == 0) v_top[(slot * G + g) * 4 + block] = __uint_as_float(top);
+        }
+        if (lane == 0) have[slot * 4 + block] = here;
+        if (b + 3 < all) {
+          bring(b + 3, page);
+          page = look(b + 6);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
       }
     }
   } else {
@@ -1353,8 +1361,8 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
     int f_exp = 0;
     bool ok = true;
     for (int t = 0; t < n_tiles; ++t) {
-      const int slot = t & 1, key0 = (tile0 + t) * TILE_KEYS;
-      ok = wait(&full[slot], t / 2) && wait(&s_full[t % S::S_BUFS], t / S::S_BUFS);
+      const int slot = t % S::SLOTS, key0 = (tile0 + t) * TILE_KEYS;
+      ok = wait(&full[slot], t / S::SLOTS) && wait(&s_full[t % S::S_BUFS], t / S::S_BUFS);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -1363,24 +1371,24 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
       if (live) {
         // scores over c1
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int g = 0; g < G; ++g) {
+          float raw[2][32];
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            float raw[32];
-            tmem_ld32(t_lane + ((t % S::S_BUFS) * G + g) * TILE_KEYS + 32 * c, raw);
-            tmem_ld_wait();
+          for (int c = 0; c < 2; ++c) tmem_ld32(t_lane + ((t % S::S_BUFS) * G + g) * TILE_KEYS + 32 * c, raw[c]);
+          tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 st = ks[g * 16 + 8 * c + i], mi = ks[(G + g) * 16 + 8 * c + i];
-              float2 &u = x[16 * c + 2 * i], &v = x[16 * c + 2 * i + 1];
-              u = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.x, mi.y))
-                         : __ffma2_rn(both(qs[g]), make_float2(mi.x, mi.y), u);
-              v = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.z, mi.w))
-                         : __ffma2_rn(both(qs[g]), make_float2(mi.z, mi.w), v);
-              u = __ffma2_rn(make_float2(raw[4 * i], raw[4 * i + 1]), make_float2(st.x, st.y), u);
-              v = __ffma2_rn(make_float2(raw[4 * i + 2], raw[4 * i + 3]), make_float2(st.z, st.w), v);
-            }
+          for (int i = 0; i < 16; ++i) {
+            const float* r = raw[i / 8] + 4 * (i % 8);
+            const float4 st = ks[g * 16 + i], mi = ks[(G + g) * 16 + i];
+            float2 &u = x[2 * i], &v = x[2 * i + 1];
+            u = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.x, mi.y))
+                       : __ffma2_rn(both(qs[g]), make_float2(mi.x, mi.y), u);
+            v = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.z, mi.w))
+                       : __ffma2_rn(both(qs[g]), make_float2(mi.z, mi.w), v);
+            u = __ffma2_rn(make_float2(r[0], r[1]), make_float2(st.x, st.y), u);
+            v = __ffma2_rn(make_float2(r[2], r[3]), make_float2(st.z, st.w), v);
           }
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -1389,7 +1397,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
       auto p_free = [&](bool last) {
         const int before = last ? t - 1 : t - S::P_BUFS;
         if (before < 0) return true;
-        const bool w = __all_sync(0xffffffffu, wait(&empty[before & 1], before / 2));
+        const bool w = __all_sync(0xffffffffu, wait(&empty[before % S::SLOTS], before / S::SLOTS));
         tc_fence_after();
         return w;
       };
@@ -1413,16 +1421,18 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
           if (!(seen >> (2 * i + 1) & 1)) x[i].y = -INFINITY;
         }
       }
-      float top = -INFINITY, top1 = -INFINITY;
+      float tops[4];
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        top = fmaxf(fmaxf(top, x[i].x), x[i].y);
-        top1 = fmaxf(fmaxf(top1, x[i + 1].x), x[i + 1].y);
-      }
-      top = fmaxf(top, top1) * c1;
+      for (int i = 0; i < 4; ++i) tops[i] = max3(x[i].x, x[i].y, x[i + 4].x);
+#pragma unroll
+      for (int i = 4; i < 32; ++i) tops[i % 4] = i < 8 ? fmaxf(tops[i % 4], x[i].y) : max3(tops[i % 4], x[i].x, x[i].y);
+      const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * c1;
       float v = 0.0f;
 #pragma unroll
-      for (int g = 0; g < 2 * G; ++g) v = fmaxf(v, v_top[slot * 2 * G + g]);
+      for (int g = 0; g < G; ++g) {
+        const float4 w = *reinterpret_cast<const float4*>(v_top + (slot * G + g) * 4);
+        v = max3(v, max3(w.x, w.y, w.z), w.w);
+      }
       bool waited = false;
       if (__any_sync(0xffffffffu, top > limit || v > step_top)) {
         int up = 0;
@@ -1505,7 +1515,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[t & 1]);
     }
-    if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, wait(&empty[(n_tiles - 1) & 1], (n_tiles - 1) / 2));
+    if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, wait(&empty[(n_tiles - 1) % S::SLOTS], (n_tiles - 1) / S::SLOTS));
     if (ok && live) {
       tc_fence_after();
       const float sum = l.x + l.y;
@@ -1670,7 +1680,7 @@ bool go(Args& a, int max_len, cudaStream_t s) {
     if (rows <= 8) return wide ? few<T, DIM, GROUP, 1, WIDE>(a, units, s) : few<T, DIM, GROUP, 1, 4>(a, units, s);
     return wide ? few<T, DIM, GROUP, 2, 8>(a, units, s) : few<T, DIM, GROUP, 2, 4>(a, units, s);
   }
-  if (getenv("KV_TILE") && DIM / GROUP <= 2) return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, s);
+  if (getenv("KV_TILE") != nullptr && DIM / GROUP <= 2) return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, s);
   return rows <= 32 ? many<T, DIM, GROUP, 1, 2>(a, units, s) : many<T, DIM, GROUP, 1, 4>(a, units, s);
 }
 
