@@ -286,60 +286,86 @@ __device__ __forceinline__ void share_units(int lo, int hi, int rank, int split,
   }
 }
 
+// Four neighbouring channels of a row.
+template <typename T>
+__device__ __forceinline__ void put4(T* p, bool wide, float4 x) {
+  __align__(8) T e[4] = {static_cast<T>(x.x), static_cast<T>(x.y), static_cast<T>(x.z), static_cast<T>(x.w)};
+  if (wide) {
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = e[i];
+  }
+}
+
+// A part of a row: four channels of O, the row's maximum and sum; parts add up.
+struct Part {
+  float4 o;
+  float top, sum;
+  __device__ __forceinline__ void add(float4 x, float m, float l, float to) {
+    const float f = m == to ? 1.0f : ex2(m - to);
+    o.x = fmaf(x.x, f, o.x);
+    o.y = fmaf(x.y, f, o.y);
+    o.z = fmaf(x.z, f, o.z);
+    o.w = fmaf(x.w, f, o.w);
+    sum = fmaf(l, f, sum);
+  }
+};
+
 // Joins the parts of KW key groups, and of the CTAs of the cluster, and writes
 // the rows.  A part is O [rows][DIM] and, per row, the maximum and the sum.
 template <typename T, int DIM, int KW, int ROWS, int THREADS>
 __device__ __forceinline__ void join(const Args& a, const Share& s, float* part_o, float* part_m, float* part_l) {
+  constexpr int V = DIM / 4;
+  auto local = [&](int row, int v) {
+    Part p{make_float4(0, 0, 0, 0), part_m[row], 0.0f};
+#pragma unroll
+    for (int k = 1; k < KW; ++k) p.top = fmaxf(p.top, part_m[k * ROWS + row]);
+#pragma unroll
+    for (int k = 0; k < KW; ++k)
+      p.add(reinterpret_cast<const float4*>(part_o + (k * ROWS + row) * DIM)[v], part_m[k * ROWS + row],
+            part_l[k * ROWS + row], p.top);
+    return p;
+  };
+  auto write = [&](int row, int v, const Part& p) {
+    const int at = s.row0 + row, t = at / a.per, h = s.head * a.per + (at - t * a.per);
+    const float f = p.sum == 0.0f ? 0.0f : 1.0f / p.sum;
+    put4(static_cast<T*>(a.out) + (s.e.row0 + t) * a.o_row + h * a.o_head + 4 * v, a.out_wide,
+         make_float4(p.o.x * f, p.o.y * f, p.o.z * f, p.o.w * f));
+    if (a.lse && v == 0)
+      a.lse[static_cast<int64_t>(s.e.row0 + t) * a.q_heads + h] =
+          p.sum == 0.0f ? -INFINITY : (p.top + log2f(p.sum)) * 0.6931471805599453f;
+  };
+  if (a.split == 1) {
+    for (int x = threadIdx.x; x < s.n_rows * V; x += THREADS) write(x / V, x % V, local(x / V, x % V));
+    return;
+  }
   float* cta_o = part_o + (KW > 1 ? KW * ROWS * DIM : 0);
   float* cta_m = part_m + (KW > 1 ? KW * ROWS : 0);
   float* cta_l = part_l + (KW > 1 ? KW * ROWS : 0);
   if (KW > 1) {
-    for (int x = threadIdx.x; x < s.n_rows * DIM; x += THREADS) {
-      const int row = x / DIM;
-      float top = part_m[row];
-#pragma unroll
-      for (int k = 1; k < KW; ++k) top = fmaxf(top, part_m[k * ROWS + row]);
-      float o = 0.0f, sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const float mk = part_m[k * ROWS + row];
-        const float f = mk == top ? 1.0f : ex2(mk - top);
-        o = fmaf(part_o[k * ROWS * DIM + x], f, o);
-        sum = fmaf(part_l[k * ROWS + row], f, sum);
-      }
-      cta_o[x] = o;
-      if (x % DIM == 0) {
-        cta_m[row] = top;
-        cta_l[row] = sum;
+    for (int x = threadIdx.x; x < s.n_rows * V; x += THREADS) {
+      const int row = x / V, v = x % V;
+      const Part p = local(row, v);
+      reinterpret_cast<float4*>(cta_o + row * DIM)[v] = p.o;
+      if (v == 0) {
+        cta_m[row] = p.top;
+        cta_l[row] = p.sum;
       }
     }
   }
-  if (a.split > 1)
-    cg::this_cluster().sync();
-  else
-    __syncthreads();
-  for (int x = threadIdx.x + s.rank * THREADS; x < s.n_rows * DIM; x += a.split * THREADS) {
-    const int row = x / DIM, d = x % DIM;
-    float top = cta_m[row], o = cta_o[x], sum = cta_l[row];
-    if (a.split > 1) {
-      top = -INFINITY;
-      for (int k = 0; k < a.split; ++k) top = fmaxf(top, *cg::this_cluster().map_shared_rank(cta_m + row, k));
-      o = sum = 0.0f;
-      for (int k = 0; k < a.split; ++k) {
-        const float mk = *cg::this_cluster().map_shared_rank(cta_m + row, k);
-        const float f = mk == top ? 1.0f : ex2(mk - top);
-        o = fmaf(*cg::this_cluster().map_shared_rank(cta_o + x, k), f, o);
-        sum = fmaf(*cg::this_cluster().map_shared_rank(cta_l + row, k), f, sum);
-      }
-    }
-    const int t = (s.row0 + row) / a.per, h = s.head * a.per + (s.row0 + row - t * a.per);
-    static_cast<T*>(a.out)[(s.e.row0 + t) * a.o_row + h * a.o_head + d] =
-        static_cast<T>(sum == 0.0f ? 0.0f : o / sum);
-    if (a.lse && d == 0)
-      a.lse[static_cast<int64_t>(s.e.row0 + t) * a.q_heads + h] =
-          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  auto cluster = cg::this_cluster();
+  cluster.sync();
+  for (int x = threadIdx.x + s.rank * THREADS; x < s.n_rows * V; x += a.split * THREADS) {
+    const int row = x / V, v = x % V;
+    Part p{make_float4(0, 0, 0, 0), -INFINITY, 0.0f};
+    for (int k = 0; k < a.split; ++k) p.top = fmaxf(p.top, *cluster.map_shared_rank(cta_m + row, k));
+    for (int k = 0; k < a.split; ++k)
+      p.add(reinterpret_cast<const float4*>(cluster.map_shared_rank(cta_o + row * DIM, k))[v],
+            *cluster.map_shared_rank(cta_m + row, k), *cluster.map_shared_rank(cta_l + row, k), p.top);
+    write(row, v, p);
   }
-  if (a.split > 1) cg::this_cluster().sync();  // nobody leaves while its part may be read
+  cluster.sync();  // nobody leaves while its part may be read
 }
 
 // ---------------------------------------------------------------------------
@@ -1024,27 +1050,48 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
         low[g] += __shfl_xor_sync(0xffffffffu, low[g], 1);
         low[g] += __shfl_xor_sync(0xffffffffu, low[g], 2);
       }
-      if (row < s.n_rows) {
-        if (j == 0) {
+      if (row >= s.n_rows) continue;
+      const int at = s.row0 + row, t = at / a.per, h = s.head * a.per + (at - t * a.per);
+      T* out = static_cast<T*>(a.out) + (s.e.row0 + t) * a.o_row + h * a.o_head + 8 * j;
+      // without a split the row is whole: it is written from here
+      const float f = a.split > 1 ? back : sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (j == 0) {
+        if (a.split > 1) {
           part_m[row] = m[r][u];
           part_l[row] = sum * back;
+        } else if (a.lse) {
+          a.lse[static_cast<int64_t>(s.e.row0 + t) * a.q_heads + h] =
+              sum == 0.0f ? -INFINITY : (m[r][u] - f_exp + log2f(sum)) * 0.6931471805599453f;
         }
-        // columns 2 j, 2 j + 1 of product i are channels 8 j + i and 8 j + 4 + i, times 16 for odd i
+      }
+      // columns 2 j, 2 j + 1 of product i are channels 8 j + i and 8 j + 4 + i, times 16 for odd i
 #pragma unroll
-        for (int hw = 0; hw < 2 * H; ++hw)
+      for (int hw = 0; hw < 2 * H; ++hw) {
+        float y[8];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float(&y)[4][4] = o[r][hw / 2][hw % 2];
-            const float c = o8[r][32 * hw / GROUP][2 * u], w = low[32 * hw / GROUP];
-            float4 out;
-            out.x = fmaf(y[0][2 * u + x] - c, 16777216.0f, w) * back;
-            out.y = fmaf(fmaf(y[1][2 * u + x], 0.0625f, -c), 16777216.0f, w) * back;
-            out.z = fmaf(y[2][2 * u + x] - c, 16777216.0f, w) * back;
-            out.w = fmaf(fmaf(y[3][2 * u + x], 0.0625f, -c), 16777216.0f, w) * back;
-            *reinterpret_cast<float4*>(part_o + row * DIM + 32 * hw + 8 * j + 4 * x) = out;
+        for (int x = 0; x < 8; ++x)
+          y[x] = fmaf(fmaf(o[r][hw / 2][hw % 2][x % 4][2 * u + x / 4], x % 2 ? 0.0625f : 1.0f,
+                           -o8[r][32 * hw / GROUP][2 * u]),
+                      16777216.0f, low[32 * hw / GROUP]) *
+                 f;
+        if (a.split > 1) {
+          float4* to = reinterpret_cast<float4*>(part_o + row * DIM + 32 * hw + 8 * j);
+          to[0] = make_float4(y[0], y[1], y[2], y[3]);
+          to[1] = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+          __align__(16) T e[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) e[x] = static_cast<T>(y[x]);
+          if (a.out_wide) {
+            *reinterpret_cast<uint4*>(out + 32 * hw) = *reinterpret_cast<const uint4*>(e);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) out[32 * hw + x] = e[x];
           }
+        }
       }
     }
+  if (a.split == 1) return;
   __syncthreads();
   join<T, DIM, 1, S::ROWS, S::THREADS>(a, s, part_o, part_m, part_l);
 }
@@ -1052,7 +1099,8 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 // ---------------------------------------------------------------------------
 // tiles of 128 rows on tcgen05
 // ---------------------------------------------------------------------------
-// One CTA takes 128 rows and walks their keys 64 at a time.  Three warps unpack, a
+// One CTA takes 128 rows and walks their keys 128 at a time (64 where the sums for two
+// groups would not leave room for a second CTA).  Three warps unpack, a
 // block each in turn: codes go from global memory through registers into operand tiles in shared memory (K
 // as they are, V less 8, so that no further product is needed), a code being an fp16 subnormal as above, steps and minima
 // into fp32 arrays.  One thread issues the matrix instructions: S = Q K^T (a
@@ -1064,30 +1112,31 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 // which is how the unpacking warps write it without bank conflicts; the rows
 // are put in order when they are written out.
 constexpr int TILE_ROWS = 128;
-constexpr int TILE_KEYS = 64;
 
 template <int DIM, int GROUP>
 struct TileShape {
   static constexpr int THREADS = 256;  // a warp that issues, 3 that unpack, 4 of softmax
-  static constexpr int SLOTS = 4;      // units of unpacked keys
   static constexpr int H = DIM / 64, G = DIM / GROUP;
   static constexpr int CTAS = DIM == 64 ? 2 : 1;  // an SM
-  // tensor memory: S (G sums a buffer), P, O
-  static constexpr int S_BUFS = G == 1 || DIM == 128 ? 2 : 1;
-  static constexpr int P_BUFS = G == 1 ? 2 : 1;
-  static constexpr int P_COL = S_BUFS * G * TILE_KEYS;
-  static constexpr int O_COL = P_COL + P_BUFS * G * TILE_KEYS / 2;
+  // Keys of a unit.  What a unit costs whatever its keys (barriers, the vote on the maximum) was a quarter of the
+  // softmax's time at 64 keys.
+  static constexpr int KEYS = DIM == 64 && G == 2 ? 64 : 128;
+  static constexpr int BLOCKS = KEYS / BLOCK;
+  static constexpr int SLOTS = 256 / KEYS;  // units of unpacked keys
+  // tensor memory: S (a sum for each group), P, O
+  static constexpr int P_COL = G * KEYS;
+  static constexpr int O_COL = P_COL + G * KEYS / 2;
   static constexpr int COLS = DIM == 64 ? 256 : 512;
   // two CTAs an SM: the softmax takes registers from the unpacking (128 a thread at launch)
   static constexpr bool SPLIT = CTAS == 2;
-  static constexpr int LAUNCH_REGS = 128, UNPACK_REGS = 72, SOFTMAX_REGS = 184;
+  static constexpr int LAUNCH_REGS = 128, UNPACK_REGS = 64, SOFTMAX_REGS = 192;
   static_assert(UNPACK_REGS + SOFTMAX_REGS <= 2 * LAUNCH_REGS, "register split");
   static_assert(O_COL + DIM <= COLS, "tensor memory");
   // shared memory
   static constexpr int Q_BYTES = H * TILE_ROWS * 128;
-  static constexpr int K_BYTES = H * TILE_KEYS * 128;
-  static constexpr int V_BYTES = DIM * 128;
-  static constexpr int PAR = 4 * G * TILE_KEYS * 4;  // ks, km, vs, vm
+  static constexpr int K_BYTES = H * KEYS * 128;
+  static constexpr int V_BYTES = KEYS / 64 * DIM * 128;  // 64 keys of every channel, and the next 64
+  static constexpr int PAR = 4 * G * KEYS * 4;  // ks, km, vs, vm
   static constexpr int SLOT = K_BYTES + V_BYTES;
   static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * (SLOT + PAR) + 512;
 };
@@ -1098,10 +1147,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// (No memory clobber: it would keep the loads of the next keys' steps behind the store.)
 __device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -1127,30 +1176,28 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that accesses stay known as shared)
   uint8_t* sq = smem;
   uint8_t* slots = sq + S::Q_BYTES;
-  float* par = reinterpret_cast<float*>(slots + S::SLOTS * S::SLOT);  // [slot][ks, km, vs, vm][G][64]
+  float* par = reinterpret_cast<float*>(slots + S::SLOTS * S::SLOT);  // [slot][ks, km, vs, vm][G][KEYS]
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(par) + S::SLOTS * S::PAR);
   // The next completion of each barrier needs the waiter of the one before: no waiter is ever two phases behind.
   // empty[t % SLOTS]: the product of unit t is done.
   uint64_t *q_full = bars, *full = bars + 1, *empty = full + S::SLOTS, *s_full = empty + S::SLOTS,
-           *s_empty = s_full + 2, *p_full = s_empty + 2;
-  float* v_top = reinterpret_cast<float*>(bars + 16);       // [slot][G][4] largest step of V in each block
-  int* have = reinterpret_cast<int*>(v_top + S::SLOTS * G * 4);  // [slot][4] blocks that exist
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(have + S::SLOTS * 4);
+           *s_empty = s_full + 1, *p_full = s_empty + 1;
+  float* v_top = reinterpret_cast<float*>(bars + 16);                    // [slot][G][BLOCKS] largest step of V
+  int* have = reinterpret_cast<int*>(v_top + S::SLOTS * G * S::BLOCKS);  // [slot][BLOCKS] blocks that exist
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(have + S::SLOTS * S::BLOCKS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(7 + 2 * S::SLOTS <= 16 && 16 * 8 + (G + 1) * S::SLOTS * 16 + 8 <= 512, "barriers");
+  static_assert(4 + 2 * S::SLOTS + 1 <= 16 && 16 * 8 + (G + 1) * S::SLOTS * S::BLOCKS * 4 + 8 <= 512, "barriers");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 128);
     for (int i = 0; i < S::SLOTS; ++i) {
-      mbar_init(&full[i], 4);
+      mbar_init(&full[i], S::BLOCKS);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 4);
-      mbar_init(&p_full[i], 4);
-    }
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&p_full[i], 4);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -1178,26 +1225,27 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
     s.range(a, 0, lo_cta, x_);
     s.range(a, TILE_ROWS, x_, hi_cta);
   }
-  const int tile0 = lo_cta / TILE_KEYS;
-  const int n_tiles = any && hi_cta > lo_cta ? (hi_cta + TILE_KEYS - 1) / TILE_KEYS - tile0 : 0;
+  const int tile0 = lo_cta / S::KEYS;
+  const int n_tiles = any && hi_cta > lo_cta ? (hi_cta + S::KEYS - 1) / S::KEYS - tile0 : 0;
   auto wait = [&](uint64_t* bar, int use) {  // for the use-th completion of a barrier
     return mbar_wait(bar, static_cast<uint32_t>(use & 1), nullptr, abort_flag, 0);
   };
 
   // issue, by one thread: the product O += P V of unit t
   constexpr int PV_N = G == 1 ? DIM : GROUP;
+  const uint64_t dq = sdesc_sw128(smem_u32(sq)), dk0 = sdesc_sw128(smem_u32(slots)),
+                 dv0 = sdesc_sw128(smem_u32(slots + S::K_BYTES));
   auto issue_pv = [&](int t) {
     if (!wait(&p_full[t & 1], t / 2)) return false;
     tc_fence_after();
-    const uint64_t dv = sdesc_sw128(smem_u32(slots + t % S::SLOTS * S::SLOT + S::K_BYTES));
-    const uint32_t p = tmem + S::P_COL + (t % S::P_BUFS) * (G * TILE_KEYS / 2);
+    const uint64_t dv = dv0 + static_cast<uint64_t>(t % S::SLOTS * (S::SLOT >> 4));
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        umma_ts(tmem + S::O_COL + g * PV_N, p + g * (TILE_KEYS / 2) + 8 * k,
-                dv + static_cast<uint64_t>((g * PV_N * 128) >> 4) + 2 * k, idesc_f16_f32(128, PV_N),
-                t > 0 || k > 0 ? 1u : 0u);
+      for (int k = 0; k < S::BLOCKS; ++k)
+        umma_ts(tmem + S::O_COL + g * PV_N, tmem + S::P_COL + g * (S::KEYS / 2) + 8 * k,
+                dv + static_cast<uint64_t>((k / 4 * DIM * 128 + g * PV_N * 128) >> 4) + 2 * (k % 4),
+                idesc_f16_f32(128, PV_N), t > 0 || k > 0 ? 1u : 0u);
     umma_commit(&empty[t % S::SLOTS]);
     return true;
   };
@@ -1205,20 +1253,20 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
   auto issue = [&](int t) {
     if (t == 0 && !wait(q_full, 0)) return false;
     if (!wait(&full[t % S::SLOTS], t / S::SLOTS)) return false;
-    if (t >= S::S_BUFS && !wait(&s_empty[t % S::S_BUFS], t / S::S_BUFS - 1)) return false;
+    if (t > 0 && !wait(s_empty, t - 1)) return false;
     tc_fence_after();
-    const uint64_t dq = sdesc_sw128(smem_u32(sq)), dk = sdesc_sw128(smem_u32(slots + t % S::SLOTS * S::SLOT));
+    const uint64_t dk = dk0 + static_cast<uint64_t>(t % S::SLOTS * (S::SLOT >> 4));
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int k = 0; k < GROUP / 16; ++k) {
         const int c = g * GROUP / 16 + k, h = c / 4;  // 16 channels c of half h
-        umma_ss(tmem + ((t % S::S_BUFS) * G + g) * TILE_KEYS,
+        umma_ss(tmem + g * S::KEYS,
                 dq + static_cast<uint64_t>((h * TILE_ROWS * 128) >> 4) + 2 * (c % 4),
-                dk + static_cast<uint64_t>((h * TILE_KEYS * 128) >> 4) + 2 * (c % 4), idesc_f16_f32(128, TILE_KEYS),
+                dk + static_cast<uint64_t>((h * S::KEYS * 128) >> 4) + 2 * (c % 4), idesc_f16_f32(128, S::KEYS),
                 k > 0 ? 1u : 0u);
       }
-    umma_commit(&s_full[t % S::S_BUFS]);
+    umma_commit(s_full);
     return t == 0 || issue_pv(t - 1);
   };
 
@@ -1241,7 +1289,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
       const uint32_t head_bytes = static_cast<uint32_t>(BB) << a.block_lg, page_bytes = head_bytes * a.c.kv_heads;
       const uint8_t* base = static_cast<const uint8_t*>(a.c.pool) +
                             (static_cast<uint64_t>(a.layer) * a.c.n_pages * a.c.kv_heads + s.head) * head_bytes;
-      const int first = 4 * tile0, n_blocks = (hi_cta + BLOCK - 1) / BLOCK - first, all = 4 * n_tiles;
+      const int first = S::BLOCKS * tile0, n_blocks = (hi_cta + BLOCK - 1) / BLOCK - first, all = S::BLOCKS * n_tiles;
       const int in_page = (1 << a.block_lg) - 1;
       auto look = [&](int b) { return b < n_blocks ? table[(first + b) >> a.block_lg] : -2; };
       uint4 code[2][H];
@@ -1266,40 +1314,40 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
       bring(warp - 1, look(warp - 1));
       int page = look(warp + 2);
       for (int b = warp - 1; b < all; b += 3) {
-        const int t = b / 4, block = b % 4, slot = t % S::SLOTS;
+        const int t = b / S::BLOCKS, block = b % S::BLOCKS, slot = t % S::SLOTS;
         if (t >= S::SLOTS && !__all_sync(0xffffffffu, wait(&empty[slot], t / S::SLOTS - 1))) break;
         uint8_t* sk = slots + slot * S::SLOT + block * (16 * 128) + k_at;
-        uint8_t* sv = slots + slot * S::SLOT + S::K_BYTES + v_at;
+        uint8_t* sv = slots + slot * S::SLOT + S::K_BYTES + block / 4 * (DIM * 128) + v_at;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {  // K: word x is w = x % 2 of key n + 8 (x / 2)
             const uint32_t k = x == 0 ? code[0][h].x : x == 1 ? code[0][h].y : x == 2 ? code[0][h].z : code[0][h].w;
             uint8_t* to = x % 2 ? sk + (n & 4 ? -64 : 64) : sk;  // 16-byte piece (4 w + j) ^ n of the row
-            *reinterpret_cast<uint4*>(to + h * (TILE_KEYS * 128) + x / 2 * (8 * 128)) =
+            *reinterpret_cast<uint4*>(to + h * (S::KEYS * 128) + x / 2 * (8 * 128)) =
                 make_uint4(k & M0, k & M1, k >> 8 & M0, k >> 8 & M1);
           }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {  // V: word x is w = x % 2 of keys 2 j, 2 j + 1 (+ 8 (x / 2))
             const uint32_t v = x == 0 ? code[1][h].x : x == 1 ? code[1][h].y : x == 2 ? code[1][h].z : code[1][h].w;
-            uint8_t* to = sv + (((2 * block + x / 2) ^ n) << 4) + (64 * h + 32 * (x % 2)) * 128;
+            uint8_t* to = sv + (((2 * (block % 4) + x / 2) ^ n) << 4) + (64 * h + 32 * (x % 2)) * 128;
             *reinterpret_cast<uint32_t*>(to) = less(v & M0, EIGHTS);
             *reinterpret_cast<uint32_t*>(to + 8 * 128) = less(v & M1, EIGHTS << 4);
             *reinterpret_cast<uint32_t*>(to + 16 * 128) = less(v >> 8 & M0, EIGHTS);
             *reinterpret_cast<uint32_t*>(to + 24 * 128) = less(v >> 8 & M1, EIGHTS << 4);
           }
         }
-        float* p = par + slot * (S::PAR / 4) + side * (2 * G * TILE_KEYS) + 16 * block + token;
+        float* p = par + slot * (S::PAR / 4) + side * (2 * G * S::KEYS) + 16 * block + token;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const float step = step_of(word[g]), low = low_of(word[g]);
-          p[g * TILE_KEYS] = step;
-          p[(G + g) * TILE_KEYS] = side ? fmaf(step, 8.0f, low) : low;
+          p[g * S::KEYS] = step;
+          p[(G + g) * S::KEYS] = side ? fmaf(step, 8.0f, low) : low;
           // (as whole numbers positive floats keep their order; a NaN or K's step counts as 0)
           const uint32_t top = __reduce_max_sync(0xffffffffu, side ? __float_as_uint(fmaxf(step, 0.0f)) : 0u);
-          if (lane == 0) v_top[(slot * G + g) * 4 + block] = __uint_as_float(top);
+          if (lane == 0) v_top[(slot * G + g) * S::BLOCKS + block] = __uint_as_float(top);
         }
-        if (lane == 0) have[slot * 4 + block] = here;
+        if (lane == 0) have[slot * S::BLOCKS + block] = here;
         if (b + 3 < all) {
           bring(b + 3, page);
           page = look(b + 6);
@@ -1361,77 +1409,95 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
     int f_exp = 0;
     bool ok = true;
     for (int t = 0; t < n_tiles; ++t) {
-      const int slot = t % S::SLOTS, key0 = (tile0 + t) * TILE_KEYS;
-      ok = wait(&full[slot], t / S::SLOTS) && wait(&s_full[t % S::S_BUFS], t / S::S_BUFS);
+      const int slot = t % S::SLOTS, key0 = (tile0 + t) * S::KEYS;
+      ok = wait(&full[slot], t / S::SLOTS) && wait(s_full, t);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      float2 x[TILE_KEYS / 2];
+      float2 x[S::KEYS / 2];
       const float4* ks = reinterpret_cast<const float4*>(par + slot * (S::PAR / 4));
       if (live) {
         // scores over c1
+        float raw[G == 1 ? S::KEYS / 32 : 1][32];
+        if (G == 1) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          float raw[2][32];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) tmem_ld32(t_lane + ((t % S::S_BUFS) * G + g) * TILE_KEYS + 32 * c, raw[c]);
+          for (int c = 0; c < S::KEYS / 32; ++c) tmem_ld32(t_lane + 32 * c, raw[c * (G == 1)]);
           tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float* r = raw[i / 8] + 4 * (i % 8);
-            const float4 st = ks[g * 16 + i], mi = ks[(G + g) * 16 + i];
-            float2 &u = x[2 * i], &v = x[2 * i + 1];
-            u = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.x, mi.y))
-                       : __ffma2_rn(both(qs[g]), make_float2(mi.x, mi.y), u);
-            v = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.z, mi.w))
-                       : __ffma2_rn(both(qs[g]), make_float2(mi.z, mi.w), v);
-            u = __ffma2_rn(make_float2(r[0], r[1]), make_float2(st.x, st.y), u);
-            v = __ffma2_rn(make_float2(r[2], r[3]), make_float2(st.z, st.w), v);
-          }
         }
+#pragma unroll
+        for (int c = 0; c < S::KEYS / 32; ++c)
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            if (G > 1) {
+              tmem_ld32(t_lane + g * S::KEYS + 32 * c, raw[0]);
+              tmem_ld_wait();
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float* r = raw[c * (G == 1)] + 4 * i;
+              const float4 st = ks[g * (S::KEYS / 4) + 8 * c + i], mi = ks[(G + g) * (S::KEYS / 4) + 8 * c + i];
+              float2 &u = x[16 * c + 2 * i], &v = x[16 * c + 2 * i + 1];
+              u = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.x, mi.y))
+                         : __ffma2_rn(both(qs[g]), make_float2(mi.x, mi.y), u);
+              v = g == 0 ? __fmul2_rn(both(qs[0]), make_float2(mi.z, mi.w))
+                         : __ffma2_rn(both(qs[g]), make_float2(mi.z, mi.w), v);
+              u = __ffma2_rn(make_float2(r[0], r[1]), make_float2(st.x, st.y), u);
+              v = __ffma2_rn(make_float2(r[2], r[3]), make_float2(st.z, st.w), v);
+            }
+          }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[t % S::S_BUFS]);
-      // P may be written once the product that read its buffer is done
-      auto p_free = [&](bool last) {
-        const int before = last ? t - 1 : t - S::P_BUFS;
-        if (before < 0) return true;
-        const bool w = __all_sync(0xffffffffu, wait(&empty[before % S::SLOTS], before / S::SLOTS));
+      if (lane == 0) mbar_arrive(s_empty);
+      // P may be written once the product that read the last one is done
+      auto p_free = [&] {
+        if (t == 0) return true;
+        const bool w = __all_sync(0xffffffffu, wait(&empty[(t - 1) % S::SLOTS], (t - 1) / S::SLOTS));
         tc_fence_after();
         return w;
       };
       if (!live) {
-        if (!(ok = p_free(true))) break;
+        if (!(ok = p_free())) break;
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t & 1]);
         continue;
       }
-      const int4 got = *reinterpret_cast<const int4*>(have + 4 * slot);
-      const bool part = key0 < lo_all || key0 + TILE_KEYS > hi_all || !(got.x & got.y & got.z & got.w);
-      uint64_t seen = ~0ull;
-      if (part) {
-        const int first = min(max(lo - key0, 0), 64), past = min(max(hi - key0, 0), 64);
-        seen = past > first ? (past == 64 ? ~0ull : (1ull << past) - 1) & (~0ull << first) : 0ull;
-        seen &= (got.x ? 0xFFFFull : 0) | (got.y ? 0xFFFFull << 16 : 0) | (got.z ? 0xFFFFull << 32 : 0) |
-                (got.w ? 0xFFFFull << 48 : 0);
+      bool part = key0 < lo_all || key0 + S::KEYS > hi_all;
+      int4 got[S::BLOCKS / 4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (!(seen >> (2 * i) & 1)) x[i].x = -INFINITY;
-          if (!(seen >> (2 * i + 1) & 1)) x[i].y = -INFINITY;
+      for (int i = 0; i < S::BLOCKS / 4; ++i) {
+        got[i] = *reinterpret_cast<const int4*>(have + S::BLOCKS * slot + 4 * i);
+        part |= !(got[i].x & got[i].y & got[i].z & got[i].w);
+      }
+      uint32_t seen[S::KEYS / 32];
+      if (part) {
+#pragma unroll
+        for (int i = 0; i < S::KEYS / 32; ++i) {
+          const int first = min(max(lo - key0 - 32 * i, 0), 32), past = min(max(hi - key0 - 32 * i, 0), 32);
+          seen[i] = past > first ? (past == 32 ? ~0u : (1u << past) - 1) & (~0u << first) : 0u;
+          const int4 h = got[i / 2];
+          seen[i] &= ((i % 2 ? h.z : h.x) ? 0xFFFFu : 0u) | ((i % 2 ? h.w : h.y) ? 0xFFFF0000u : 0u);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            if (!(seen[i] >> (2 * k) & 1)) x[16 * i + k].x = -INFINITY;
+            if (!(seen[i] >> (2 * k + 1) & 1)) x[16 * i + k].y = -INFINITY;
+          }
         }
       }
       float tops[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) tops[i] = max3(x[i].x, x[i].y, x[i + 4].x);
 #pragma unroll
-      for (int i = 4; i < 32; ++i) tops[i % 4] = i < 8 ? fmaxf(tops[i % 4], x[i].y) : max3(tops[i % 4], x[i].x, x[i].y);
+      for (int i = 4; i < S::KEYS / 2; ++i) tops[i % 4] = i < 8 ? fmaxf(tops[i % 4], x[i].y) : max3(tops[i % 4], x[i].x, x[i].y);
       const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * c1;
       float v = 0.0f;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float4 w = *reinterpret_cast<const float4*>(v_top + (slot * G + g) * 4);
-        v = max3(v, max3(w.x, w.y, w.z), w.w);
+#pragma unroll
+        for (int i = 0; i < S::BLOCKS / 4; ++i) {
+          const float4 w = *reinterpret_cast<const float4*>(v_top + (slot * G + g) * S::BLOCKS + 4 * i);
+          v = max3(v, max3(w.x, w.y, w.z), w.w);
+        }
       }
       bool waited = false;
       if (__any_sync(0xffffffffu, top > limit || v > step_top)) {
@@ -1450,7 +1516,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
 #pragma unroll
         for (int g = 0; g < G; ++g) z[g] = __fmul2_rn(z[g], both(f));
         if (t > 0) {
-          if (!(ok = p_free(true))) break;  // the last product into O is done
+          if (!(ok = p_free())) break;  // the last product into O is done
           waited = true;
 #pragma unroll 1
           for (int c = 0; c < DIM / 32; ++c) {
@@ -1468,12 +1534,12 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
           tmem_st_wait();
         }
       }
-      if (!waited && !(ok = p_free(false))) break;
+      if (!waited && !(ok = p_free())) break;
       // p F, its sums, and P = p F s
       auto probabilities = [&](auto tag) {
         constexpr bool PART = decltype(tag)::value;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {  // 16 keys
+        for (int c = 0; c < S::BLOCKS; ++c) {  // 16 keys
           uint32_t w[G][8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -1486,13 +1552,14 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-              const float4 st = ks[(2 * G + g) * 16 + 4 * c + i], mi = ks[(3 * G + g) * 16 + 4 * c + i];
+              const float4 st = ks[(2 * G + g) * (S::KEYS / 4) + 4 * c + i],
+                           mi = ks[(3 * G + g) * (S::KEYS / 4) + 4 * c + i];
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 float2 y = __fmul2_rn(p[k], k ? make_float2(st.z, st.w) : make_float2(st.x, st.y));
                 float2 low = k ? make_float2(mi.z, mi.w) : make_float2(mi.x, mi.y);
                 if (PART) {  // a key that the row does not see: not even its NaN counts
-                  const uint32_t in = static_cast<uint32_t>(seen >> (16 * c + 4 * i + 2 * k));
+                  const uint32_t in = seen[c / 2] >> (16 * (c % 2) + 4 * i + 2 * k);
                   if (!(in & 1)) y.x = low.x = 0.0f;
                   if (!(in & 2)) y.y = low.y = 0.0f;
                 }
@@ -1503,7 +1570,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
           }
 #pragma unroll
           for (int g = 0; g < G; ++g)
-            tmem_st8u(t_lane + S::P_COL + ((t % S::P_BUFS) * G + g) * (TILE_KEYS / 2) + 8 * c, w[g]);
+            tmem_st8u(t_lane + S::P_COL + g * (S::KEYS / 2) + 8 * c, w[g]);
         }
       };
       if (part)
@@ -1518,7 +1585,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
     if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, wait(&empty[(n_tiles - 1) % S::SLOTS], (n_tiles - 1) / S::SLOTS));
     if (ok && live) {
       tc_fence_after();
-      const float sum = l.x + l.y;
+      const float sum = l.x + l.y, f = sum == 0.0f ? 0.0f : 1.0f / sum;
       const int r = s.row0 + row, q_row = r / a.per, h = s.head * a.per + (r - q_row * a.per);
       T* out = static_cast<T*>(a.out) + (s.e.row0 + q_row) * a.o_row + h * a.o_head;
 #pragma unroll 1
@@ -1537,7 +1604,7 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
 #pragma unroll
           for (int i = 0; i < 32; ++i) {  // column 8 i + n is channel 4 n + i, times 16 for odd i
             const float b = fmaf(y[i], (i / 8) % 2 ? 1048576.0f : 16777216.0f, low);
-            e[4 * (i % 8) + i / 8] = static_cast<T>(sum == 0.0f ? 0.0f : b / sum);
+            e[4 * (i % 8) + i / 8] = static_cast<T>(b * f);
           }
           if (a.out_wide) {
 #pragma unroll
@@ -1602,11 +1669,11 @@ void set_up(K kernel, Launch& l, int threads, int smem, cudaLaunchConfig_t& cfg,
 
 // Launches `items` (tiles of rows x kv heads) with the keys of each split over a
 // cluster: as finely as all items still run at once and each key group has a
-// unit (`groups` a CTA); where even whole items do not all run at once, into twice as many
-// CTAs as do, so that the last ones leave little of the GPU idle.
+// unit (`groups` a CTA).  `halve`: where whole items take one to two rounds of the GPU, into halves, so
+// that the last ones leave less of it idle (64 x 8 items over 4099-8191 keys: 105 us against 116).
 template <typename K>
 bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_rows, int groups, int units,
-           cudaStream_t s) {
+           bool halve, cudaStream_t s) {
   Launch& l = launches[a.c.device & 63];
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
@@ -1618,7 +1685,7 @@ bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_
   int split = 1;
   for (int k = 2; k <= most; ++k)
     if (l.active[k] >= items) split = k;
-  if (split == 1 && items > l.active[1] / 2 && items < 2 * l.active[1] && most >= 8) split = 2;
+  if (halve && split == 1 && items > l.active[1] / 2 && items < 2 * l.active[1] && most >= 8) split = 2;
   if (items * split > 0x7fffffff) return false;
   a.tiles = static_cast<int>(tiles);
   a.split = split;
@@ -1637,13 +1704,13 @@ template <typename T, int DIM, int GROUP, int NT, int KW>
 bool few(Args& a, int units, cudaStream_t s) {
   using S = FewShape<DIM, GROUP, NT, KW>;
   static Launch launches[64];
-  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, s);
+  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, true, s);
 }
 template <typename T, int DIM, int GROUP, int MT, int MW>
 bool many(Args& a, int units, cudaStream_t s) {
   using S = ManyShape<DIM, GROUP, MT, MW>;
   static Launch launches[64];
-  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 4, units, s);
+  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 4, units, false, s);
 }
 
 template <typename T, int DIM, int GROUP>
@@ -1680,7 +1747,11 @@ bool go(Args& a, int max_len, cudaStream_t s) {
     if (rows <= 8) return wide ? few<T, DIM, GROUP, 1, WIDE>(a, units, s) : few<T, DIM, GROUP, 1, 4>(a, units, s);
     return wide ? few<T, DIM, GROUP, 2, 8>(a, units, s) : few<T, DIM, GROUP, 2, 4>(a, units, s);
   }
-  if (getenv("KV_TILE") != nullptr && DIM / GROUP <= 2) return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, s);
+  // Tiles of 128 rows win above 64 rows (64 x 8 items over 1000 keys, us: 64 rows 60 against 61, 96 rows 64 against
+  // 105, 128 rows 68 against 106), if there is one for every SM: they do not split the keys (8 tiles over 4000 keys: 73
+  // against 22).  Sums for four groups do not fit the tensor memory.
+  if (DIM / GROUP <= 2 && rows > 64 && items * ((rows + TILE_ROWS - 1) / TILE_ROWS) >= num_sms())
+    return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, s);
   return rows <= 32 ? many<T, DIM, GROUP, 1, 2>(a, units, s) : many<T, DIM, GROUP, 1, 4>(a, units, s);
 }
 

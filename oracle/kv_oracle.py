@@ -57,21 +57,41 @@ def quantise_group(x):
     return codes, s, m
 
 
+def _quantise_rows(flat):
+    """Rows of float32 -> values they stand for and steps.  In float64 where that decides surely, else exactly."""
+    wide = flat.astype(np.float64)
+    ok = np.isfinite(flat).all(-1)
+    low, high = np.where(ok[:, None], wide, 0).min(-1), np.where(ok[:, None], wide, 0).max(-1)
+    bits = low.astype(np.float32).view(np.uint32).astype(np.int64)
+    m = bf16_bits_value((bits + np.where(bits >> 31, 0xFFFF, 0)) >> 16).astype(np.float64)
+    part, power = np.frexp((high - m) / 15)
+    s = np.ldexp(np.ceil(part * 256), power - 8)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        q = (wide - m[:, None]) / s[:, None]
+        codes = np.rint(q)
+        near = np.abs(np.abs(q - np.floor(q)) - 0.5) < 1e-9  # of a tie
+        edge = np.abs(part * 256 - np.rint(part * 256)) < 1e-9  # of a bf16 step
+    size = np.abs(np.where(ok[:, None], wide, 0)).max(-1)
+    sure = ok & ~near.any(-1) & ~edge & (s > 1e-30) & (s > size * 2.0 ** -20) & (size < 1e30)
+    values, steps_ = np.empty(flat.shape, np.float32), np.where(sure, s, 0)
+    values[sure] = (codes * s[:, None] + m[:, None])[sure].astype(np.float32)
+    for i in np.flatnonzero(~sure):
+        codes_i, s_i, m_i = quantise_group(flat[i])
+        values[i] = np.nan if codes_i is None else (codes_i * float(s_i) + float(m_i)).astype(np.float32)
+        steps_[i] = s_i
+    return values, steps_
+
+
 def quantise(x, group):
     """[..., dim] -> the float32 values that its groups stand for."""
-    x = np.asarray(x, np.float32)
-    flat = x.reshape(-1, group)
-    out = np.empty(flat.shape, np.float32)
-    for i, row in enumerate(flat):
-        codes, s, m = quantise_group(row)
-        out[i] = np.nan if codes is None else (codes * float(s) + float(m)).astype(np.float32)
-    return out.reshape(x.shape)
+    x = np.ascontiguousarray(x, np.float32)
+    return _quantise_rows(x.reshape(-1, group))[0].reshape(x.shape)
 
 
 def steps(x, group):
     """[..., dim] -> the step s of each value's group, in float64."""
-    flat = np.asarray(x, np.float32).reshape(-1, group)
-    return np.repeat([float(quantise_group(row)[1]) for row in flat], group).reshape(np.shape(x))
+    x = np.ascontiguousarray(x, np.float32)
+    return np.repeat(_quantise_rows(x.reshape(-1, group))[1], group).reshape(x.shape)
 
 
 def unpack_block(block, dim, group):
@@ -104,31 +124,35 @@ def visible(p: int, length: int, chunk: int, left: int):
 def attention(q, k, v, step, positions, scale, chunk, left, seen=None):
     """q [rows, heads, dim], k and v [keys, kv heads, dim] in float64; step: those of v's groups.  Returns
     out, lse, and parts of a bound: the largest sum of |q| |k| scale over the visible keys of each (row, head);
-    per output the weighted sums of |v| and of 8 steps, and the keys times the largest step.
+    per output the weighted sums of |v| and of 8 steps, and the keys times the largest step of all.
     `seen`: keys that exist (bool), default all."""
     rows, heads, dim = q.shape
-    per = heads // k.shape[1]
+    kv = k.shape[1]
+    per = heads // kv
+    keys = np.arange(k.shape[0])
+    span = np.array([visible(p, k.shape[0], chunk, left) for p in positions], np.int64).reshape(rows, 2)
+    see = (keys >= span[:, :1]) & (keys < span[:, 1:])  # [rows, keys]
+    if seen is not None:
+        see &= seen
+    none = ~see.any(-1)
     out, lse = np.zeros(q.shape), np.full((rows, heads), -np.inf)
     size, weight, coarse, most = np.zeros((rows, heads)), np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape)
-    for r, p in enumerate(positions):
-        lo, hi = visible(p, k.shape[0], chunk, left)
-        at = np.arange(lo, max(lo, hi))
-        if seen is not None:
-            at = at[seen[at]]
-        if at.size == 0:
-            continue
-        for h in range(heads):
-            kk, vv = k[at, h // per], v[at, h // per]
-            s = kk @ q[r, h] * scale
-            top = s.max()
-            w = np.exp(s - top)
-            lse[r, h] = top + np.log(w.sum())
-            w /= w.sum()
-            out[r, h] = w @ vv
-            size[r, h] = (np.abs(kk) @ np.abs(q[r, h])).max() * abs(scale)
-            weight[r, h] = w @ np.abs(vv)
-            coarse[r, h] = w @ step[at, h // per] * 8
-            most[r, h] = at.size * step[at, h // per].max(0)
+    if k.shape[0] == 0 or none.all():
+        return out, lse, size, weight, coarse, most
+    for h in range(heads):
+        g = h // per
+        kk, vv, st = (np.where(see.any(0)[:, None], x[:, g], 0.0) for x in (k, v, step))  # what nobody sees may be NaN
+        s = np.where(see, q[:, h] @ kk.T * scale, -np.inf)
+        top = np.where(none, 0.0, s.max(-1))
+        w = np.exp(s - top[:, None])
+        total = np.where(none, 1.0, w.sum(-1))
+        lse[:, h] = np.where(none, -np.inf, top + np.log(total))
+        w /= total[:, None]
+        out[:, h] = w @ vv
+        size[:, h] = np.where(see, np.abs(q[:, h]) @ np.abs(kk).T, 0.0).max(-1) * abs(scale)
+        weight[:, h] = w @ np.abs(vv)
+        coarse[:, h] = w @ st * 8
+        most[:, h] = see.sum(-1)[:, None] * st.max(0)
     return out, lse, size, weight, coarse, most
 
 

@@ -331,6 +331,62 @@ def test_attention(case, dtype):
         at += n
 
 
+@pytest.mark.parametrize("dim,group,page,chunk,left", [(64, 64, 16, 1, -1), (64, 32, 32, 0, -1), (128, 64, 64, 20, 33),
+                                                       (64, 64, 64, 25, 0), (128, 32, 16, 1, 50)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attention_many_entries(dim, group, page, chunk, left, dtype):
+    """Enough rows for the whole GPU: ragged entries of up to 140 rows, empty and refused ones among them, a page
+    outside the pool, NaN in keys that some rows must not see, strided output."""
+    heads, per, n = 3, 2, 60
+    rng = np.random.default_rng(dim + group + chunk)
+    lengths = rng.integers(1, 200, n).tolist()
+    lengths[3], lengths[7], lengths[11] = 0, 256, 128
+    counts = [int(min(rng.integers(1, 71), 70)) for _ in lengths]
+    counts[7], counts[9], counts[11] = 70, 0, 64
+    c = Cache(n_pages=sum(-(-x // page) for x in lengths) + 3, n_seq=n, max_pages=-(-256 // page) + 1, heads=heads, dim=dim,
+              group=group, page=page, fill=0xFF)
+    held = c.fill(lengths, seed=chunk)
+    start = [x - m for x, m in zip(lengths, counts)]
+    start[20] = ko.REFUSED
+    bad = torch.full((1, heads, dim), float("nan"), device="cuda")
+    c.write(bad, bad, c.batch([1], seqs=[7], start=[255]), "fp32")  # the last key of the longest
+    lost = None
+    if page == 16:
+        lost = 11
+        c.table[11, 3] = -7
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn(sum(counts), heads * per, dim, generator=g).to(TORCH[dtype])
+    out = torch.full((sum(counts) + 1, heads * per, dim + 8), 3.0, dtype=TORCH[dtype], device="cuda")
+    lse = torch.full((sum(counts), heads * per), 3.0, device="cuda")
+    qd = q.cuda()
+    rows = c.batch(counts, start=start)
+    c.c.attention(0, rows, heads * per, dtype, qd.data_ptr(), out.data_ptr(), lse=lse.data_ptr(), scale=-0.2, chunk=chunk,
+                  left=left, out_strides=(out.stride(0), out.stride(1)))
+    torch.cuda.synchronize()
+    assert c.c.status() == (c.kv.PAGE if lost else 0)
+    assert (out[-1] == 3).all() and (out[..., dim:] == 3).all()
+    at = 0
+    for i, (k, v, st) in enumerate(held):
+        m = counts[i]
+        o, l = out[at:at + m, :, :dim], lse[at:at + m]
+        pos = [start[i] + t for t in range(m)]
+        seen = np.ones(len(k), bool)
+        if i == lost:
+            seen[48:64] = False
+        if i == 7:  # the rows that see the NaN are NaN throughout, the others know nothing of it
+            hit = np.array([ko.visible(p, 256, chunk, left)[1] == 256 for p in pos])
+            assert torch.isnan(o[hit]).all() and torch.isnan(l[hit]).all() and hit.any()
+            o, l, pos, qq = o[~hit], l[~hit], [p for p, b in zip(pos, hit) if not b], q[at:at + m][~hit]
+            assert chunk == 0 or len(pos)
+        else:
+            qq = q[at:at + m]
+        if i == 20:
+            assert (o == 0).all() and torch.isneginf(l).all()
+        elif len(pos):
+            check(o, l, ko.attention(qq.double().numpy(), k, v, st, pos, -0.2, chunk, left, seen=seen), dtype)
+        at += m
+
+
 @pytest.mark.parametrize("length", [1, 15, 16, 255, 1025, 4099])
 @pytest.mark.parametrize("dim,per", [(64, 1), (128, 4)])
 def test_attention_long(length, dim, per):

@@ -150,3 +150,17 @@ def test_oracle_quantiser():
     assert ko.quantise_group(np.full(32, 3.0, np.float32))[0].max() == 0
     assert ko.quantise_group(np.array([1, np.inf], np.float32))[0] is None
     assert ko.quantise_group(np.array([-3e38, 3e38], np.float32))[0] is None
+
+
+def test_oracle_quantiser_in_bulk_is_the_exact_one():
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((300, 32)).astype(np.float32)
+    x[100:200] = ((x[100:200].view(np.uint32) >> 16) << 16).view(np.float32)  # bf16: ties
+    x[200:220] *= np.exp(rng.uniform(-30, 30, (20, 32))).astype(np.float32)
+    x[220] = 1.5
+    x[221, 3] = np.nan
+    got, steps = ko.quantise(x, 32), ko.steps(x, 32)
+    for i, row in enumerate(x):
+        codes, s, m = ko.quantise_group(row)
+        want = np.full(32, np.nan, np.float32) if codes is None else (codes * float(s) + float(m)).astype(np.float32)
+        assert np.array_equal(got[i], want, equal_nan=True) and np.array_equal(steps[i, 0], s, equal_nan=True)
