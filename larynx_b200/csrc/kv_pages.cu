@@ -357,25 +357,36 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_kv_move(const lx_kv_cache c) {
   const int pieces = static_cast<int>((bytes + PIECE - 1) / PIECE);
   const long long items = static_cast<long long>(moves) * c.n_layers * pieces;
   uint8_t* pool = static_cast<uint8_t*>(c.pool);
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+  // the next piece is read while one is written
+  uint4 x[2][4];
+  uint8_t* to[2] = {nullptr, nullptr};
+  int left[2] = {0, 0};
+  auto read = [&](long long it, int buf) {
+    left[buf] = 0;
+    if (it >= items) return;
     const int piece = static_cast<int>(it % pieces);
     const int layer = static_cast<int>(it / pieces % c.n_layers), m = static_cast<int>(it / pieces / c.n_layers);
-    const int from = src_list(c)[m], to = dst_list(c)[m];
-    if (!page_ok(c, from) || !page_ok(c, to)) continue;
-    const size_t off = static_cast<size_t>(piece) * PIECE;
-    const uint8_t* s = pool + (static_cast<size_t>(layer) * c.n_pages + from) * bytes + off;
-    uint8_t* d = pool + (static_cast<size_t>(layer) * c.n_pages + to) * bytes + off;
-    uint4 x[4];
+    const int from = src_list(c)[m], page = dst_list(c)[m];
+    if (!page_ok(c, from) || !page_ok(c, page)) return;
+    const size_t off = static_cast<size_t>(piece) * PIECE, plane = static_cast<size_t>(layer) * c.n_pages;
+    const uint8_t* s = pool + (plane + from) * bytes + off + 16 * threadIdx.x;
+    to[buf] = pool + (plane + page) * bytes + off + 16 * threadIdx.x;
+    left[buf] = static_cast<int>(min(bytes - off, static_cast<size_t>(PIECE))) - 16 * static_cast<int>(threadIdx.x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const size_t o = 16 * (threadIdx.x + static_cast<size_t>(i) * MOVE_THREADS);
-      if (off + o < bytes) x[i] = *reinterpret_cast<const uint4*>(s + o);
-    }
+    for (int i = 0; i < 4; ++i)
+      if (16 * MOVE_THREADS * i < left[buf]) x[buf][i] = __ldcs(reinterpret_cast<const uint4*>(s + 16 * MOVE_THREADS * i));
+  };
+  auto write = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const size_t o = 16 * (threadIdx.x + static_cast<size_t>(i) * MOVE_THREADS);
-      if (off + o < bytes) *reinterpret_cast<uint4*>(d + o) = x[i];
-    }
+    for (int i = 0; i < 4; ++i)
+      if (16 * MOVE_THREADS * i < left[buf]) __stcs(reinterpret_cast<uint4*>(to[buf] + 16 * MOVE_THREADS * i), x[buf][i]);
+  };
+  read(blockIdx.x, 0);
+  for (long long it = blockIdx.x; it < items; it += 2ll * gridDim.x) {
+    read(it + gridDim.x, 1);
+    write(0);
+    read(it + 2ll * gridDim.x, 0);
+    write(1);
   }
   if (REMAP) {
     const int u = c.scratch[USED];
@@ -400,7 +411,7 @@ bool batch_ok(const lx_kv_cache* c, int n, const void* a, const void* b) {
 
 template <bool REMAP>
 bool move(const lx_kv_cache& c, cudaStream_t s) {
-  return launch(k_kv_move<REMAP>, dim3(4 * num_sms()), dim3(MOVE_THREADS), 0, s, c);
+  return launch(k_kv_move<REMAP>, dim3(16 * num_sms()), dim3(MOVE_THREADS), 0, s, c);
 }
 
 template <bool COPY>
