@@ -24,7 +24,7 @@
 // share the keys' bytes.  In both a cluster of CTAs splits the keys of long
 // sequences, joined through shared memory in a fixed order: no workspace in
 // global memory, so calls may overlap.  The bytes come through rings of
-// cp.async stages.
+// bulk copies, two blocks a stage.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -47,21 +47,39 @@ constexpr int P_TOP = 7;              // F x the largest step is 2^7 at most: 2^
 constexpr float STEP_MIN = 8.0779357e-28f;  // 2^-90: F stays below 2^101, so that sums of p F do not overflow
 constexpr float STEP_MAX = 8.5070592e37f;   // 2^126
 
+// Division of 32-bit numbers by one that the host knows (multiply high, two shifts; exact for all of them).  A
+// block begins with a dozen of divisions, and each took twenty instructions of every warp.
+struct Divisor {
+  uint32_t d, mul, shift1, shift2;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by) {
+    uint32_t l = 0;
+    while ((1ull << l) < by) ++l;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - by)) / by + 1);
+    shift1 = l < 1 ? l : 1;
+    shift2 = l > 0 ? l - 1 : 0;
+  }
+  __device__ __forceinline__ int over(int n) const {  // n / d, n >= 0
+    const uint32_t x = static_cast<uint32_t>(n), t = __umulhi(mul, x);
+    return static_cast<int>((t + ((x - t) >> shift1)) >> shift2);
+  }
+};
+
 struct Mask {
-  int chunk, left;
+  Divisor chunk;  // 0: none
+  int left;
   // keys [lo, hi) that a row at position p sees
   __device__ __forceinline__ void range(int p, int len, int& lo, int& hi) const {
     lo = 0;
     hi = len;
-    if (chunk > 0) {
-      int at = p;
-      if (chunk > 1) {
-        at = p / chunk;
-        if (p < 0 && at * chunk != p) --at;  // rounds down
+    if (chunk.d > 0) {
+      const int c = static_cast<int>(chunk.d), at = p >= 0 ? chunk.over(p) : ~chunk.over(~p), begin = at * c;
+      if (begin < 0) {
+        hi = max(0, min(len, begin + c));
+      } else {
+        hi = begin >= len ? len : static_cast<int>(min(static_cast<uint32_t>(len), static_cast<uint32_t>(begin) + c));
+        if (left >= 0) lo = max(0, begin - left);
       }
-      const long long begin = static_cast<long long>(at) * chunk;
-      hi = static_cast<int>(max(0ll, min(static_cast<long long>(len), begin + chunk)));
-      if (left >= 0) lo = static_cast<int>(max(0ll, begin - left));
     }
   }
 };
@@ -95,13 +113,11 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Bulk copy of `bytes` (a multiple of 16) into this CTA's shared memory, counted on an mbarrier.
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 __device__ __forceinline__ uint4 lds128(const void* p) { return *reinterpret_cast<const uint4*>(p); }
@@ -126,7 +142,8 @@ __device__ __forceinline__ int step_exponent(float v) {
 struct Args {
   lx_kv_cache c;
   lx_kv_rows r;
-  int layer, q_heads, per, tiles, split, block_lg;  // block_lg: log2 of the blocks of a page
+  int layer, q_heads, split, block_lg;  // block_lg: log2 of the blocks of a page
+  Divisor per, heads, tiles, split_by, items;  // query heads a kv head, kv heads, tiles of rows, split, n x kv heads
   const void* q;
   int64_t q_row, q_head;
   bool wide, out_wide;  // 16-byte accesses
@@ -171,9 +188,10 @@ struct Share {
   int head, row0, n_rows, rows, len, start, rank;
   // the rows of the CTA are rows row0 .. row0 + n_rows - 1 of the entry's (query row, query head) pairs
   __device__ __forceinline__ bool take(const Args& a, int tile_rows) {
-    rank = blockIdx.x % a.split;
-    const int item = blockIdx.x / a.split, x = item / a.c.kv_heads;
-    return take_at(a, x / a.tiles, item % a.c.kv_heads, x % a.tiles, tile_rows);
+    const int block = static_cast<int>(blockIdx.x), item = a.split_by.over(block), x = a.heads.over(item);
+    const int entry = a.tiles.over(x);
+    rank = block - item * a.split;
+    return take_at(a, entry, item - x * a.c.kv_heads, x - entry * static_cast<int>(a.tiles.d), tile_rows);
   }
   __device__ __forceinline__ bool take_at(const Args& a, int entry, int kv_head, int tile, int tile_rows) {
     head = kv_head;
@@ -183,7 +201,7 @@ struct Share {
     const int length = a.c.lengths[ok ? slot : 0], given = a.r.start ? a.r.start[entry] : 0;
     const int first = a.r.row0 ? a.r.row0[entry] : 0, end = a.r.row0 ? a.r.row0[entry + 1] : 0;
     e = entry_of(a.c, a.r, slot, first, end, entry);
-    rows = e.rows * a.per;
+    rows = e.rows * static_cast<int>(a.per.d);
     row0 = tile * tile_rows;
     if (row0 >= rows) return false;  // for the whole cluster
     n_rows = min(tile_rows, rows - row0);
@@ -198,91 +216,109 @@ struct Share {
   // keys that row `row` (behind the last one: the last one) of the CTA sees
   __device__ __forceinline__ void range(const Args& a, int row, int& lo, int& hi) const {
     lo = hi = 0;
-    if (start != LX_KV_REFUSED) a.mask.range(start + (row0 + min(row, n_rows - 1)) / a.per, len, lo, hi);
+    if (start != LX_KV_REFUSED) a.mask.range(start + a.per.over(row0 + min(row, n_rows - 1)), len, lo, hi);
   }
   template <typename T>
   __device__ __forceinline__ const T* query(const Args& a, int row) const {
-    const int x = row0 + min(row, n_rows - 1), t = x / a.per;
-    return static_cast<const T*>(a.q) + (e.row0 + t) * a.q_row + (head * a.per + (x - t * a.per)) * a.q_head;
+    const int x = row0 + min(row, n_rows - 1), t = a.per.over(x);
+    return static_cast<const T*>(a.q) + (e.row0 + t) * a.q_row + head_of(a, x, t) * a.q_head;
+  }
+  // query head of row x of the entry, which is its t-th query row
+  __device__ __forceinline__ int64_t head_of(const Args& a, int x, int t) const {
+    return head * static_cast<int>(a.per.d) + (x - t * static_cast<int>(a.per.d));
   }
 };
 
-// The ring through which THREADS threads bring the blocks of units unit, unit + STRIDE, ... below
-// the end into shared memory, STAGES - 1 units ahead.
-template <int BB, int STAGES, int STRIDE, int THREADS>
+// The ring through which a warp brings units first, first + STRIDE, ... below the end into shared memory, STAGES - 1
+// units ahead, by bulk copies of one lane.  (Copies of 16 bytes by every lane took 43 of 320 instructions a block and a
+// fifth of the time.)  Page ids are looked up for 32 blocks at once, a lane each, and 32 blocks ahead.
+template <int BB, int STAGES, int STRIDE>
 struct Ring {
   const int32_t* table;
   const uint8_t* base;  // of the layer and head, in page 0
   uint32_t page_bytes;  // from a page to the next, the same layer and head
-  int n_pages, block_lg, tid;
-  uint32_t smem;        // this ring's first stage
-  int next, n_blocks;   // next unit to load; blocks below this one exist
-  int page[2];          // of its blocks, looked up one unit ahead; -2: no such block
-  int first[STAGES - 1][2];  // the same of the first units, looked up at once
-  uint32_t got;         // two bits a loaded unit, the last in the lowest place: which blocks are there
+  uint32_t smem;        // the first stage
+  uint64_t* bars;       // [STAGES]
+  int* held;            // [STAGES] two bits: which blocks of the unit are there
   int* error;
+  int n_pages, block_lg, lane, first, count, n_blocks;  // blocks below n_blocks exist
+  int issued, stage;    // units issued; the next one's stage
+  int pages, ahead;     // this lane's page ids
+  uint32_t valid;
 
-  __device__ __forceinline__ void look_up(int unit, int (&page)[2]) const {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) page[b] = 2 * unit + b < n_blocks ? table[(2 * unit + b) >> block_lg] : -2;
+  __device__ __forceinline__ int look_up(int batch) const {
+    const int i = 16 * batch + lane / 2, block = 2 * (first + i * STRIDE) + lane % 2;
+    return i < count && block < n_blocks ? table[block >> block_lg] : -2;
   }
-  __device__ __forceinline__ void load(int stage) {
-    bring(stage, page);
-    look_up(next, page);
+  __device__ __forceinline__ void check() {
+    const bool ok = static_cast<uint32_t>(pages) < static_cast<uint32_t>(n_pages);
+    if (!ok && pages != -2) atomicOr(error, LX_KV_PAGE);
+    valid = __ballot_sync(0xffffffffu, ok);
   }
-  __device__ __forceinline__ void bring(int stage, const int (&page)[2]) {
-    got <<= 2;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if (static_cast<uint32_t>(page[b]) < static_cast<uint32_t>(n_pages)) {
-        got |= 1u << b;
-        const int in_page = (2 * next + b) & ((1 << block_lg) - 1);
-        const uint8_t* src = base + static_cast<uint64_t>(static_cast<uint32_t>(page[b])) * page_bytes +
-                             (in_page * BB + 16 * tid);
-        const uint32_t dst = smem + (2 * stage + b) * BB + 16 * tid;
-#pragma unroll
-        for (int x = 0; x < (BB / 16 + THREADS - 1) / THREADS; ++x)
-          if (BB / 16 >= THREADS * (x + 1) || tid + THREADS * x < BB / 16)
-            cp_async16(dst + 16 * THREADS * x, src + 16 * THREADS * x);
-      } else if (page[b] != -2 && tid == 0) {
-        atomicOr(error, LX_KV_PAGE);
-      }
-    }
-    cp_async_commit();
-    next += STRIDE;
-  }
-  __device__ __forceinline__ void start(const Args& a, const Share& s, int unit, int unit_end, int hi, uint8_t* stages,
-                                        int thread) {
+  __device__ __forceinline__ void set_up(const Args& a, const Share& s, int unit, int unit_end, int hi,
+                                         uint8_t* stages, uint64_t* barriers, int* flags) {
     table = a.c.table + static_cast<size_t>(s.e.slot < 0 ? 0 : s.e.slot) * a.c.max_pages;
     const uint32_t head_bytes = static_cast<uint32_t>(BB) << a.block_lg;
     page_bytes = head_bytes * a.c.kv_heads;
     base = static_cast<const uint8_t*>(a.c.pool) +
            (static_cast<uint64_t>(a.layer) * a.c.n_pages * a.c.kv_heads + s.head) * head_bytes;
+    smem = smem_u32(stages);
+    bars = barriers;
+    held = flags;
+    error = a.c.error;
     n_pages = a.c.n_pages;
     block_lg = a.block_lg;
-    tid = thread;
-    smem = smem_u32(stages);
-    next = unit;
+    lane = threadIdx.x % 32;
+    first = unit;
+    count = max(0, (unit_end - unit + STRIDE - 1) / STRIDE);
     n_blocks = min(2 * unit_end, (hi + BLOCK - 1) / BLOCK);
-    got = 0;
-    error = a.c.error;
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) look_up(unit + i * STRIDE, first[i]);
-    look_up(unit + (STAGES - 1) * STRIDE, page);
+    issued = stage = 0;
+    pages = look_up(0);
+    ahead = look_up(1);
+  }
+  // The whole warp.
+  __device__ __forceinline__ void issue() {
+    if (issued >= count) return;
+    const int k = issued % 16;
+    if (k == 0 && issued > 0) {
+      pages = ahead;
+      check();
+      ahead = look_up(issued / 16 + 1);
+    }
+    const int page0 = __shfl_sync(0xffffffffu, pages, 2 * k), page1 = __shfl_sync(0xffffffffu, pages, 2 * k + 1);
+    if (lane == 0) {
+      const uint32_t got = valid >> (2 * k) & 3u, dst = smem + stage * (2 * BB);
+      const int block = 2 * (first + issued * STRIDE), mask = (1 << block_lg) - 1;
+      const uint8_t* src = base + static_cast<uint64_t>(static_cast<uint32_t>(page0)) * page_bytes + (block & mask) * BB;
+      held[stage] = static_cast<int>(got);
+      mbar_arrive_expect_tx(&bars[stage], (got & 1u ? BB : 0) + (got & 2u ? BB : 0));
+      if (block_lg > 0 && got == 3u) {  // the two lie together
+        copy_bulk(dst, src, 2 * BB, &bars[stage]);
+      } else {
+        if (got & 1u) copy_bulk(dst, src, BB, &bars[stage]);
+        if (got & 2u)
+          copy_bulk(dst + BB,
+                    base + static_cast<uint64_t>(static_cast<uint32_t>(page1)) * page_bytes + ((block + 1) & mask) * BB, BB,
+                    &bars[stage]);
+      }
+    }
+    ++issued;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   __device__ __forceinline__ void fill() {
+    check();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) bring(i, first[i]);
+    for (int i = 0; i < STAGES - 1; ++i) issue();
   }
 };
 
 // The units [first, last) of this CTA for keys [lo, hi) of its rows.
-__device__ __forceinline__ void share_units(int lo, int hi, int rank, int split, int& first, int& last) {
+__device__ __forceinline__ void share_units(int lo, int hi, int rank, const Divisor& split, int& first, int& last) {
   first = last = 0;
   if (hi > lo) {
     const int u = lo / UNIT, count = (hi + UNIT - 1) / UNIT - u;
-    first = u + static_cast<int>(static_cast<long long>(count) * rank / split);
-    last = u + static_cast<int>(static_cast<long long>(count) * (rank + 1) / split);
+    first = u + split.over(count * rank);  // (count < 2^25, split <= 16)
+    last = u + split.over(count * (rank + 1));
   }
 }
 
@@ -328,7 +364,8 @@ __device__ __forceinline__ void join(const Args& a, const Share& s, float* part_
     return p;
   };
   auto write = [&](int row, int v, const Part& p) {
-    const int at = s.row0 + row, t = at / a.per, h = s.head * a.per + (at - t * a.per);
+    const int at = s.row0 + row, t = a.per.over(at);
+    const int64_t h = s.head_of(a, at, t);
     const float f = p.sum == 0.0f ? 0.0f : 1.0f / p.sum;
     put4(static_cast<T*>(a.out) + (s.e.row0 + t) * a.o_row + h * a.o_head + 4 * v, a.out_wide,
          make_float4(p.o.x * f, p.o.y * f, p.o.z * f, p.o.w * f));
@@ -385,7 +422,8 @@ struct FewShape {
   static constexpr int STAGES = DIM == 64 ? 4 : 3;
   static constexpr int RING = KW * STAGES * 2 * BB;
   static constexpr int JOIN = (KW + 1) * ROWS * (DIM + 2) * 4;
-  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+  static constexpr int BARS = (RING > JOIN ? RING : JOIN) + 15 & ~15;
+  static constexpr int SMEM = BARS + KW * STAGES * 12 + 16;
 };
 
 template <typename T, int DIM, int GROUP, int NT, int KW>
@@ -394,6 +432,13 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
   constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS);     // [KW][STAGES]
+  int* held = reinterpret_cast<int*>(bars + KW * S::STAGES);        // [KW][STAGES]
+  volatile int* abort_flag = held + KW * S::STAGES;
+  if (lane < S::STAGES) mbar_init(&bars[warp * S::STAGES + lane], 1);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  fence_mbar_init();
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
   Share s;
@@ -408,11 +453,11 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
 #pragma unroll
     for (int x = 0; x < 2; ++x) s.range(a, 8 * r + 2 * j + x, lo[r][x], hi[r][x]);
   int unit, unit_end;
-  share_units(lo_cta, hi_cta, s.rank, a.split, unit, unit_end);
+  share_units(lo_cta, hi_cta, s.rank, a.split_by, unit, unit_end);
   unit += warp;
-  Ring<BB, S::STAGES, KW, 32> ring;
+  Ring<BB, S::STAGES, KW> ring;
   uint8_t* stages = smem + warp * S::STAGES * 2 * BB;
-  ring.start(a, s, unit, unit_end, hi_cta, stages, lane);
+  ring.set_up(a, s, unit, unit_end, hi_cta, stages, bars + warp * S::STAGES, held + warp * S::STAGES);
 
   // the query: lane (n, j) holds channels 64 h + 32 w + 8 j + {0..7} of row 8 r + n
   uint32_t qb[NT][H][2][2][2];
@@ -492,58 +537,63 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
   }
 
   int stage = 0;
+  uint32_t phase = 0;
   const int slot = 16 * (n / 2) + 4 * (n % 2);  // bytes to the parameters of key n; those of n + 8 are 8 further
 #pragma unroll 1
   for (; unit < unit_end; unit += KW) {
-    cp_async_wait<S::STAGES - 2>();
-    __syncwarp();
-    ring.load(stage == 0 ? S::STAGES - 1 : stage - 1);
+    const bool come = mbar_wait(&ring.bars[stage], phase, nullptr, abort_flag, 0);
+    if (!__all_sync(0xffffffffu, come)) break;
+    ring.issue();  // into the stage of the unit before, which every lane is done with
     const uint8_t* data = stages + 2 * stage * BB;
-    const uint32_t got = ring.got >> (2 * (S::STAGES - 1)) & 3u;
-    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+    const uint32_t got = static_cast<uint32_t>(ring.held[stage]);
+    if (++stage == S::STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
     const int key0 = unit * UNIT;
 
     // PART: not every row sees every key of the unit (a body of its own, so that the others carry no selects)
     auto body = [&](auto tag) {
     constexpr bool PART = decltype(tag)::value;
-    // scores in log2 units, of (rows 2 j, 2 j + 1): s2[block][r][key n or n + 8]
+    // scores in log2 units, of (rows 2 j, 2 j + 1): s2[block][r][key n or n + 8].  (The products of the blocks and
+    // groups take turns: each waits for its own last one only.)
     float2 s2[2][NT][2];
+    float raw[2][G][NT][4];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const uint8_t* d = data + b * BB;
+    for (int q = 0; q < GROUP / 32; ++q)
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float raw[NT][4];
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int hw = g * GROUP / 32; hw < (g + 1) * GROUP / 32; ++hw) {
-          const uint4 k = lds128(d + 512 * (hw / 2) + 16 * lane);
-          const uint32_t k0 = hw % 2 ? k.y : k.x, k1 = hw % 2 ? k.w : k.z;
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const uint32_t x0 = k0 >> (8 * t), x1 = k1 >> (8 * t);
+          for (int b = 0; b < 2; ++b) {
+            const int hw = g * (GROUP / 32) + q;
+            const uint4 k = lds128(data + b * BB + 512 * (hw / 2) + 16 * lane);
+            const uint32_t x0 = (hw % 2 ? k.y : k.x) >> (8 * t), x1 = (hw % 2 ? k.w : k.z) >> (8 * t);
 #pragma unroll
             for (int r = 0; r < NT; ++r) {
               const uint32_t(&y)[2] = qb[r][hw / 2][hw % 2][t];
-              if (hw == g * GROUP / 32 && t == 0)
-                mma0(raw[r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
+              if (q == 0 && t == 0)
+                mma0(raw[b][g][r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
               else
-                mma(raw[r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
+                mma(raw[b][g][r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
             }
           }
-        }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint32_t p = lds32(d + param_offset(DIM) + 64 * g + slot + 8 * t);
+          const uint32_t p = lds32(data + b * BB + param_offset(DIM) + 64 * g + slot + 8 * t);
           const float ks = step_of(p) * c1, km = low_of(p);
 #pragma unroll
           for (int r = 0; r < NT; ++r) {
             float2& y = s2[b][r][t];
-            y.x = fmaf(raw[r][2 * t], ks, g == 0 ? qs[r][g].x * km : fmaf(qs[r][g].x, km, y.x));
-            y.y = fmaf(raw[r][2 * t + 1], ks, g == 0 ? qs[r][g].y * km : fmaf(qs[r][g].y, km, y.y));
+            y.x = fmaf(raw[b][g][r][2 * t], ks, g == 0 ? qs[r][g].x * km : fmaf(qs[r][g].x, km, y.x));
+            y.y = fmaf(raw[b][g][r][2 * t + 1], ks, g == 0 ? qs[r][g].y * km : fmaf(qs[r][g].y, km, y.y));
           }
         }
-      }
-    }
     // steps and centred minima of V
     float vs[2][G][2], vm[2][G][2];
 #pragma unroll
@@ -626,10 +676,9 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
       }
     }
     // p F, its sums, and O += (p F s) c
+    uint32_t pb[2][NT][G][2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const uint8_t* d = data + b * BB + 512 * H;
-      uint32_t pb[NT][G][2];
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < NT; ++r)
 #pragma unroll
@@ -647,13 +696,17 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
             }
             z[r][g].x = fmaf(p.x, low.x, z[r][g].x);
             z[r][g].y = fmaf(p.y, low.y, z[r][g].y);
-            pb[r][g][t] = transpose8(half_pair(w));
+            pb[b][r][g][t] = transpose8(half_pair(w));
           }
         }
 #pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const uint8_t* d = data + b * BB + 512 * H;
+#pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int r = 0; r < NT; ++r) mma(o8[r][g], EIGHTS, EIGHTS, EIGHTS, EIGHTS, pb[r][g][0], pb[r][g][1]);
+        for (int r = 0; r < NT; ++r)
+          mma(o8[r][g], EIGHTS, EIGHTS, EIGHTS, EIGHTS, pb[b][r][g][0], pb[b][r][g][1]);
 #pragma unroll
       for (int hw = 0; hw < 2 * H; ++hw) {
         const uint4 x = lds128(d + 512 * (hw / 2) + 16 * lane);
@@ -663,8 +716,8 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
           const uint32_t x0 = v0 >> (8 * i), x1 = v1 >> (8 * i);
 #pragma unroll
           for (int r = 0; r < NT; ++r)
-            mma(o[r][hw / 2][hw % 2][i], x0 & M0, x0 & M1, x1 & M0, x1 & M1, pb[r][32 * hw / GROUP][0],
-                pb[r][32 * hw / GROUP][1]);
+            mma(o[r][hw / 2][hw % 2][i], x0 & M0, x0 & M1, x1 & M0, x1 & M1, pb[b][r][32 * hw / GROUP][0],
+                pb[b][r][32 * hw / GROUP][1]);
         }
       }
     }
@@ -674,8 +727,8 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
     else
       body(std::false_type());
   }
-  cp_async_wait<0>();
   __syncthreads();  // every ring has been read: the joining takes their place
+  if (threadIdx.x == 0 && *abort_flag) flag(a.c, LX_KV_STUCK);
 
   float* part_o = reinterpret_cast<float*>(smem);  // [KW + 1][ROWS][DIM], the last one the CTA's
   float* part_m = part_o + (KW + 1) * S::ROWS * DIM;
@@ -730,7 +783,8 @@ struct ManyShape {
   static constexpr int STAGES = 4;
   static constexpr int RING = STAGES * 2 * BB;
   static constexpr int JOIN = ROWS * (DIM + 2) * 4;
-  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+  static constexpr int BARS = (RING > JOIN ? RING : JOIN) + 15 & ~15;
+  static constexpr int SMEM = BARS + STAGES * 12 + 16;
 };
 
 template <typename T, int DIM, int GROUP, int MT, int MW>
@@ -740,6 +794,13 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
   const int warp_row = 16 * MT * warp;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS);  // [STAGES]
+  int* held = reinterpret_cast<int*>(bars + S::STAGES);          // [STAGES]
+  volatile int* abort_flag = held + S::STAGES;
+  if (threadIdx.x < S::STAGES) mbar_init(&bars[threadIdx.x], 1);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  fence_mbar_init();
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
   Share s;
@@ -756,9 +817,9 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 #pragma unroll
     for (int u = 0; u < 2; ++u) s.range(a, warp_row + 16 * r + n + 8 * u, lo[r][u], hi[r][u]);
   int unit, unit_end;
-  share_units(lo_cta, hi_cta, s.rank, a.split, unit, unit_end);
-  Ring<BB, S::STAGES, 1, 32 * MW> ring;
-  ring.start(a, s, unit, unit_end, hi_cta, smem, threadIdx.x);
+  share_units(lo_cta, hi_cta, s.rank, a.split_by, unit, unit_end);
+  Ring<BB, S::STAGES, 1> ring;
+  if (warp == 0) ring.set_up(a, s, unit, unit_end, hi_cta, smem, bars, held);
 
   // the query: lane (n, j) holds channels 64 h + 32 w + 8 j + {0..7} of rows n and n + 8 of each 16
   uint32_t qa[MT][H][2][2][4];
@@ -774,7 +835,7 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 #pragma unroll
         for (int hw = 0; hw < 2 * H; ++hw) raw[r][u][hw / 2][hw % 2].load(p + 32 * hw, a.wide);
       }
-    ring.fill();
+    if (warp == 0) ring.fill();
     float x[MT][2][H][2][8], top = 0.0f;
 #pragma unroll
     for (int r = 0; r < MT; ++r)
@@ -847,14 +908,18 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
   }
 
   int stage = 0;
+  uint32_t phase = 0;
 #pragma unroll 1
   for (; unit < unit_end; ++unit) {
-    cp_async_wait<S::STAGES - 2>();
-    __syncthreads();
-    ring.load(stage == 0 ? S::STAGES - 1 : stage - 1);
+    const bool come = mbar_wait(&bars[stage], phase, nullptr, abort_flag, 0);
+    if (!__syncthreads_and(come)) break;
+    if (warp == 0) ring.issue();  // into the stage of the unit before, which every warp is done with
     const uint8_t* data = smem + 2 * stage * BB;
-    const uint32_t got = ring.got >> (2 * (S::STAGES - 1)) & 3u;
-    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+    const uint32_t got = static_cast<uint32_t>(held[stage]);
+    if (++stage == S::STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
 #pragma unroll 1
     for (int b = 0; b < 2; ++b) {
       const int key0 = unit * UNIT + 16 * b;
@@ -1029,8 +1094,8 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
         body(std::false_type());
     }
   }
-  cp_async_wait<0>();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) flag(a.c, LX_KV_STUCK);
 
   float* part_o = reinterpret_cast<float*>(smem);  // [ROWS][DIM]
   float* part_m = part_o + S::ROWS * DIM;
@@ -1051,7 +1116,8 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
         low[g] += __shfl_xor_sync(0xffffffffu, low[g], 2);
       }
       if (row >= s.n_rows) continue;
-      const int at = s.row0 + row, t = at / a.per, h = s.head * a.per + (at - t * a.per);
+      const int at = s.row0 + row, t = a.per.over(at);
+      const int64_t h = s.head_of(a, at, t);
       T* out = static_cast<T*>(a.out) + (s.e.row0 + t) * a.o_row + h * a.o_head + 8 * j;
       // without a split the row is whole: it is written from here
       const float f = a.split > 1 ? back : sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -1216,9 +1282,9 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
   Share s;
   bool any;
   {
-    const int per_tile = a.r.n * a.c.kv_heads, tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per_tile;
-    const int x = blockIdx.x % per_tile;
-    any = s.take_at(a, x / a.c.kv_heads, x % a.c.kv_heads, tile, TILE_ROWS);
+    const int block = static_cast<int>(blockIdx.x), back = a.items.over(block), x = block - back * static_cast<int>(a.items.d);
+    const int entry = a.heads.over(x);
+    any = s.take_at(a, entry, x - entry * a.c.kv_heads, static_cast<int>(a.tiles.d) - 1 - back, TILE_ROWS);
   }
   int lo_cta = 0, hi_cta = 0, x_;
   if (any) {
@@ -1586,7 +1652,8 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
     if (ok && live) {
       tc_fence_after();
       const float sum = l.x + l.y, f = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int r = s.row0 + row, q_row = r / a.per, h = s.head * a.per + (r - q_row * a.per);
+      const int r = s.row0 + row, q_row = a.per.over(r);
+      const int64_t h = s.head_of(a, r, q_row);
       T* out = static_cast<T*>(a.out) + (s.e.row0 + q_row) * a.o_row + h * a.o_head;
 #pragma unroll 1
       for (int c = 0; c < DIM / 32; ++c) {
@@ -1667,28 +1734,37 @@ void set_up(K kernel, Launch& l, int threads, int smem, cudaLaunchConfig_t& cfg,
   l.ready = l.active[1] > 0;
 }
 
-// Launches `items` (tiles of rows x kv heads) with the keys of each split over a
-// cluster: as finely as all items still run at once and each key group has a
-// unit (`groups` a CTA).  `halve`: where whole items take one to two rounds of the GPU, into halves, so
-// that the last ones leave less of it idle (64 x 8 items over 4099-8191 keys: 105 us against 116).
+// Launches `items` (tiles of rows x kv heads) with the keys of each split over a cluster of the size that
+// costs least: as many rounds of the GPU as it takes, of a fixed part and the units that a key group (`groups` a CTA)
+// then has.  The fixed part, in units: `whole` for a CTA of its own, `joined` for one of a cluster.  Few rows, 128
+// channels, 512 items, us a call: 32 keys 9 in two rounds, then 1.1 a unit a round; over 4099-8191 keys 116, 105, 114,
+// 119 for clusters of 1 to 4 (larger clusters fill the GPU less evenly: a thirtieth each).
 template <typename K>
 bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_rows, int groups, int units,
-           bool halve, cudaStream_t s) {
+           double whole, double joined, cudaStream_t s) {
   Launch& l = launches[a.c.device & 63];
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
   set_up(kernel, l, threads, smem, cfg, attr);
   if (!l.ready) return false;
-  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per + tile_rows - 1) / tile_rows;
+  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per.d + tile_rows - 1) / tile_rows;
   const long long items = tiles * a.r.n * a.c.kv_heads;
   const int most = min(16, (units + groups - 1) / groups);
   int split = 1;
-  for (int k = 2; k <= most; ++k)
-    if (l.active[k] >= items) split = k;
-  if (halve && split == 1 && items > l.active[1] / 2 && items < 2 * l.active[1] && most >= 8) split = 2;
+  double best = 0.0;
+  for (int k = 1; k <= most; ++k) {
+    if (l.active[k] == 0) continue;
+    const double rounds = static_cast<double>((items + l.active[k] - 1) / l.active[k]);
+    const double cost = rounds * ((k > 1 ? joined : whole) + (units + groups * k - 1) / (groups * k)) * (1 + (k - 1) / 30.0);
+    if (k == 1 || cost < best) {
+      best = cost;
+      split = k;
+    }
+  }
   if (items * split > 0x7fffffff) return false;
-  a.tiles = static_cast<int>(tiles);
+  a.tiles = Divisor(static_cast<uint32_t>(tiles));
   a.split = split;
+  a.split_by = Divisor(split);
   cfg.gridDim = dim3(static_cast<unsigned>(items * split));
   cfg.stream = s;
   attr[0].val.clusterDim.x = split;
@@ -1704,13 +1780,13 @@ template <typename T, int DIM, int GROUP, int NT, int KW>
 bool few(Args& a, int units, cudaStream_t s) {
   using S = FewShape<DIM, GROUP, NT, KW>;
   static Launch launches[64];
-  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, true, s);
+  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, 6.0, 7.0, s);
 }
 template <typename T, int DIM, int GROUP, int MT, int MW>
 bool many(Args& a, int units, cudaStream_t s) {
   using S = ManyShape<DIM, GROUP, MT, MW>;
   static Launch launches[64];
-  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 4, units, false, s);
+  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 1, units, 5.0, 15.0, s);
 }
 
 template <typename T, int DIM, int GROUP>
@@ -1727,17 +1803,17 @@ bool tile(Args& a, cudaStream_t s) {
       return false;
     done = true;
   }
-  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per + TILE_ROWS - 1) / TILE_ROWS;
+  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per.d + TILE_ROWS - 1) / TILE_ROWS;
   const long long ctas = tiles * a.r.n * a.c.kv_heads;
   if (ctas > 0x7fffffff) return false;
-  a.tiles = static_cast<int>(tiles);
+  a.tiles = Divisor(static_cast<uint32_t>(tiles));
   a.split = 1;
   return launch(kernel, dim3(static_cast<unsigned>(ctas)), dim3(S::THREADS), S::SMEM, s, a);
 }
 
 template <typename T, int DIM, int GROUP>
 bool go(Args& a, int max_len, cudaStream_t s) {
-  const long long rows = static_cast<long long>(a.r.max_rows) * a.per;
+  const long long rows = static_cast<long long>(a.r.max_rows) * a.per.d;
   const long long items = static_cast<long long>(a.r.n) * a.c.kv_heads;
   const int units = (max_len + UNIT - 1) / UNIT;
   if (rows <= 16) {
@@ -1769,7 +1845,10 @@ extern "C" int lx_kv_attention(const lx_kv_cache* c, int32_t layer, const lx_kv_
   if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4)) return LX_ERR_ARG;
   if (q_heads <= 0 || q_heads % c->kv_heads != 0 || q_heads > 65535) return LX_ERR_ARG;
   if (!std::isfinite(scale) || chunk < 0 || (chunk == 0 && left >= 0) || max_len < 0) return LX_ERR_ARG;
-  if (static_cast<long long>(rows->n) * rows->max_rows > 0x7fffffff) return LX_ERR_ARG;
+  if (static_cast<long long>(rows->n) * rows->max_rows > 0x7fffffff ||
+      static_cast<long long>(rows->n) * c->kv_heads > 0x7fffffff ||
+      static_cast<long long>(rows->max_rows) * (q_heads / c->kv_heads) > 0x7fffffff)
+    return LX_ERR_ARG;
   if (rows->max_rows == 0 || rows->total == 0) return LX_OK;
   OnDevice on(c->device);
   if (!on.ok()) return LX_ERR_CUDA;
@@ -1778,7 +1857,9 @@ extern "C" int lx_kv_attention(const lx_kv_cache* c, int32_t layer, const lx_kv_
   a.r = *rows;
   a.layer = layer;
   a.q_heads = q_heads;
-  a.per = q_heads / c->kv_heads;
+  a.per = Divisor(q_heads / c->kv_heads);
+  a.heads = Divisor(c->kv_heads);
+  a.items = Divisor(static_cast<uint32_t>(rows->n) * static_cast<uint32_t>(c->kv_heads));
   a.block_lg = c->page == 16 ? 0 : c->page == 32 ? 1 : c->page == 64 ? 2 : 3;
   a.q = q;
   a.q_row = q_row;
@@ -1790,7 +1871,9 @@ extern "C" int lx_kv_attention(const lx_kv_cache* c, int32_t layer, const lx_kv_
   a.o_head = o_head;
   a.lse = lse;
   a.scale = scale;
-  a.mask = Mask{chunk, left};
+  a.mask.chunk = chunk > 0 ? Divisor(chunk < MAX_TOKENS ? chunk : MAX_TOKENS) : Divisor();
+  if (chunk == 0) a.mask.chunk.d = 0;
+  a.mask.left = left;
   const int most = max_len > 0 && max_len < c->max_pages * c->page ? max_len : c->max_pages * c->page;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   bool ok = false;
