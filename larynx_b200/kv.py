@@ -43,21 +43,21 @@ class LxKvRows(ctypes.Structure):
 def _declare(lib):
     if getattr(lib, "_kv_declared", False):
         return lib
+    # (structures pass by their address: a typed pointer costs the interpreter more than the rest of a short call)
     vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
-    cache, rows = ctypes.POINTER(LxKvCache), ctypes.POINTER(LxKvRows)
     for name in ("lx_kv_pool_bytes", "lx_kv_scratch_ints"):
-        getattr(lib, name).argtypes = [cache]
+        getattr(lib, name).argtypes = [vp]
         getattr(lib, name).restype = ctypes.c_size_t
-    lib.lx_kv_reset.argtypes = [cache, vp]
-    lib.lx_kv_status.argtypes = [cache, ctypes.POINTER(i32), vp]
-    lib.lx_kv_extend.argtypes = [cache, i32, vp, vp, vp, vp]
+    lib.lx_kv_reset.argtypes = [vp, vp]
+    lib.lx_kv_status.argtypes = [vp, ctypes.POINTER(i32), vp]
+    lib.lx_kv_extend.argtypes = [vp, i32, vp, vp, vp, vp]
     for name in ("lx_kv_write", "lx_kv_read"):
-        getattr(lib, name).argtypes = [cache, i32, rows, i32, vp, i64, i64, vp, i64, i64, vp]
-    lib.lx_kv_attention.argtypes = [cache, i32, rows, i32, i32, vp, i64, i64, vp, i64, i64, vp, ctypes.c_float, i32,
-                                    i32, i32, vp]
+        getattr(lib, name).argtypes = [vp, i32, vp, i32, vp, i64, i64, vp, i64, i64, vp]
+    lib.lx_kv_attention.argtypes = [vp, i32, vp, i32, i32, vp, i64, i64, vp, i64, i64, vp, ctypes.c_float, i32, i32,
+                                    i32, vp]
     for name in ("lx_kv_fork", "lx_kv_copy", "lx_kv_free"):
-        getattr(lib, name).argtypes = [cache, i32, vp, vp, vp]
-    lib.lx_kv_compact.argtypes = [cache, vp, vp]
+        getattr(lib, name).argtypes = [vp, i32, vp, vp, vp]
+    lib.lx_kv_compact.argtypes = [vp, vp, vp]
     for name in KV_EXPORTS[2:]:
         getattr(lib, name).restype = ctypes.c_int
     lib._kv_declared = True
@@ -67,13 +67,13 @@ def _declare(lib):
 def pool_bytes(n_layers: int, n_pages: int, kv_heads: int, head_dim: int, group: int, page: int) -> int:
     """Bytes of the pool of a cache of this geometry (0 when it is not valid)."""
     c = LxKvCache(0, n_layers, n_pages, 1, 1, kv_heads, head_dim, group, page)
-    return int(_declare(load_library()).lx_kv_pool_bytes(ctypes.byref(c)))
+    return int(_declare(load_library()).lx_kv_pool_bytes(ctypes.addressof(c)))
 
 
 def scratch_ints(n_pages: int, n_seq: int, max_pages: int) -> int:
     """32-bit words of scratch that a cache needs (0 when the sizes are not valid)."""
     c = LxKvCache(0, 1, n_pages, n_seq, max_pages, 1, 64, 64, 16)
-    return int(_declare(load_library()).lx_kv_scratch_ints(ctypes.byref(c)))
+    return int(_declare(load_library()).lx_kv_scratch_ints(ctypes.addressof(c)))
 
 
 class KVCache:
@@ -83,17 +83,22 @@ class KVCache:
     def __init__(self, n_layers: int, n_pages: int, n_seq: int, max_pages: int, kv_heads: int, head_dim: int,
                  group: int, page: int, pool_ptr: int, table_ptr: int, lengths_ptr: int, refs_ptr: int,
                  scratch_ptr: int, error_ptr: int, device: int = 0):
-        self._lib = _declare(load_library())
+        lib = self._lib = _declare(load_library())
         self._c = LxKvCache(device, n_layers, n_pages, n_seq, max_pages, kv_heads, head_dim, group, page, pool_ptr,
                             table_ptr, lengths_ptr, refs_ptr, scratch_ptr, error_ptr)
-        self._ref = ctypes.byref(self._c)
-        if not self._lib.lx_kv_pool_bytes(self._ref):
+        self._at = ctypes.addressof(self._c)
+        if not lib.lx_kv_pool_bytes(self._at):
             raise KVError("KVCache: geometry not supported (head_dim 64 or 128, group 32 or 64, page 16, 32, 64 or "
                           "128, counts positive)")
+        self._dim, self._row = head_dim, kv_heads * head_dim
+        self._extend, self._write, self._read, self._attention = (lib.lx_kv_extend, lib.lx_kv_write, lib.lx_kv_read,
+                                                                  lib.lx_kv_attention)
+        self._fork, self._copy, self._free, self._compact = (lib.lx_kv_fork, lib.lx_kv_copy, lib.lx_kv_free,
+                                                             lib.lx_kv_compact)
 
-    def _check(self, rc: int, what: str) -> None:
-        if rc != LX_OK:
-            raise KVError(f"lx_kv_{what} failed: {ERRORS.get(rc, rc)}")
+    @staticmethod
+    def _fail(rc: int, what: str) -> None:
+        raise KVError(f"lx_kv_{what} failed: {ERRORS.get(rc, rc)}")
 
     @staticmethod
     def rows(n: int, total: int, max_rows: int, seqs: int = 0, row0: int = 0, start: int = 0) -> LxKvRows:
@@ -102,58 +107,74 @@ class KVCache:
 
     def reset(self, stream: int = 0) -> None:
         """Empty the cache (lengths, tables, refs, error; not the pool)."""
-        self._check(self._lib.lx_kv_reset(self._ref, stream or None), "reset")
+        rc = self._lib.lx_kv_reset(self._at, stream)
+        if rc != LX_OK:
+            self._fail(rc, "reset")
 
     def status(self, stream: int = 0) -> int:
         """Wait for the stream; the error bits since the last call (FULL, SLOT, WIDTH, PAGE, ROWS, STUCK)."""
         bits = ctypes.c_int32(0)
-        self._check(self._lib.lx_kv_status(self._ref, ctypes.byref(bits), stream or None), "status")
+        rc = self._lib.lx_kv_status(self._at, ctypes.byref(bits), stream)
+        if rc != LX_OK:
+            self._fail(rc, "status")
         return bits.value
 
     def extend(self, n: int, seqs_ptr: int, counts_ptr: int, start_ptr: int, stream: int = 0) -> None:
         """Grow sequences; start gets their old lengths, REFUSED where the pool did not suffice."""
-        self._check(self._lib.lx_kv_extend(self._ref, n, seqs_ptr, counts_ptr, start_ptr, stream or None), "extend")
-
-    def _strides(self, strides):
-        return (self._c.kv_heads * self._c.head_dim, self._c.head_dim) if strides is None else strides
+        rc = self._extend(self._at, n, seqs_ptr, counts_ptr, start_ptr, stream)
+        if rc != LX_OK:
+            self._fail(rc, "extend")
 
     def write(self, layer: int, rows: LxKvRows, dtype: str, k_ptr: int, v_ptr: int, k_strides=None, v_strides=None,
               stream: int = 0) -> None:
         """Quantise rows [total, kv_heads, head_dim] into a layer; strides are (row, head) in elements."""
-        ks, vs = self._strides(k_strides), self._strides(v_strides)
-        self._check(self._lib.lx_kv_write(self._ref, layer, ctypes.byref(rows), DTYPES[dtype], k_ptr, ks[0], ks[1],
-                                          v_ptr, vs[0], vs[1], stream or None), "write")
+        kr, kh = k_strides or (self._row, self._dim)
+        vr, vh = v_strides or (self._row, self._dim)
+        rc = self._write(self._at, layer, ctypes.addressof(rows), DTYPES[dtype], k_ptr, kr, kh, v_ptr, vr, vh, stream)
+        if rc != LX_OK:
+            self._fail(rc, "write")
 
     def read(self, layer: int, rows: LxKvRows, dtype: str, k_ptr: int, v_ptr: int, k_strides=None, v_strides=None,
              stream: int = 0) -> None:
         """The values of rows of a layer, into [total, kv_heads, head_dim]."""
-        ks, vs = self._strides(k_strides), self._strides(v_strides)
-        self._check(self._lib.lx_kv_read(self._ref, layer, ctypes.byref(rows), DTYPES[dtype], k_ptr, ks[0], ks[1],
-                                         v_ptr, vs[0], vs[1], stream or None), "read")
+        kr, kh = k_strides or (self._row, self._dim)
+        vr, vh = v_strides or (self._row, self._dim)
+        rc = self._read(self._at, layer, ctypes.addressof(rows), DTYPES[dtype], k_ptr, kr, kh, v_ptr, vr, vh, stream)
+        if rc != LX_OK:
+            self._fail(rc, "read")
 
     def attention(self, layer: int, rows: LxKvRows, q_heads: int, dtype: str, q_ptr: int, out_ptr: int, lse: int = 0,
                   scale: float = 0.125, chunk: int = 0, left: int = -1, max_len: int = 0, q_strides=None,
                   out_strides=None, stream: int = 0) -> None:
         """Attention of rows [total, q_heads, head_dim] over a layer; chunk 0 = full, 1 = causal, n = block-causal."""
-        d = self._c.head_dim
-        qs = (q_heads * d, d) if q_strides is None else q_strides
-        os = (q_heads * d, d) if out_strides is None else out_strides
-        self._check(self._lib.lx_kv_attention(self._ref, layer, ctypes.byref(rows), q_heads, DTYPES[dtype], q_ptr,
-                                              qs[0], qs[1], out_ptr, os[0], os[1], lse or None, scale, chunk, left,
-                                              max_len, stream or None), "attention")
+        d = self._dim
+        qr, qh = q_strides or (q_heads * d, d)
+        orow, oh = out_strides or (q_heads * d, d)
+        rc = self._attention(self._at, layer, ctypes.addressof(rows), q_heads, DTYPES[dtype], q_ptr, qr, qh, out_ptr, orow,
+                             oh, lse, scale, chunk, left, max_len, stream)
+        if rc != LX_OK:
+            self._fail(rc, "attention")
 
     def fork(self, n: int, src_ptr: int, dst_ptr: int, stream: int = 0) -> None:
         """dst[i] (empty) shares the pages of src[i]."""
-        self._check(self._lib.lx_kv_fork(self._ref, n, src_ptr, dst_ptr, stream or None), "fork")
+        rc = self._fork(self._at, n, src_ptr, dst_ptr, stream)
+        if rc != LX_OK:
+            self._fail(rc, "fork")
 
     def copy(self, n: int, src_ptr: int, dst_ptr: int, stream: int = 0) -> None:
         """dst[i] (empty) becomes a copy of src[i] on fresh pages."""
-        self._check(self._lib.lx_kv_copy(self._ref, n, src_ptr, dst_ptr, stream or None), "copy")
+        rc = self._copy(self._at, n, src_ptr, dst_ptr, stream)
+        if rc != LX_OK:
+            self._fail(rc, "copy")
 
     def free(self, n: int, seqs_ptr: int, keep_ptr: int, stream: int = 0) -> None:
         """Cut sequences to their first keep[i] tokens."""
-        self._check(self._lib.lx_kv_free(self._ref, n, seqs_ptr, keep_ptr, stream or None), "free")
+        rc = self._free(self._at, n, seqs_ptr, keep_ptr, stream)
+        if rc != LX_OK:
+            self._fail(rc, "free")
 
     def compact(self, used_ptr: int, stream: int = 0) -> None:
         """Move the used pages to the lowest ids; used gets their count."""
-        self._check(self._lib.lx_kv_compact(self._ref, used_ptr, stream or None), "compact")
+        rc = self._compact(self._at, used_ptr, stream)
+        if rc != LX_OK:
+            self._fail(rc, "compact")
