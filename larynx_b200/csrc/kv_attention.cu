@@ -27,7 +27,9 @@
 // bulk copies, two blocks a stage.
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <cmath>
+#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
@@ -139,10 +141,13 @@ __device__ __forceinline__ int step_exponent(float v) {
   return static_cast<int>(bits >> 23) - 127;
 }
 
+constexpr int LONGEST_FIRST = 128;  // entries that a block puts in order
+
 struct Args {
   lx_kv_cache c;
   lx_kv_rows r;
   int layer, q_heads, split, block_lg;  // block_lg: log2 of the blocks of a page
+  bool longest_first;                   // few rows: entries in the order of their lengths
   Divisor per, heads, tiles, split_by, items;  // query heads a kv head, kv heads, tiles of rows, split, n x kv heads
   const void* q;
   int64_t q_row, q_head;
@@ -187,11 +192,35 @@ struct Share {
   Entry e;
   int head, row0, n_rows, rows, len, start, rank;
   // the rows of the CTA are rows row0 .. row0 + n_rows - 1 of the entry's (query row, query head) pairs
-  __device__ __forceinline__ bool take(const Args& a, int tile_rows) {
+  __device__ __forceinline__ bool take(const Args& a, int tile_rows, int* lengths = nullptr, int threads = 0) {
     const int block = static_cast<int>(blockIdx.x), item = a.split_by.over(block), x = a.heads.over(item);
-    const int entry = a.tiles.over(x);
+    const int place = a.tiles.over(x), tile = x - place * static_cast<int>(a.tiles.d);
     rank = block - item * a.split;
-    return take_at(a, entry, item - x * a.c.kv_heads, x - entry * static_cast<int>(a.tiles.d), tile_rows);
+    const int entry = lengths && a.longest_first ? by_length(a, place, lengths, threads) : place;
+    return take_at(a, entry, item - x * a.c.kv_heads, tile, tile_rows);
+  }
+  // The entry whose place among all of them, longest first, is `place`.  (Equal ones in their order: a place each.)
+  static __device__ __forceinline__ int by_length(const Args& a, int place, int* lengths, int threads) {
+    const int n = a.r.n;
+    for (int i = threadIdx.x; i < (n + 3 & ~3); i += threads) {
+      const int slot = i >= n ? -1 : a.r.seqs ? a.r.seqs[i] : i;
+      lengths[i] = slot >= 0 && slot < a.c.n_seq ? length_of(a.c, slot) : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += threads) {
+      const int mine = lengths[i];
+      int before = 0;
+      for (int k = 0; k < n; k += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(lengths + k);  // (behind the last one: -1, at places >= i)
+        before += x.x >= mine + (k >= i);
+        before += x.y >= mine + (k + 1 >= i);
+        before += x.z >= mine + (k + 2 >= i);
+        before += x.w >= mine + (k + 3 >= i);
+      }
+      if (before == place) lengths[LONGEST_FIRST] = i;
+    }
+    __syncthreads();
+    return lengths[LONGEST_FIRST];
   }
   __device__ __forceinline__ bool take_at(const Args& a, int entry, int kv_head, int tile, int tile_rows) {
     head = kv_head;
@@ -304,6 +333,14 @@ struct Ring {
     }
     ++issued;
     stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  // The copies still on their way after a wait has given up, `taken` units having come.  (Again with a limit.)
+  __device__ __forceinline__ void drain(int taken) const {
+    held[0] = 0;  // (no longer needed: the flag of these waits)
+    __syncwarp();
+#pragma unroll 1
+    for (int i = taken; i < issued; ++i)
+      mbar_wait(&bars[i % STAGES], static_cast<uint32_t>(i / STAGES & 1), nullptr, held, 0);
   }
   __device__ __forceinline__ void fill() {
     check();
@@ -423,7 +460,8 @@ struct FewShape {
   static constexpr int RING = KW * STAGES * 2 * BB;
   static constexpr int JOIN = (KW + 1) * ROWS * (DIM + 2) * 4;
   static constexpr int BARS = (RING > JOIN ? RING : JOIN) + 15 & ~15;
-  static constexpr int SMEM = BARS + KW * STAGES * 12 + 16;
+  static constexpr int ORDER = BARS + KW * STAGES * 12 + 4 + 15 & ~15;  // lengths of the entries, and the place found
+  static constexpr int SMEM = ORDER + LONGEST_FIRST * 4 + 16;
 };
 
 template <typename T, int DIM, int GROUP, int NT, int KW>
@@ -442,7 +480,15 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
   pdl_wait();
   pdl_launch_dependents();
   Share s;
-  if (!s.take(a, S::ROWS)) return;
+  if (!s.take(a, S::ROWS, reinterpret_cast<int*>(smem + S::ORDER), S::THREADS)) {
+    // (Were the lengths written meanwhile, against the rules, the CTAs of a cluster may hold different entries: even
+    // then none leaves while another may read its part.)
+    if (a.longest_first && a.split > 1) {
+      cg::this_cluster().sync();
+      cg::this_cluster().sync();
+    }
+    return;
+  }
 
   // keys seen by this lane's rows 8 r + 2 j + x, and by every row
   int lo[NT][2], hi[NT][2], lo_all, hi_all, lo_cta, hi_cta;
@@ -727,6 +773,7 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
     else
       body(std::false_type());
   }
+  if (unit < unit_end) ring.drain((unit - ring.first) / KW);
   __syncthreads();  // every ring has been read: the joining takes their place
   if (threadIdx.x == 0 && *abort_flag) flag(a.c, LX_KV_STUCK);
 
@@ -1094,6 +1141,7 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
         body(std::false_type());
     }
   }
+  if (unit < unit_end && warp == 0) ring.drain(unit - ring.first);
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag) flag(a.c, LX_KV_STUCK);
 
@@ -1703,7 +1751,8 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
 // ---------------------------------------------------------------------------
 // What a kernel needs to be launched on one device: set up at its first call.
 struct Launch {
-  bool ready = false;
+  std::mutex lock;
+  std::atomic<bool> ready{false};
   int active[17];  // clusters of 1 .. 16 CTAs that the GPU holds at once
 };
 
@@ -1717,7 +1766,9 @@ void set_up(K kernel, Launch& l, int threads, int smem, cudaLaunchConfig_t& cfg,
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
-  if (l.ready) return;
+  if (l.ready.load(std::memory_order_acquire)) return;
+  std::lock_guard<std::mutex> one(l.lock);
+  if (l.ready.load(std::memory_order_relaxed)) return;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
       cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
     return;
@@ -1731,7 +1782,7 @@ void set_up(K kernel, Launch& l, int threads, int smem, cudaLaunchConfig_t& cfg,
       cudaGetLastError();
     }
   }
-  l.ready = l.active[1] > 0;
+  l.ready.store(l.active[1] > 0, std::memory_order_release);
 }
 
 // Launches `items` (tiles of rows x kv heads) with the keys of each split over a cluster of the size that
@@ -1765,6 +1816,7 @@ bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_
   a.tiles = Divisor(static_cast<uint32_t>(tiles));
   a.split = split;
   a.split_by = Divisor(split);
+  a.longest_first = a.r.n > 1 && a.r.n <= LONGEST_FIRST && items > l.active[split];
   cfg.gridDim = dim3(static_cast<unsigned>(items * split));
   cfg.stream = s;
   attr[0].val.clusterDim.x = split;
@@ -1792,9 +1844,9 @@ bool many(Args& a, int units, cudaStream_t s) {
 template <typename T, int DIM, int GROUP>
 bool tile(Args& a, cudaStream_t s) {
   using S = TileShape<DIM, GROUP>;
-  static bool ready[64] = {false};
+  static std::atomic<bool> ready[64];
   auto kernel = k_kv_tile<T, DIM, GROUP>;
-  bool& done = ready[a.c.device & 63];
+  std::atomic<bool>& done = ready[a.c.device & 63];
   if (!done) {
     // setmaxnreg.inc waits for registers that the block was launched with: no launch unless they cover the split
     cudaFuncAttributes fa;

@@ -6,8 +6,9 @@ Attention's bound, per output:
   * the probabilities' rounding to fp16.  A value is held as v = s c + m = s (c - 8) + (m + 8 s), and its first
     part is multiplied by fp16(p s): off by 2^-11 p s |c - 8| <= 2^-11 p 8 s a key, so by 2^-11 of the weighted sum
     of 8 s (not of |v|, which is smaller where s (c - 8) and m + 8 s have opposite signs).  Below the fp16 range
-    p s is off by 2^-25 absolute, where the largest step seen is scaled to over 2^10: 2^-35 of it a key, times
-    |c - 8| <= 8, over a denominator of at least 1: 2^-32 of the keys times the largest step;
+    p s is off by at most 2^-25 absolute, where the largest step seen is scaled to over 2^6: 2^-31 of it a key, times
+    |c - 8| <= 8, over a denominator of at least 1 (the score that set the running maximum has p = 1): 2^-28 of the
+    keys times the largest step;
   * the scores' error: a score is a sum in fp32 of at most 2 * 128 terms, each off by at most a few 2^-24, so it
     is off by at most dS = 2^-16 (256 * 2^-24) times the sum of |q| |k| scale, and 2^-18 for the exponential's own
     error; weights then move by at most 2 dS relative, and the output by that of the weighted sum of |v| + 8 s
@@ -116,7 +117,7 @@ def check(out, lse, want, dtype):
     ref, rl, size, weight, coarse, most = want
     out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
     ds = 2.0 ** -16 * size + 2.0 ** -18
-    tol = HALF[dtype] * np.abs(ref) + 2.0 ** -11 * coarse + 2.0 ** -32 * most + 2 * ds[..., None] * (weight + coarse)
+    tol = HALF[dtype] * np.abs(ref) + 2.0 ** -11 * coarse + 2.0 ** -28 * most + 2 * ds[..., None] * (weight + coarse)
     bad = np.abs(out - ref) > tol
     assert np.isfinite(out).all() and not bad.any(), (np.argwhere(bad)[:4], np.abs(out - ref).max())
     none = np.isinf(rl)
@@ -385,6 +386,40 @@ def test_attention_many_entries(dim, group, page, chunk, left, dtype):
         elif len(pos):
             check(o, l, ko.attention(qq.double().numpy(), k, v, st, pos, -0.2, chunk, left, seen=seen), dtype)
         at += m
+
+
+@pytest.mark.parametrize("dim,group,heads,per,count", [(64, 64, 8, 1, 128), (64, 32, 13, 2, 101), (128, 64, 8, 4, 127),
+                                                     (128, 32, 9, 12, 70), (64, 64, 8, 3, 129)])
+def test_attention_more_items_than_fit(dim, group, heads, per, count):
+    """More blocks than the GPU holds at once (entries are then taken longest first): lengths of every kind, equal ones,
+    none, slots in another order, the same slot twice, one that does not exist, entries without rows."""
+    rng = np.random.default_rng(count)
+    lengths = rng.integers(0, 200, count).tolist()
+    lengths[3:40] = [33] * 37
+    lengths[50] = lengths[51] = 0
+    lengths[60] = 700
+    c = Cache(n_pages=sum(-(-n // 16) for n in lengths), n_seq=count, max_pages=44, heads=heads, dim=dim, group=group)
+    held = c.fill(lengths, seed=count)
+    seqs = rng.permutation(count).tolist()
+    seqs[5] = seqs[6]
+    seqs[7] = count
+    counts = rng.integers(0, 2, count).tolist()
+    counts[7] = 1
+    counts[seqs.index(60)] = 1
+    g = torch.Generator().manual_seed(count)
+    q = torch.randn(sum(counts), heads * per, dim, generator=g).to(torch.bfloat16)
+    for max_len in (0, 700):
+        out, lse = c.attend(q.cuda(), c.batch(counts, seqs=seqs, max_rows=1), "bf16", scale=dim ** -0.5, chunk=1, max_len=max_len)
+        assert c.c.status() == c.kv.SLOT
+        at = 0
+        for slot, n in zip(seqs, counts):
+            if n and slot == count:
+                assert (out[at] == 0).all() and torch.isneginf(lse[at]).all()
+            elif n:
+                k, v, st = held[slot]
+                want = ko.attention(q[at:at + 1].double().numpy(), k, v, st, [len(k) - 1], dim ** -0.5, 1, -1)
+                check(out[at:at + 1], lse[at:at + 1], want, "bf16")
+            at += n
 
 
 @pytest.mark.parametrize("length", [1, 15, 16, 255, 1025, 4099])
