@@ -147,7 +147,7 @@ struct Args {
   lx_kv_cache c;
   lx_kv_rows r;
   int layer, q_heads, split, block_lg;  // block_lg: log2 of the blocks of a page
-  bool longest_first;                   // few rows: entries in the order of their lengths
+  bool longest_first;                   // entries in the order of their lengths
   Divisor per, heads, tiles, split_by, items;  // query heads a kv head, kv heads, tiles of rows, split, n x kv heads
   const void* q;
   int64_t q_row, q_head;
@@ -192,12 +192,19 @@ struct Share {
   Entry e;
   int head, row0, n_rows, rows, len, start, rank;
   // the rows of the CTA are rows row0 .. row0 + n_rows - 1 of the entry's (query row, query head) pairs
-  __device__ __forceinline__ bool take(const Args& a, int tile_rows, int* lengths = nullptr, int threads = 0) {
+  __device__ __forceinline__ bool take(const Args& a, int tile_rows, int* lengths, int threads) {
     const int block = static_cast<int>(blockIdx.x), item = a.split_by.over(block), x = a.heads.over(item);
     const int place = a.tiles.over(x), tile = x - place * static_cast<int>(a.tiles.d);
     rank = block - item * a.split;
-    const int entry = lengths && a.longest_first ? by_length(a, place, lengths, threads) : place;
-    return take_at(a, entry, item - x * a.c.kv_heads, tile, tile_rows);
+    const int entry = a.longest_first ? by_length(a, place, lengths, threads) : place;
+    const bool any = take_at(a, entry, item - x * a.c.kv_heads, tile, tile_rows);
+    // (Were the lengths written meanwhile, against the rules, the CTAs of a cluster may hold different entries: even
+    // then none leaves while another may read its part.)
+    if (!any && a.longest_first && a.split > 1) {
+      cg::this_cluster().sync();
+      cg::this_cluster().sync();
+    }
+    return any;
   }
   // The entry whose place among all of them, longest first, is `place`.  (Equal ones in their order: a place each.)
   static __device__ __forceinline__ int by_length(const Args& a, int place, int* lengths, int threads) {
@@ -480,15 +487,7 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
   pdl_wait();
   pdl_launch_dependents();
   Share s;
-  if (!s.take(a, S::ROWS, reinterpret_cast<int*>(smem + S::ORDER), S::THREADS)) {
-    // (Were the lengths written meanwhile, against the rules, the CTAs of a cluster may hold different entries: even
-    // then none leaves while another may read its part.)
-    if (a.longest_first && a.split > 1) {
-      cg::this_cluster().sync();
-      cg::this_cluster().sync();
-    }
-    return;
-  }
+  if (!s.take(a, S::ROWS, reinterpret_cast<int*>(smem + S::ORDER), S::THREADS)) return;
 
   // keys seen by this lane's rows 8 r + 2 j + x, and by every row
   int lo[NT][2], hi[NT][2], lo_all, hi_all, lo_cta, hi_cta;
@@ -831,7 +830,8 @@ struct ManyShape {
   static constexpr int RING = STAGES * 2 * BB;
   static constexpr int JOIN = ROWS * (DIM + 2) * 4;
   static constexpr int BARS = (RING > JOIN ? RING : JOIN) + 15 & ~15;
-  static constexpr int SMEM = BARS + STAGES * 12 + 16;
+  static constexpr int ORDER = BARS + STAGES * 12 + 4 + 15 & ~15;
+  static constexpr int SMEM = ORDER + LONGEST_FIRST * 4 + 16;
 };
 
 template <typename T, int DIM, int GROUP, int MT, int MW>
@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
   pdl_wait();
   pdl_launch_dependents();
   Share s;
-  if (!s.take(a, S::ROWS)) return;
+  if (!s.take(a, S::ROWS, reinterpret_cast<int*>(smem + S::ORDER), S::THREADS)) return;
 
   // keys seen by this lane's rows warp_row + 16 r + n + 8 u; by every row of the warp; by one of the warp, the CTA
   int lo[MT][2], hi[MT][2], lo_all, hi_all, lo_warp, hi_warp, lo_cta, hi_cta, x_;

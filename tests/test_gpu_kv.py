@@ -389,7 +389,8 @@ def test_attention_many_entries(dim, group, page, chunk, left, dtype):
 
 
 @pytest.mark.parametrize("dim,group,heads,per,count", [(64, 64, 8, 1, 128), (64, 32, 13, 2, 101), (128, 64, 8, 4, 127),
-                                                     (128, 32, 9, 12, 70), (64, 64, 8, 3, 129)])
+                                                     (128, 32, 9, 12, 70), (64, 64, 8, 3, 129),
+                                                     (64, 64, 9, 40, 80), (128, 32, 8, 33, 61)])
 def test_attention_more_items_than_fit(dim, group, heads, per, count):
     """More blocks than the GPU holds at once (entries are then taken longest first): lengths of every kind, equal ones,
     none, slots in another order, the same slot twice, one that does not exist, entries without rows."""
