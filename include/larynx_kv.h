@@ -100,7 +100,7 @@ typedef struct lx_kv_cache {
 
 /* The rows of a batch: entry i has rows row0[i] .. row0[i + 1] - 1 of the
  * caller's packed arrays, for positions start[i] + 0, 1, ... of slot seqs[i].
- * Device arrays; `total` counts all packed rows and max_rows is at least the
+ * Device arrays, n at least 1; `total` counts all packed rows and max_rows is at least the
  * most rows of one entry (rows past either are not touched). */
 typedef struct lx_kv_rows {
   int32_t n, total, max_rows;
@@ -125,8 +125,8 @@ int lx_kv_status(const lx_kv_cache* c, int32_t* bits, void* stream);
  * its old length.  New pages are the free ones of lowest id, given out in the
  * order of the batch; a last page that is not full and shared with another
  * sequence is replaced by a copy first (all layers), so that lx_kv_write never
- * changes a fork.  Entry i is served if the pages needed by entries 0 .. i fit the free ones; an entry that
- * is not served gets start[i] = LX_KV_REFUSED (its rows are skipped by the
+ * changes a fork.  Entry i is served if the pages needed by entries 0 .. i fit
+ * the free ones; an entry that is not served gets start[i] = LX_KV_REFUSED (its rows are skipped by the
  * other calls) and leaves its sequence as it was. */
 int lx_kv_extend(const lx_kv_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, int32_t* start,
                  void* stream);
@@ -152,9 +152,12 @@ int lx_kv_read(const lx_kv_cache* c, int32_t layer, const lx_kv_rows* rows, int3
  *   chunk  > 0: hi = min(length, (floor(p / chunk) + 1) chunk), and with
  *   left >= 0   lo = max(0, floor(p / chunk) chunk - left), else lo = 0
  * (chunk 1 is causal; left < 0 looks back without limit).  A row that sees
- * nothing gets zeros and lse = -inf; so do the rows of refused entries.  Keys on a page that is not in the pool are not seen (LX_KV_PAGE).
+ * nothing gets zeros and lse = -inf; so do the rows of refused entries.  Keys on
+ * a page that is not in the pool are not seen (LX_KV_PAGE).
  * max_len: an upper bound of the lengths, which only steers how the work is
- * split; 0 = max_pages * page.  The result does not depend on other entries. */
+ * split; 0 = max_pages * page.  No entry's values enter another's result (the
+ * order of its sums, so its last bits, follows from n, max_rows and max_len;
+ * the same call gives the same bits). */
 int lx_kv_attention(const lx_kv_cache* c, int32_t layer, const lx_kv_rows* rows, int32_t q_heads, int32_t dtype,
                     const void* q, int64_t q_row, int64_t q_head, void* out, int64_t o_row, int64_t o_head,
                     float* lse, float scale, int32_t chunk, int32_t left, int32_t max_len, void* stream);

@@ -472,7 +472,8 @@ struct FewShape {
 };
 
 template <typename T, int DIM, int GROUP, int NT, int KW>
-__global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / KW - (NT - 1)) k_kv_few(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / KW - (NT - 1))
+    k_kv_few(const __grid_constant__ Args a) {
   using S = FewShape<DIM, GROUP, NT, KW>;
   constexpr int H = DIM / 64, G = DIM / GROUP, BB = S::BB;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -599,173 +600,173 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
 
     // PART: not every row sees every key of the unit (a body of its own, so that the others carry no selects)
     auto body = [&](auto tag) {
-    constexpr bool PART = decltype(tag)::value;
-    // scores in log2 units, of (rows 2 j, 2 j + 1): s2[block][r][key n or n + 8].  (The products of the blocks and
-    // groups take turns: each waits for its own last one only.)
-    float2 s2[2][NT][2];
-    float raw[2][G][NT][4];
+      constexpr bool PART = decltype(tag)::value;
+      // scores in log2 units, of (rows 2 j, 2 j + 1): s2[block][r][key n or n + 8].  (The products of the blocks and
+      // groups take turns: each waits for its own last one only.)
+      float2 s2[2][NT][2];
+      float raw[2][G][NT][4];
 #pragma unroll
-    for (int q = 0; q < GROUP / 32; ++q)
+      for (int q = 0; q < GROUP / 32; ++q)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+          for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int hw = g * (GROUP / 32) + q;
-            const uint4 k = lds128(data + b * BB + 512 * (hw / 2) + 16 * lane);
-            const uint32_t x0 = (hw % 2 ? k.y : k.x) >> (8 * t), x1 = (hw % 2 ? k.w : k.z) >> (8 * t);
+            for (int b = 0; b < 2; ++b) {
+              const int hw = g * (GROUP / 32) + q;
+              const uint4 k = lds128(data + b * BB + 512 * (hw / 2) + 16 * lane);
+              const uint32_t x0 = (hw % 2 ? k.y : k.x) >> (8 * t), x1 = (hw % 2 ? k.w : k.z) >> (8 * t);
 #pragma unroll
-            for (int r = 0; r < NT; ++r) {
-              const uint32_t(&y)[2] = qb[r][hw / 2][hw % 2][t];
-              if (q == 0 && t == 0)
-                mma0(raw[b][g][r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
-              else
-                mma(raw[b][g][r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
+              for (int r = 0; r < NT; ++r) {
+                const uint32_t(&y)[2] = qb[r][hw / 2][hw % 2][t];
+                if (q == 0 && t == 0)
+                  mma0(raw[b][g][r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
+                else
+                  mma(raw[b][g][r], x0 & M0, x1 & M0, x0 & M1, x1 & M1, y[0], y[1]);
+              }
             }
-          }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t p = lds32(data + b * BB + param_offset(DIM) + 64 * g + slot + 8 * t);
-          const float ks = step_of(p) * c1, km = low_of(p);
-#pragma unroll
-          for (int r = 0; r < NT; ++r) {
-            float2& y = s2[b][r][t];
-            y.x = fmaf(raw[b][g][r][2 * t], ks, g == 0 ? qs[r][g].x * km : fmaf(qs[r][g].x, km, y.x));
-            y.y = fmaf(raw[b][g][r][2 * t + 1], ks, g == 0 ? qs[r][g].y * km : fmaf(qs[r][g].y, km, y.y));
-          }
-        }
-    // steps and centred minima of V
-    float vs[2][G][2], vm[2][G][2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t p = lds32(data + b * BB + param_offset(DIM) + 64 * (G + g) + slot + 8 * t);
-          vs[b][g][t] = step_of(p);
-          vm[b][g][t] = fmaf(vs[b][g][t], 8.0f, low_of(p));
-        }
-    uint32_t seen = 0;  // bit 4 NT b + 4 r + 2 t + x
-    if (PART) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int key = (got >> b & 1) ? key0 + 16 * b + 8 * t + n : -1;
-          bool any = false;
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int r = 0; r < NT; ++r)
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t p = lds32(data + b * BB + param_offset(DIM) + 64 * g + slot + 8 * t);
+            const float ks = step_of(p) * c1, km = low_of(p);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const bool in = key >= lo[r][x] && key < hi[r][x];
-              any |= in;
-              seen |= static_cast<uint32_t>(in) << (4 * NT * b + 4 * r + 2 * t + x);
-              if (!in) (x ? s2[b][r][t].y : s2[b][r][t].x) = -INFINITY;
+            for (int r = 0; r < NT; ++r) {
+              float2& y = s2[b][r][t];
+              y.x = fmaf(raw[b][g][r][2 * t], ks, g == 0 ? qs[r][g].x * km : fmaf(qs[r][g].x, km, y.x));
+              y.y = fmaf(raw[b][g][r][2 * t + 1], ks, g == 0 ? qs[r][g].y * km : fmaf(qs[r][g].y, km, y.y));
             }
-          if (!any)  // a step that none of the rows sees does not count
+          }
+      // steps and centred minima of V
+      float vs[2][G][2], vm[2][G][2];
 #pragma unroll
-            for (int g = 0; g < G; ++g) vs[b][g][t] = vm[b][g][t] = 0.0f;
-        }
-    }
-    bool raise = false;
-    float2 top[NT];
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int r = 0; r < NT; ++r) {
-      top[r].x = fmaxf(fmaxf(s2[0][r][0].x, s2[0][r][1].x), fmaxf(s2[1][r][0].x, s2[1][r][1].x));
-      top[r].y = fmaxf(fmaxf(s2[0][r][0].y, s2[0][r][1].y), fmaxf(s2[1][r][0].y, s2[1][r][1].y));
-      raise |= top[r].x > m[r].x + RAISE || top[r].y > m[r].y + RAISE;
-    }
-    float v = 0.0f;
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int g = 0; g < G; ++g) v = fmaxf(v, fmaxf(fmaxf(vs[0][g][0], vs[0][g][1]), fmaxf(vs[1][g][0], vs[1][g][1])));
-    raise |= v > step_top;
-    if (__any_sync(0xffffffffu, raise)) {
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t p = lds32(data + b * BB + param_offset(DIM) + 64 * (G + g) + slot + 8 * t);
+            vs[b][g][t] = step_of(p);
+            vm[b][g][t] = fmaf(vs[b][g][t], 8.0f, low_of(p));
+          }
+      uint32_t seen = 0;  // bit 4 NT b + 4 r + 2 t + x
+      if (PART) {
 #pragma unroll
-      for (int x = 4; x < 32; x *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
-      int up = 0;
-      if (v > step_top) {
-        const int e = step_exponent(v), to = P_TOP - e;
-        up = step_top == 0.0f ? 0 : to - f_exp;
-        f_exp = to;
-        step_top = v > STEP_MAX ? INFINITY : pow2(e);
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int key = (got >> b & 1) ? key0 + 16 * b + 8 * t + n : -1;
+            bool any = false;
+#pragma unroll
+            for (int r = 0; r < NT; ++r)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const bool in = key >= lo[r][x] && key < hi[r][x];
+                any |= in;
+                seen |= static_cast<uint32_t>(in) << (4 * NT * b + 4 * r + 2 * t + x);
+                if (!in) (x ? s2[b][r][t].y : s2[b][r][t].x) = -INFINITY;
+              }
+            if (!any)  // a step that none of the rows sees does not count
+#pragma unroll
+              for (int g = 0; g < G; ++g) vs[b][g][t] = vm[b][g][t] = 0.0f;
+          }
       }
+      bool raise = false;
+      float2 top[NT];
 #pragma unroll
       for (int r = 0; r < NT; ++r) {
-#pragma unroll
-        for (int x = 4; x < 32; x *= 2) {
-          top[r].x = fmaxf(top[r].x, __shfl_xor_sync(0xffffffffu, top[r].x, x));
-          top[r].y = fmaxf(top[r].y, __shfl_xor_sync(0xffffffffu, top[r].y, x));
-        }
-        const float2 to = make_float2(fmaxf(m[r].x, top[r].x), fmaxf(m[r].y, top[r].y));
-        float2 f;
-        f.x = to.x == -INFINITY ? 1.0f : ex2(m[r].x - to.x + up);
-        f.y = to.y == -INFINITY ? 1.0f : ex2(m[r].y - to.y + up);
-        m[r] = to;
-        off[r].x = (to.x == -INFINITY ? 0.0f : to.x) - f_exp;
-        off[r].y = (to.y == -INFINITY ? 0.0f : to.y) - f_exp;
-        l[r] = __fmul2_rn(l[r], f);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          z[r][g] = __fmul2_rn(z[r][g], f);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) o8[r][g][x] *= x % 2 ? f.y : f.x;
-        }
-#pragma unroll
-        for (int x = 0; x < H * 16; ++x) o[r][x / 16][x / 8 % 2][x / 4 % 2][x % 4] *= x % 2 ? f.y : f.x;
+        top[r].x = fmaxf(fmaxf(s2[0][r][0].x, s2[0][r][1].x), fmaxf(s2[1][r][0].x, s2[1][r][1].x));
+        top[r].y = fmaxf(fmaxf(s2[0][r][0].y, s2[0][r][1].y), fmaxf(s2[1][r][0].y, s2[1][r][1].y));
+        raise |= top[r].x > m[r].x + RAISE || top[r].y > m[r].y + RAISE;
       }
-    }
-    // p F, its sums, and O += (p F s) c
-    uint32_t pb[2][NT][G][2];
+      float v = 0.0f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int g = 0; g < G; ++g) v = fmaxf(v, fmaxf(fmaxf(vs[0][g][0], vs[0][g][1]), fmaxf(vs[1][g][0], vs[1][g][1])));
+      raise |= v > step_top;
+      if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-      for (int r = 0; r < NT; ++r)
+        for (int x = 4; x < 32; x *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+        int up = 0;
+        if (v > step_top) {
+          const int e = step_exponent(v), to = P_TOP - e;
+          up = step_top == 0.0f ? 0 : to - f_exp;
+          f_exp = to;
+          step_top = v > STEP_MAX ? INFINITY : pow2(e);
+        }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float2 y = __fadd2_rn(s2[b][r][t], make_float2(-off[r].x, -off[r].y));
-          const float2 p = make_float2(ex2(y.x), ex2(y.y));
-          l[r] = __fadd2_rn(l[r], p);
+        for (int r = 0; r < NT; ++r) {
+#pragma unroll
+          for (int x = 4; x < 32; x *= 2) {
+            top[r].x = fmaxf(top[r].x, __shfl_xor_sync(0xffffffffu, top[r].x, x));
+            top[r].y = fmaxf(top[r].y, __shfl_xor_sync(0xffffffffu, top[r].y, x));
+          }
+          const float2 to = make_float2(fmaxf(m[r].x, top[r].x), fmaxf(m[r].y, top[r].y));
+          float2 f;
+          f.x = to.x == -INFINITY ? 1.0f : ex2(m[r].x - to.x + up);
+          f.y = to.y == -INFINITY ? 1.0f : ex2(m[r].y - to.y + up);
+          m[r] = to;
+          off[r].x = (to.x == -INFINITY ? 0.0f : to.x) - f_exp;
+          off[r].y = (to.y == -INFINITY ? 0.0f : to.y) - f_exp;
+          l[r] = __fmul2_rn(l[r], f);
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            float2 w = make_float2(p.x * vs[b][g][t], p.y * vs[b][g][t]), low = both(vm[b][g][t]);
-            if (PART) {  // a key that a row does not see: not even its NaN counts
-              const uint32_t in = seen >> (4 * NT * b + 4 * r + 2 * t);
-              if (!(in & 1)) w.x = low.x = 0.0f;
-              if (!(in & 2)) w.y = low.y = 0.0f;
-            }
-            z[r][g].x = fmaf(p.x, low.x, z[r][g].x);
-            z[r][g].y = fmaf(p.y, low.y, z[r][g].y);
-            pb[b][r][g][t] = transpose8(half_pair(w));
+            z[r][g] = __fmul2_rn(z[r][g], f);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o8[r][g][x] *= x % 2 ? f.y : f.x;
           }
-        }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const uint8_t* d = data + b * BB + 512 * H;
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int r = 0; r < NT; ++r)
-          mma(o8[r][g], EIGHTS, EIGHTS, EIGHTS, EIGHTS, pb[b][r][g][0], pb[b][r][g][1]);
-#pragma unroll
-      for (int hw = 0; hw < 2 * H; ++hw) {
-        const uint4 x = lds128(d + 512 * (hw / 2) + 16 * lane);
-        const uint32_t v0 = hw % 2 ? x.y : x.x, v1 = hw % 2 ? x.w : x.z;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t x0 = v0 >> (8 * i), x1 = v1 >> (8 * i);
-#pragma unroll
-          for (int r = 0; r < NT; ++r)
-            mma(o[r][hw / 2][hw % 2][i], x0 & M0, x0 & M1, x1 & M0, x1 & M1, pb[b][r][32 * hw / GROUP][0],
-                pb[b][r][32 * hw / GROUP][1]);
+          for (int x = 0; x < H * 16; ++x) o[r][x / 16][x / 8 % 2][x / 4 % 2][x % 4] *= x % 2 ? f.y : f.x;
         }
       }
-    }
+      // p F, its sums, and O += (p F s) c
+      uint32_t pb[2][NT][G][2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < NT; ++r)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float2 y = __fadd2_rn(s2[b][r][t], make_float2(-off[r].x, -off[r].y));
+            const float2 p = make_float2(ex2(y.x), ex2(y.y));
+            l[r] = __fadd2_rn(l[r], p);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              float2 w = make_float2(p.x * vs[b][g][t], p.y * vs[b][g][t]), low = both(vm[b][g][t]);
+              if (PART) {  // a key that a row does not see: not even its NaN counts
+                const uint32_t in = seen >> (4 * NT * b + 4 * r + 2 * t);
+                if (!(in & 1)) w.x = low.x = 0.0f;
+                if (!(in & 2)) w.y = low.y = 0.0f;
+              }
+              z[r][g].x = fmaf(p.x, low.x, z[r][g].x);
+              z[r][g].y = fmaf(p.y, low.y, z[r][g].y);
+              pb[b][r][g][t] = transpose8(half_pair(w));
+            }
+          }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint8_t* d = data + b * BB + 512 * H;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int r = 0; r < NT; ++r)
+            mma(o8[r][g], EIGHTS, EIGHTS, EIGHTS, EIGHTS, pb[b][r][g][0], pb[b][r][g][1]);
+#pragma unroll
+        for (int hw = 0; hw < 2 * H; ++hw) {
+          const uint4 x = lds128(d + 512 * (hw / 2) + 16 * lane);
+          const uint32_t v0 = hw % 2 ? x.y : x.x, v1 = hw % 2 ? x.w : x.z;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x0 = v0 >> (8 * i), x1 = v1 >> (8 * i);
+#pragma unroll
+            for (int r = 0; r < NT; ++r)
+              mma(o[r][hw / 2][hw % 2][i], x0 & M0, x0 & M1, x1 & M0, x1 & M1, pb[b][r][32 * hw / GROUP][0],
+                  pb[b][r][32 * hw / GROUP][1]);
+          }
+        }
+      }
     };
     if (got != 3u || key0 < lo_all || key0 + UNIT > hi_all)
       body(std::true_type());
@@ -972,168 +973,168 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
       const int key0 = unit * UNIT + 16 * b;
       if (key0 >= hi_warp || key0 + 16 <= lo_warp || !(got >> b & 1)) continue;
       auto body = [&](auto tag) {
-      constexpr bool PART = decltype(tag)::value;  // not every row of the warp sees every key
-      const uint8_t* d = data + b * BB;
-      float2 s2[MT][2][2];  // scores in log2 units: [rows 16 r + n, + 8][keys 2 j + {0, 1}, {8, 9}]
+        constexpr bool PART = decltype(tag)::value;  // not every row of the warp sees every key
+        const uint8_t* d = data + b * BB;
+        float2 s2[MT][2][2];  // scores in log2 units: [rows 16 r + n, + 8][keys 2 j + {0, 1}, {8, 9}]
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float raw[MT][2][4];
+        for (int g = 0; g < G; ++g) {
+          float raw[MT][2][4];
 #pragma unroll
-        for (int hw = g * GROUP / 32; hw < (g + 1) * GROUP / 32; ++hw) {
-          const uint4 k = lds128(d + 512 * (hw / 2) + 16 * lane);
-          const uint32_t kw[2] = {hw % 2 ? k.y : k.x, hw % 2 ? k.w : k.z};
+          for (int hw = g * GROUP / 32; hw < (g + 1) * GROUP / 32; ++hw) {
+            const uint4 k = lds128(d + 512 * (hw / 2) + 16 * lane);
+            const uint32_t kw[2] = {hw % 2 ? k.y : k.x, hw % 2 ? k.w : k.z};
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              const uint32_t y = kw[t] >> (8 * x);
+              for (int t = 0; t < 2; ++t) {
+                const uint32_t y = kw[t] >> (8 * x);
 #pragma unroll
-              for (int r = 0; r < MT; ++r) {
-                const uint32_t(&q)[4] = qa[r][hw / 2][hw % 2][x];
-                if (hw == g * GROUP / 32 && x == 0)
-                  mma0(raw[r][t], q[0], q[1], q[2], q[3], y & M0, y & M1);
-                else
-                  mma(raw[r][t], q[0], q[1], q[2], q[3], y & M0, y & M1);
+                for (int r = 0; r < MT; ++r) {
+                  const uint32_t(&q)[4] = qa[r][hw / 2][hw % 2][x];
+                  if (hw == g * GROUP / 32 && x == 0)
+                    mma0(raw[r][t], q[0], q[1], q[2], q[3], y & M0, y & M1);
+                  else
+                    mma(raw[r][t], q[0], q[1], q[2], q[3], y & M0, y & M1);
+                }
               }
-            }
-        }
-        const uint4 kp = lds128(d + param_offset(DIM) + 64 * g + 16 * j);
+          }
+          const uint4 kp = lds128(d + param_offset(DIM) + 64 * g + 16 * j);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t p0 = t ? kp.z : kp.x, p1 = t ? kp.w : kp.y;
-          const float2 ks = __fmul2_rn(make_float2(step_of(p0), step_of(p1)), both(c1));
-          const float2 km = make_float2(low_of(p0), low_of(p1));
-#pragma unroll
-          for (int r = 0; r < MT; ++r)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const float2 base =
-                  g == 0 ? __fmul2_rn(both(qs[r][u][g]), km) : __ffma2_rn(both(qs[r][u][g]), km, s2[r][u][t]);
-              s2[r][u][t] = __ffma2_rn(make_float2(raw[r][t][2 * u], raw[r][t][2 * u + 1]), ks, base);
-            }
-        }
-      }
-      float2 vs[G][2], vm[G][2];
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint4 vp = lds128(d + param_offset(DIM) + 64 * (G + g) + 16 * j);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t p0 = t ? vp.z : vp.x, p1 = t ? vp.w : vp.y;
-          vs[g][t] = make_float2(step_of(p0), step_of(p1));
-          vm[g][t] = __ffma2_rn(vs[g][t], both(8.0f), make_float2(low_of(p0), low_of(p1)));
-        }
-      }
-      uint32_t seen = 0;  // bit 8 r + 4 u + 2 t + x
-      if (PART) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int key = key0 + 8 * t + 2 * j + x;
-            bool any = false;
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t p0 = t ? kp.z : kp.x, p1 = t ? kp.w : kp.y;
+            const float2 ks = __fmul2_rn(make_float2(step_of(p0), step_of(p1)), both(c1));
+            const float2 km = make_float2(low_of(p0), low_of(p1));
 #pragma unroll
             for (int r = 0; r < MT; ++r)
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                const bool in = key >= lo[r][u] && key < hi[r][u];
-                any |= in;
-                seen |= static_cast<uint32_t>(in) << (8 * r + 4 * u + 2 * t + x);
-                if (!in) (x ? s2[r][u][t].y : s2[r][u][t].x) = -INFINITY;
+                const float2 base =
+                    g == 0 ? __fmul2_rn(both(qs[r][u][g]), km) : __ffma2_rn(both(qs[r][u][g]), km, s2[r][u][t]);
+                s2[r][u][t] = __ffma2_rn(make_float2(raw[r][t][2 * u], raw[r][t][2 * u + 1]), ks, base);
               }
-            if (!any)
-#pragma unroll
-              for (int g = 0; g < G; ++g) (x ? vs[g][t].y : vs[g][t].x) = (x ? vm[g][t].y : vm[g][t].x) = 0.0f;
           }
-      }
-      bool raise = false;
-      float top[MT][2], v = 0.0f;
-#pragma unroll
-      for (int r = 0; r < MT; ++r)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          top[r][u] = fmaxf(fmaxf(s2[r][u][0].x, s2[r][u][0].y), fmaxf(s2[r][u][1].x, s2[r][u][1].y));
-          raise |= top[r][u] > m[r][u] + RAISE;
         }
+        float2 vs[G][2], vm[G][2];
 #pragma unroll
-      for (int g = 0; g < G; ++g) v = fmaxf(v, fmaxf(fmaxf(vs[g][0].x, vs[g][0].y), fmaxf(vs[g][1].x, vs[g][1].y)));
-      raise |= v > step_top;
-      if (__any_sync(0xffffffffu, raise)) {
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-        int up = 0;
-        if (v > step_top) {
-          const int e = step_exponent(v), to = P_TOP - e;
-          up = step_top == 0.0f ? 0 : to - f_exp;
-          f_exp = to;
-          step_top = v > STEP_MAX ? INFINITY : pow2(e);
-        }
-#pragma unroll
-        for (int r = 0; r < MT; ++r) {
-          float f[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(0xffffffffu, top[r][u], 1));
-            top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(0xffffffffu, top[r][u], 2));
-            const float to = fmaxf(m[r][u], top[r][u]);
-            f[u] = to == -INFINITY ? 1.0f : ex2(m[r][u] - to + up);
-            m[r][u] = to;
-            off[r][u] = (to == -INFINITY ? 0.0f : to) - f_exp;
-            l[r][u] = __fmul2_rn(l[r][u], both(f[u]));
-#pragma unroll
-            for (int g = 0; g < G; ++g) z[r][u][g] = __fmul2_rn(z[r][u][g], both(f[u]));
-          }
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o8[r][g][x] *= f[x / 2];
-#pragma unroll
-          for (int x = 0; x < H * 32; ++x) o[r][x / 32][x / 16 % 2][x / 4 % 4][x % 4] *= f[x / 2 % 2];
-        }
-      }
-      // p F, its sums, and O += (p F s) c
-      uint32_t pa[MT][G][4];
-#pragma unroll
-      for (int r = 0; r < MT; ++r)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int g = 0; g < G; ++g) {
+          const uint4 vp = lds128(d + param_offset(DIM) + 64 * (G + g) + 16 * j);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const float2 y = __fadd2_rn(s2[r][u][t], both(-off[r][u]));
-            const float2 p = make_float2(ex2(y.x), ex2(y.y));
-            l[r][u] = __fadd2_rn(l[r][u], p);
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-              float2 w = __fmul2_rn(p, vs[g][t]), low = vm[g][t];
-              if (PART) {  // a key that a row does not see: not even its NaN counts
-                const uint32_t in = seen >> (8 * r + 4 * u + 2 * t);
-                if (!(in & 1)) w.x = low.x = 0.0f;
-                if (!(in & 2)) w.y = low.y = 0.0f;
-              }
-              z[r][u][g] = __ffma2_rn(p, low, z[r][u][g]);
-              pa[r][g][2 * t + u] = half_pair(w);
-            }
-          }
-#pragma unroll
-      for (int r = 0; r < MT; ++r)
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-          mma(o8[r][g], pa[r][g][0], pa[r][g][1], pa[r][g][2], pa[r][g][3], EIGHTS, EIGHTS);
-#pragma unroll
-      for (int hw = 0; hw < 2 * H; ++hw) {
-        const uint4 x = lds128(d + 512 * H + 512 * (hw / 2) + 16 * lane);
-        const uint32_t v0 = hw % 2 ? x.y : x.x, v1 = hw % 2 ? x.w : x.z;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t y0 = v0 >> (8 * i), y1 = v1 >> (8 * i);
-#pragma unroll
-          for (int r = 0; r < MT; ++r) {
-            const uint32_t(&p)[4] = pa[r][32 * hw / GROUP];
-            mma(o[r][hw / 2][hw % 2][2 * i], p[0], p[1], p[2], p[3], y0 & M0, y1 & M0);
-            mma(o[r][hw / 2][hw % 2][2 * i + 1], p[0], p[1], p[2], p[3], y0 & M1, y1 & M1);
+            const uint32_t p0 = t ? vp.z : vp.x, p1 = t ? vp.w : vp.y;
+            vs[g][t] = make_float2(step_of(p0), step_of(p1));
+            vm[g][t] = __ffma2_rn(vs[g][t], both(8.0f), make_float2(low_of(p0), low_of(p1)));
           }
         }
-      }
+        uint32_t seen = 0;  // bit 8 r + 4 u + 2 t + x
+        if (PART) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int key = key0 + 8 * t + 2 * j + x;
+              bool any = false;
+#pragma unroll
+              for (int r = 0; r < MT; ++r)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  const bool in = key >= lo[r][u] && key < hi[r][u];
+                  any |= in;
+                  seen |= static_cast<uint32_t>(in) << (8 * r + 4 * u + 2 * t + x);
+                  if (!in) (x ? s2[r][u][t].y : s2[r][u][t].x) = -INFINITY;
+                }
+              if (!any)
+#pragma unroll
+                for (int g = 0; g < G; ++g) (x ? vs[g][t].y : vs[g][t].x) = (x ? vm[g][t].y : vm[g][t].x) = 0.0f;
+            }
+        }
+        bool raise = false;
+        float top[MT][2], v = 0.0f;
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            top[r][u] = fmaxf(fmaxf(s2[r][u][0].x, s2[r][u][0].y), fmaxf(s2[r][u][1].x, s2[r][u][1].y));
+            raise |= top[r][u] > m[r][u] + RAISE;
+          }
+#pragma unroll
+        for (int g = 0; g < G; ++g) v = fmaxf(v, fmaxf(fmaxf(vs[g][0].x, vs[g][0].y), fmaxf(vs[g][1].x, vs[g][1].y)));
+        raise |= v > step_top;
+        if (__any_sync(0xffffffffu, raise)) {
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          int up = 0;
+          if (v > step_top) {
+            const int e = step_exponent(v), to = P_TOP - e;
+            up = step_top == 0.0f ? 0 : to - f_exp;
+            f_exp = to;
+            step_top = v > STEP_MAX ? INFINITY : pow2(e);
+          }
+#pragma unroll
+          for (int r = 0; r < MT; ++r) {
+            float f[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(0xffffffffu, top[r][u], 1));
+              top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(0xffffffffu, top[r][u], 2));
+              const float to = fmaxf(m[r][u], top[r][u]);
+              f[u] = to == -INFINITY ? 1.0f : ex2(m[r][u] - to + up);
+              m[r][u] = to;
+              off[r][u] = (to == -INFINITY ? 0.0f : to) - f_exp;
+              l[r][u] = __fmul2_rn(l[r][u], both(f[u]));
+#pragma unroll
+              for (int g = 0; g < G; ++g) z[r][u][g] = __fmul2_rn(z[r][u][g], both(f[u]));
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o8[r][g][x] *= f[x / 2];
+#pragma unroll
+            for (int x = 0; x < H * 32; ++x) o[r][x / 32][x / 16 % 2][x / 4 % 4][x % 4] *= f[x / 2 % 2];
+          }
+        }
+        // p F, its sums, and O += (p F s) c
+        uint32_t pa[MT][G][4];
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const float2 y = __fadd2_rn(s2[r][u][t], both(-off[r][u]));
+              const float2 p = make_float2(ex2(y.x), ex2(y.y));
+              l[r][u] = __fadd2_rn(l[r][u], p);
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+                float2 w = __fmul2_rn(p, vs[g][t]), low = vm[g][t];
+                if (PART) {  // a key that a row does not see: not even its NaN counts
+                  const uint32_t in = seen >> (8 * r + 4 * u + 2 * t);
+                  if (!(in & 1)) w.x = low.x = 0.0f;
+                  if (!(in & 2)) w.y = low.y = 0.0f;
+                }
+                z[r][u][g] = __ffma2_rn(p, low, z[r][u][g]);
+                pa[r][g][2 * t + u] = half_pair(w);
+              }
+            }
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            mma(o8[r][g], pa[r][g][0], pa[r][g][1], pa[r][g][2], pa[r][g][3], EIGHTS, EIGHTS);
+#pragma unroll
+        for (int hw = 0; hw < 2 * H; ++hw) {
+          const uint4 x = lds128(d + 512 * H + 512 * (hw / 2) + 16 * lane);
+          const uint32_t v0 = hw % 2 ? x.y : x.x, v1 = hw % 2 ? x.w : x.z;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t y0 = v0 >> (8 * i), y1 = v1 >> (8 * i);
+#pragma unroll
+            for (int r = 0; r < MT; ++r) {
+              const uint32_t(&p)[4] = pa[r][32 * hw / GROUP];
+              mma(o[r][hw / 2][hw % 2][2 * i], p[0], p[1], p[2], p[3], y0 & M0, y1 & M0);
+              mma(o[r][hw / 2][hw % 2][2 * i + 1], p[0], p[1], p[2], p[3], y0 & M1, y1 & M1);
+            }
+          }
+        }
       };
       if (key0 < lo_all || key0 + 16 > hi_all)
         body(std::true_type());
@@ -1330,8 +1331,8 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
   Share s;
   bool any;
   {
-    const int block = static_cast<int>(blockIdx.x), back = a.items.over(block), x = block - back * static_cast<int>(a.items.d);
-    const int entry = a.heads.over(x);
+    const int block = static_cast<int>(blockIdx.x), back = a.items.over(block);
+    const int x = block - back * static_cast<int>(a.items.d), entry = a.heads.over(x);
     any = s.take_at(a, entry, x - entry * a.c.kv_heads, static_cast<int>(a.tiles.d) - 1 - back, TILE_ROWS);
   }
   int lo_cta = 0, hi_cta = 0, x_;
@@ -1602,7 +1603,8 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
 #pragma unroll
       for (int i = 0; i < 4; ++i) tops[i] = max3(x[i].x, x[i].y, x[i + 4].x);
 #pragma unroll
-      for (int i = 4; i < S::KEYS / 2; ++i) tops[i % 4] = i < 8 ? fmaxf(tops[i % 4], x[i].y) : max3(tops[i % 4], x[i].x, x[i].y);
+      for (int i = 4; i < S::KEYS / 2; ++i)
+        tops[i % 4] = i < 8 ? fmaxf(tops[i % 4], x[i].y) : max3(tops[i % 4], x[i].x, x[i].y);
       const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * c1;
       float v = 0.0f;
 #pragma unroll

@@ -30,28 +30,29 @@ __device__ __forceinline__ int32_t* row_of(const lx_kv_cache& c, int slot) {
 }
 
 // Exclusive sum over the block of x, and the block's total.
-__device__ __forceinline__ int block_scan(int x, int* total) {
-  __shared__ int part[32];
+template <typename N>
+__device__ __forceinline__ N block_scan(N x, N* total) {
+  __shared__ N part[32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int sum = x;
+  N sum = x;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    const N y = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += y;
   }
   if (lane == 31) part[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    int y = part[lane];
+    N y = part[lane];
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      const N z = __shfl_up_sync(0xffffffffu, y, o);
       if (lane >= o) y += z;
     }
     part[lane] = y;
   }
   __syncthreads();
-  const int before = warp ? part[warp - 1] : 0;
+  const N before = warp ? part[warp - 1] : 0;
   *total = part[31];
   __syncthreads();
   return before + sum - x;
@@ -82,7 +83,7 @@ struct FirstNamed {
     atomicMin(&who[at], i);
   }
 };
-inline int hash_slots(int n) {
+constexpr int hash_slots(int n) {
   int m = 64;
   while (m < 2 * n) m *= 2;
   return m;
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ int sm[];
-  int* before = sm;          // [n + 1] pages that earlier entries need
+  int* before = sm;            // [n + 1] pages that earlier entries need (2^30: more than any pool has)
   int* slot = before + n + 1;  // [n] the sequence that grows, -1: refused
   int* tail = slot + n;        // [n] page to copy first, -1: none (COPY: the source slot)
   int* len = tail + n;         // [n] tokens before the call (COPY: of the source)
@@ -110,7 +111,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     if (s >= 0 && s < c.n_seq) named.name(s, i);
   }
   __syncthreads();
-  int base = 0;
+  constexpr int64_t MANY = 1 << 30;
+  int64_t base = 0;  // (4096 entries may need 2^26 pages each)
   for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
     const int i = i0 + tid;
     int need = 0;
@@ -154,12 +156,12 @@ __global__ void __launch_bounds__(PLAN_THREADS)
       tail[i] = extra;
       len[i] = tokens;
     }
-    int total;
-    const int at = block_scan(need, &total);
-    if (i < n) before[i] = base + at;
+    int64_t total;
+    const int64_t at = base + block_scan<int64_t>(need, &total);
+    if (i < n) before[i] = static_cast<int>(min(at, MANY));
     base += total;
   }
-  if (tid == 0) before[n] = base;
+  if (tid == 0) before[n] = static_cast<int>(min(base, MANY));
   __syncthreads();
   // how many pages are free
   int count = 0;
@@ -399,10 +401,16 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_kv_move(const lx_kv_cache c) {
   }
 }
 
+// Shared memory of the planning kernels for n entries: `words` for each, and the hash table.
+constexpr size_t plan_smem(int words, int n) {
+  return (static_cast<size_t>(words) * n + 1 + 2 * hash_slots(n)) * sizeof(int);
+}
+// (What the largest batch takes, whatever this one takes: a call on another thread may be about to launch a larger one.)
 template <typename K>
-bool allow_smem(K kernel, size_t bytes) {
-  return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                    static_cast<int>(bytes)) == cudaSuccess;
+bool allow_smem(K kernel, int words, int n) {
+  return plan_smem(words, n) <= 48 * 1024 ||
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(plan_smem(words, LX_KV_MAX_BATCH))) == cudaSuccess;
 }
 
 bool batch_ok(const lx_kv_cache* c, int n, const void* a, const void* b) {
@@ -419,10 +427,9 @@ int grow(const lx_kv_cache* c, int n, const int32_t* a, const int32_t* b, int32_
   OnDevice on(c->device);
   if (!on.ok()) return LX_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int hash = hash_slots(n);
-  const size_t smem = (static_cast<size_t>(4) * n + 1 + 2 * hash) * sizeof(int);
-  if (!allow_smem(k_kv_grow<COPY>, smem)) return LX_ERR_CUDA;
-  if (!launch(k_kv_grow<COPY>, dim3(1), dim3(PLAN_THREADS), smem, s, *c, n, hash, a, b, start)) return LX_ERR_CUDA;
+  if (!allow_smem(k_kv_grow<COPY>, 4, n)) return LX_ERR_CUDA;
+  if (!launch(k_kv_grow<COPY>, dim3(1), dim3(PLAN_THREADS), plan_smem(4, n), s, *c, n, hash_slots(n), a, b, start))
+    return LX_ERR_CUDA;
   return move<false>(*c, s) ? LX_OK : LX_ERR_CUDA;
 }
 
@@ -482,10 +489,9 @@ int lx_kv_fork(const lx_kv_cache* c, int32_t n, const int32_t* src, const int32_
   if (!batch_ok(c, n, src, dst)) return LX_ERR_ARG;
   OnDevice on(c->device);
   if (!on.ok()) return LX_ERR_CUDA;
-  const int hash = hash_slots(n);
-  const size_t smem = (static_cast<size_t>(n) + 2 * hash) * sizeof(int);
-  if (!allow_smem(k_kv_fork, smem)) return LX_ERR_CUDA;
-  return launch(k_kv_fork, dim3(1), dim3(PLAN_THREADS), smem, static_cast<cudaStream_t>(stream), *c, n, hash, src, dst)
+  if (!allow_smem(k_kv_fork, 1, n)) return LX_ERR_CUDA;
+  return launch(k_kv_fork, dim3(1), dim3(PLAN_THREADS), plan_smem(1, n), static_cast<cudaStream_t>(stream), *c, n,
+                hash_slots(n), src, dst)
              ? LX_OK
              : LX_ERR_CUDA;
 }

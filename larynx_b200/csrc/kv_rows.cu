@@ -370,79 +370,79 @@ __global__ void __launch_bounds__(32 * WARPS)
     } else if (head > 0) {
       bring(src, raw);
     }
-  uint32_t word[2][2 * H];
+    uint32_t word[2][2 * H];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int t = n + 8 * u;
+    for (int u = 0; u < 2; ++u) {
+      const int t = n + 8 * u;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      constexpr int PARTS = GROUP / 32;
-      float x[PARTS][8], lo = 0.0f, hi = 0.0f;
+      for (int g = 0; g < G; ++g) {
+        constexpr int PARTS = GROUP / 32;
+        float x[PARTS][8], lo = 0.0f, hi = 0.0f;
 #pragma unroll
-      for (int q = 0; q < PARTS; ++q) {
+        for (int q = 0; q < PARTS; ++q) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[q][i] = to_f32(raw[u][PARTS * g + q].e[i]);
-        if (q == 0) lo = hi = x[0][0];
+          for (int i = 0; i < 8; ++i) x[q][i] = to_f32(raw[u][PARTS * g + q].e[i]);
+          if (q == 0) lo = hi = x[0][0];
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          lo = min_nan(lo, x[q][i], x[q][i + 1]);
-          hi = max_nan(hi, x[q][i], x[q][i + 1]);
+          for (int i = 0; i < 8; i += 2) {
+            lo = min_nan(lo, x[q][i], x[q][i + 1]);
+            hi = max_nan(hi, x[q][i], x[q][i + 1]);
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) {
+          lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+          hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const Params p = params_of(lo, hi);
+        if (j == 0 && t >= first && t < past)
+          *reinterpret_cast<uint32_t*>(block + param_offset(DIM) + 64 * (w.kv * G + g) + 4 * param_slot(t)) = p.packed;
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+          word[u][PARTS * g + q] = w.kv ? codes_of<false>(x[q], p) : codes_of<true>(x[q], p);
+      }
+    }
+    if (!w.kv) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        uint8_t* dst = block + 512 * h + 16 * lane;
+        if (full) {
+          *reinterpret_cast<uint4*>(dst) =
+              make_uint4(word[0][2 * h], word[0][2 * h + 1], word[1][2 * h], word[1][2 * h + 1]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (n + 8 * u >= first && n + 8 * u < past)
+              *reinterpret_cast<uint2*>(dst + 8 * u) = make_uint2(word[u][2 * h], word[u][2 * h + 1]);
         }
       }
-#pragma unroll
-      for (int o = 1; o < 4; o *= 2) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      }
-      const Params p = params_of(lo, hi);
-      if (j == 0 && t >= first && t < past)
-        *reinterpret_cast<uint32_t*>(block + param_offset(DIM) + 64 * (w.kv * G + g) + 4 * param_slot(t)) = p.packed;
-#pragma unroll
-      for (int q = 0; q < PARTS; ++q)
-        word[u][PARTS * g + q] = w.kv ? codes_of<false>(x[q], p) : codes_of<true>(x[q], p);
+      continue;
     }
-  }
-  if (!w.kv) {
+    // V: lane (n', j') of the fragment takes tokens 2 j' + {0, 1, 8, 9}, channels 32 w + 4 n' + {0..3}
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int hw = 0; hw < 2 * H; ++hw)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          sv[pair][256 * (hw / 2) + ((2 * j + q) * 4 + n / 2) * 8 + 4 * u + 2 * (hw % 2) + n % 2] =
+              static_cast<uint16_t>(word[u][hw] >> (16 * q));
+    __syncwarp();
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      uint8_t* dst = block + 512 * h + 16 * lane;
+      uint8_t* dst = block + 512 * (H + h) + 16 * lane;
+      const uint16_t* from = &sv[pair][256 * h + 8 * lane];
       if (full) {
-        *reinterpret_cast<uint4*>(dst) =
-            make_uint4(word[0][2 * h], word[0][2 * h + 1], word[1][2 * h], word[1][2 * h + 1]);
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(from);
       } else {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (n + 8 * u >= first && n + 8 * u < past)
-            *reinterpret_cast<uint2*>(dst + 8 * u) = make_uint2(word[u][2 * h], word[u][2 * h + 1]);
+        for (int i = 0; i < 8; ++i) {
+          const int t = 8 * (i / 4) + 2 * j + i % 2;
+          if (t >= first && t < past) reinterpret_cast<uint16_t*>(dst)[i] = from[i];
+        }
       }
     }
-    continue;
-  }
-  // V: lane (n', j') of the fragment takes tokens 2 j' + {0, 1, 8, 9}, channels 32 w + 4 n' + {0..3}
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int hw = 0; hw < 2 * H; ++hw)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        sv[pair][256 * (hw / 2) + ((2 * j + q) * 4 + n / 2) * 8 + 4 * u + 2 * (hw % 2) + n % 2] =
-            static_cast<uint16_t>(word[u][hw] >> (16 * q));
-  __syncwarp();
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    uint8_t* dst = block + 512 * (H + h) + 16 * lane;
-    const uint16_t* from = &sv[pair][256 * h + 8 * lane];
-    if (full) {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(from);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = 8 * (i / 4) + 2 * j + i % 2;
-        if (t >= first && t < past) reinterpret_cast<uint16_t*>(dst)[i] = from[i];
-      }
-    }
-  }
-  __syncwarp();  // before the next head's codes
+    __syncwarp();  // before the next head's codes
   }
 }
 
@@ -474,68 +474,68 @@ __global__ void __launch_bounds__(32 * WARPS)
   T* dst = (w.kv ? v : k) + w.head * head_stride;
 #pragma unroll 1
   for (int head = 0; head < w.heads; ++head, dst += head_stride, block += head_bytes) {
-  uint4 code[H];
+    uint4 code[H];
 #pragma unroll
-  for (int h = 0; h < H; ++h)
-    code[h] = held > 0 ? __ldcg(reinterpret_cast<const uint4*>(block + 512 * (w.kv * H + h) + 16 * lane))
-                       : make_uint4(0, 0, 0, 0);
-  // the parameters of this lane's tokens: n and n + 8 (K), 2 j + {0, 1, 8, 9} (V)
-  const uint8_t* par = block + param_offset(DIM) + 64 * G * w.kv;
-  uint32_t p[G][4];
+    for (int h = 0; h < H; ++h)
+      code[h] = held > 0 ? __ldcg(reinterpret_cast<const uint4*>(block + 512 * (w.kv * H + h) + 16 * lane))
+                         : make_uint4(0, 0, 0, 0);
+    // the parameters of this lane's tokens: n and n + 8 (K), 2 j + {0, 1, 8, 9} (V)
+    const uint8_t* par = block + param_offset(DIM) + 64 * G * w.kv;
+    uint32_t p[G][4];
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-    if (held > 0) {
-      if (w.kv) {
-        *reinterpret_cast<uint4*>(p[g]) = __ldcg(reinterpret_cast<const uint4*>(par + 64 * g + 16 * j));
-      } else {
-        p[g][0] = __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(n)));
-        p[g][1] = __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(n + 8)));
+    for (int g = 0; g < G; ++g)
+      if (held > 0) {
+        if (w.kv) {
+          *reinterpret_cast<uint4*>(p[g]) = __ldcg(reinterpret_cast<const uint4*>(par + 64 * g + 16 * j));
+        } else {
+          p[g][0] = __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(n)));
+          p[g][1] = __ldcg(reinterpret_cast<const uint32_t*>(par + 64 * g + 4 * param_slot(n + 8)));
+        }
       }
-    }
-  if (!w.kv) {
+    if (!w.kv) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = n + 8 * u;
+      for (int u = 0; u < 2; ++u) {
+        const int t = n + 8 * u;
+        if (t < first || t >= past) continue;
+        T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 8 * j;
+#pragma unroll
+        for (int hw = 0; hw < 2 * H; ++hw) {
+          const uint4 x = code[hw / 2];
+          const uint32_t word = u ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
+          const uint32_t q = p[32 * hw / GROUP][u];
+          const float step = bf16_value(q & 0xFFFFu), low = __uint_as_float(q & 0xFFFF0000u);
+          float even[4], odd[4];
+          codes_f32(word, even);
+          codes_f32(word >> 16, odd);
+          Pack<T, 8> y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) put2(y.e + 2 * i, fmaf(even[i], step, low), fmaf(odd[i], step, low));
+          if (t >= held) y.clear();
+          y.store(out + 32 * hw, wide);
+        }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 2 * j + 8 * (i / 2) + i % 2;
       if (t < first || t >= past) continue;
-      T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 8 * j;
+      T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 4 * n;
 #pragma unroll
       for (int hw = 0; hw < 2 * H; ++hw) {
         const uint4 x = code[hw / 2];
-        const uint32_t word = u ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
-        const uint32_t q = p[32 * hw / GROUP][u];
-        const float step = bf16_value(q & 0xFFFFu), low = __uint_as_float(q & 0xFFFF0000u);
-        float even[4], odd[4];
-        codes_f32(word, even);
-        codes_f32(word >> 16, odd);
-        Pack<T, 8> y;
+        const uint32_t word = i / 2 ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
+        const uint32_t x4 = p[32 * hw / GROUP][i];
+        const float step = bf16_value(x4 & 0xFFFFu), low = __uint_as_float(x4 & 0xFFFF0000u);
+        float e[4];
+        codes_f32(i % 2 ? word >> 16 : word, e);
+        Pack<T, 4> y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put2(y.e + 2 * i, fmaf(even[i], step, low), fmaf(odd[i], step, low));
+        for (int q = 0; q < 2; ++q) put2(y.e + 2 * q, fmaf(e[2 * q], step, low), fmaf(e[2 * q + 1], step, low));
         if (t >= held) y.clear();
         y.store(out + 32 * hw, wide);
       }
     }
-    continue;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = 2 * j + 8 * (i / 2) + i % 2;
-    if (t < first || t >= past) continue;
-    T* out = dst + (s.e.row0 + (s.pos0 + t - s.start)) * row + 4 * n;
-#pragma unroll
-    for (int hw = 0; hw < 2 * H; ++hw) {
-      const uint4 x = code[hw / 2];
-      const uint32_t word = i / 2 ? (hw % 2 ? x.w : x.z) : (hw % 2 ? x.y : x.x);
-      const uint32_t x4 = p[32 * hw / GROUP][i];
-      const float step = bf16_value(x4 & 0xFFFFu), low = __uint_as_float(x4 & 0xFFFF0000u);
-      float e[4];
-      codes_f32(i % 2 ? word >> 16 : word, e);
-      Pack<T, 4> y;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) put2(y.e + 2 * q, fmaf(e[2 * q], step, low), fmaf(e[2 * q + 1], step, low));
-      if (t >= held) y.clear();
-      y.store(out + 32 * hw, wide);
-    }
-  }
   }
 }
 

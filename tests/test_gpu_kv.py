@@ -15,6 +15,10 @@ Attention's bound, per output:
     (both parts are summed).
 lse moves by at most dS + 2^-20 + 2^-22 |lse|."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -624,6 +628,64 @@ class Both:
         data = self.c.bytes().cpu().numpy()
         for p in range(self.o.n_pages):
             assert data[:, p].tobytes() == self.o.data[p], p
+
+
+FIRST = """
+import sys, threading
+sys.path.insert(0, sys.argv[1]); sys.path.insert(0, sys.argv[1] + "/tests")
+import torch
+from test_gpu_kv import Cache
+c = Cache(n_pages=100, n_seq=8, max_pages=12, heads=40)
+c.fill([180, 33, 0, 100, 64, 1, 77, 150])
+calls = []
+for n in (1, 30, 70):  # few rows, many, tiles of 128
+    q = torch.randn(8 * n, 40, 64, device="cuda").bfloat16()
+    calls.append((q, c.batch([n] * 8), torch.empty_like(q)))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    for q, rows, out in calls:
+        c.attend(q, rows, "bf16", chunk=1, out=out, stream=torch.cuda.current_stream().cuda_stream)
+graph.replay()
+torch.cuda.synchronize()
+for q, rows, out in calls:
+    assert torch.equal(out, c.attend(q, rows, "bf16", chunk=1)[0]), "capture"
+c = Cache(n_pages=100, n_seq=8, max_pages=12, heads=40, dim=128)
+c.fill([180, 33, 0, 100, 64, 1, 77, 150])
+for n in (1, 30, 70):
+    q = torch.randn(8 * n, 40, 128, device="cuda").bfloat16()
+    rows, outs = c.batch([n] * 8), [torch.zeros_like(q) for _ in range(6)]
+    streams, go = [torch.cuda.Stream() for _ in outs], threading.Barrier(6)
+    torch.cuda.synchronize()
+    def call(i):
+        go.wait()
+        c.c.attention(0, rows, 40, "bf16", q.data_ptr(), outs[i].data_ptr(), chunk=1, stream=streams[i].cuda_stream)
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(6)]
+    [x.start() for x in threads]; [x.join() for x in threads]
+    torch.cuda.synchronize()
+    want = c.attend(q, rows, "bf16", chunk=1)[0]
+    assert all(torch.equal(x, want) for x in outs), "threads"
+assert c.c.status() == 0
+print("same bits")
+"""
+
+
+def test_first_calls_in_a_capture_and_on_threads():
+    """The first calls of a process: inside a capture, and on six threads at once."""
+    root = str(Path(__file__).resolve().parent.parent)
+    done = subprocess.run([sys.executable, "-c", FIRST, root], capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0 and "same bits" in done.stdout, done.stderr[-2000:]
+
+
+def test_extend_by_more_pages_than_32_bits_count():
+    """The pages that a batch wants add up to more than 2^31: none is served."""
+    n = 33
+    c = Cache(n_pages=8, n_seq=n, max_pages=2 ** 26, heads=1)
+    start = c.grow(list(range(n)), [2 ** 30] * n)
+    assert c.c.status() == c.kv.FULL
+    assert (start == ko.REFUSED).all() and (c.lengths == 0).all() and (c.refs == 0).all()
+    # the entries before one that is not served are
+    start = c.grow([0, 1, 2], [16, 2 ** 30, 16])
+    assert start.tolist() == [0, ko.REFUSED, ko.REFUSED] and c.lengths[:3].tolist() == [16, 0, 0] and c.c.status() == c.kv.FULL
 
 
 def test_pages_by_hand():
