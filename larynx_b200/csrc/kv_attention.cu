@@ -12,19 +12,24 @@
 // product with the constant 8 takes off what the centring needs, of the same
 // rounded values.  q is scaled by a power of two so that the largest value of
 // the rows is near 2^13 (what fp16 loses is below 2^-38 of that).  p is taken times a
-// power of two F that brings the largest step of V so far to 2^7: p s F stays
-// below 2^15, and what fp16 rounds away is 2^-11 of each term, or 2^-32 of
-// the largest.  F cancels in the quotient.
+// power of two F that brings the largest step of V so far into (2^6, 2^7]: p s F
+// does not exceed 2^15, and what fp16 rounds away is 2^-11 of each term, or 2^-31 of
+// the largest step.  F cancels in the quotient.
 //
 // The maximum is raised, and the sums rescaled, only when a score exceeds it by
 // 8 (log2 units), so p <= 2^8; likewise F only when a step exceeds its bound.
+// Scores, maxima, sums and O are fp32; P and the scaled q are the only values
+// rounded to fp16.
 //
-// Two forms, by the rows (query rows x query heads of one kv head) of an entry:
-// k_kv_few for up to 16, whose warps all split the keys, and k_kv_many, whose warps
-// share the keys' bytes.  In both a cluster of CTAs splits the keys of long
-// sequences, joined through shared memory in a fixed order: no workspace in
-// global memory, so calls may overlap.  The bytes come through rings of
-// bulk copies, two blocks a stage.
+// Three forms, by the rows (query rows x query heads of one kv head) of an entry:
+//   k_kv_few   up to 16: every warp has all rows, the warps split the keys;
+//   k_kv_many  above:    warps of 16 rows share the keys that one of them brings;
+//   k_kv_tile  above 64: tiles of 128 rows on tcgen05, where there are tiles for every SM.
+// (mma.sync reaches 550 TFLOP/s here, a third of the tensor cores; up to 16 rows
+// the bytes and the unpacking bound, not the products.)  In the first two a cluster of
+// CTAs splits the keys of long sequences, joined through shared memory in a fixed
+// order: no workspace in global memory, so calls may overlap, and the same call
+// gives the same bits.  Their bytes come through rings of bulk copies, two blocks a stage.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -459,6 +464,13 @@ __device__ __forceinline__ void join(const Args& a, const Share& s, float* part_
 // unpacking.  P^T is the transpose of what S^T leaves in the registers: one
 // movmatrix for 8 keys.  Lane (n, j) holds the scores of keys n and n + 8 with
 // rows 2 j and 2 j + 1.
+//   Bound: 128 channels, four rows, 64 entries of 4099-8191 keys: 101 us, 4.5 TB/s
+// of 6.55.  The registers allow twelve warps an SM, whose chains score, exponential,
+// product leave half of the issue slots empty (the ALU, which unpacks, is at 48 %; sixteen
+// warps of 128 registers: 114 us).  Beginning and end of a block cost as
+// much as six units: 64 entries of 41-2100 keys, 64 channels: 10.6 us against 1.7 for
+// the bytes.  One sequence of 131071 keys: 56 us (2.7 TB/s), since its 8 clusters
+// reach 80 SMs; more would take a workspace.
 template <int DIM, int GROUP, int NT, int KW>
 struct FewShape {
   static constexpr int THREADS = 32 * KW, ROWS = 8 * NT;
@@ -823,6 +835,11 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
 // ---------------------------------------------------------------------------
 // MW warps of 16 MT rows share each unit of keys.  Lane (n, j) holds the scores of rows
 // n and n + 8 of each 16 with keys 2 j + {0, 1, 8, 9}, which is how P enters the second product.
+//   Bound: the unpacking, which every warp repeats, and the softmax (the ALU at 43 %,
+// tensor pipe at 24 %, 47 % of the issue slots; 2.6 rounds of blocks with 56-556 keys each):
+// 96 entries of 56 rows, 16 heads of 64 channels: 64 us, against 12 for the products
+// at the rate of mma.sync and 9 for the bytes.  (Two warps of two tiles, which halve
+// the unpacking but not the chain: 68 us.)
 template <int DIM, int GROUP, int MT, int MW>
 struct ManyShape {
   static constexpr int THREADS = 32 * MW, ROWS = 16 * MT * MW;
@@ -1223,6 +1240,10 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 // Four warps do the softmax, a thread a row: nothing is exchanged between
 // lanes, and what a key's step and minimum cost is shared with nobody but
 // also needs no unpacking, against eight rows and unpacking in every warp in the forms above.
+//   Bound: the softmax (a row of 128 scores is read, raised, exponentiated and packed
+// by one thread) and the unpacking beside it, with two CTAs an SM taking turns: four
+// entries of 701-1500 rows, 16 heads of 64 channels: 86 us, against 14 for the
+// products; with k_kv_many 203.
 //   V's tile holds the channels of 32 in the order 8 i + n for channel 4 n + i,
 // which is how the unpacking warps write it without bank conflicts; the rows
 // are put in order when they are written out.
@@ -1871,7 +1892,9 @@ bool go(Args& a, int max_len, cudaStream_t s) {
   const long long items = static_cast<long long>(a.r.n) * a.c.kv_heads;
   const int units = (max_len + UNIT - 1) / UNIT;
   if (rows <= 16) {
-    // CTAs of four warps, or where clusters of sixteen of them leave the GPU empty, of as many as an SM holds
+    // CTAs of four warps, or where clusters of sixteen of them leave the GPU empty, of as many as an SM holds (one
+    // sequence of 131071 keys, 8 kv heads of 128 channels, us: clusters of sixteen of four warps 79, of ten of twelve 57;
+    // 64 x 8 items: four warps 105, twelve 119)
     constexpr int WIDE = DIM == 64 ? 16 : 12;
     const bool wide = items * 16 * 4 < num_sms() * 8 && units > 4 * 16;
     if (rows <= 8) return wide ? few<T, DIM, GROUP, 1, WIDE>(a, units, s) : few<T, DIM, GROUP, 1, 4>(a, units, s);

@@ -5,6 +5,11 @@
 // planning kernel, which decides in one block which page goes where, and for
 // calls that move data a copy kernel over the whole GPU that takes its list of
 // pages from the cache's scratch.
+//
+// Bound: launches and the planning block's chain of scans (some 4 us) for short calls:
+// freeing, forking and growing 4 sequences of 300 tokens takes 15-17 us, four launches;
+// DRAM for long ones: 390 MB read and as much written in 135 us, 5.8 TB/s of 6.55, where the
+// device's own copy of as much takes 125.
 #include <climits>
 
 #include "kv.cuh"
@@ -345,6 +350,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_compact(const lx_kv_cache c
   }
 }
 
+// (Sixteen blocks an SM, each reading its next piece while one is written: 146 -> 135 us for the 390 MB above.)
 constexpr int MOVE_THREADS = 256;
 constexpr int PIECE = 16 * MOVE_THREADS * 4;  // bytes that a block copies at once
 

@@ -6,6 +6,13 @@
 // so K needs no exchange; V's codes pass through shared memory.  In reading, V is
 // taken as it lies: lane (n, j) holds tokens 2 j + {0, 1, 8, 9} and channels
 // 64 h + 32 w + 4 n + {0..3}.  All of a lane's loads are in flight before the first is used.
+// A warp takes several heads of its block where there are more warps than run at once:
+// finding the block (slot, length, page: three loads in a row) costs as much as two heads.
+//
+// Bound: DRAM for long fp32 rows (8 sequences of 3001-4099 tokens, 8 heads of 128
+// channels, written and read back: 125 us, 4.2 TB/s of 6.55, the lookups before the
+// first load of a block being what is missing), latency for short ones (96 x 50 rows of
+// 16 heads: 31 us of which the bytes are 8; 64 single tokens: two launches).
 //
 // Quantising, per token and group (include/larynx_kv.h): the codes are those
 // of exact arithmetic, without branches (16-bit values meet ties in every other warp; a
@@ -100,14 +107,16 @@ __device__ __forceinline__ Params params_of(float lo, float hi) {
 // Packed sums rounded down and up.
 __device__ __forceinline__ float2 add2_rm(float2 a, float2 b) {
   float2 c;
-  asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rm.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+  asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rm.f32x2 c, a, b;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
       : "=f"(c.x), "=f"(c.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return c;
 }
 __device__ __forceinline__ float2 add2_rp(float2 a, float2 b) {
   float2 c;
-  asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rp.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+  asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rp.f32x2 c, a, b;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
       : "=f"(c.x), "=f"(c.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return c;
@@ -319,8 +328,8 @@ __device__ __forceinline__ Work work_of(const lx_kv_cache& c, const lx_kv_rows& 
 
 template <typename T, int DIM, int GROUP>
 __global__ void __launch_bounds__(32 * WARPS)
-    k_kv_write(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, int heads, const T* __restrict__ k, int64_t k_row,
-               int64_t k_head, const T* __restrict__ v, int64_t v_row, int64_t v_head, bool wide) {
+    k_kv_write(const lx_kv_cache c, int layer, const lx_kv_rows r, int blocks, int heads, const T* __restrict__ k,
+               int64_t k_row, int64_t k_head, const T* __restrict__ v, int64_t v_row, int64_t v_head, bool wide) {
   constexpr int H = DIM / 64, G = DIM / GROUP;
   __shared__ __align__(16) uint16_t sv[WARPS / 2][H * 256];
   const int pair = threadIdx.x / 64, lane = threadIdx.x % 32, n = lane / 4, j = lane % 4;
@@ -567,8 +576,8 @@ bool go(bool writes, const lx_kv_cache& c, int layer, const lx_kv_rows& r, void*
   if (writes)
     return launch(k_kv_write<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks, heads,
                   static_cast<const T*>(k), k_row, k_head, static_cast<const T*>(v), v_row, v_head, wide);
-  return launch(k_kv_read<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks, heads, static_cast<T*>(k), k_row,
-                k_head, static_cast<T*>(v), v_row, v_head, wide);
+  return launch(k_kv_read<T, DIM, GROUP>, grid, dim3(32 * WARPS), 0, s, c, layer, r, blocks, heads, static_cast<T*>(k),
+                k_row, k_head, static_cast<T*>(v), v_row, v_head, wide);
 }
 
 int rows_call(bool writes, const lx_kv_cache* c, int layer, const lx_kv_rows* r, int dtype, void* k, int64_t k_row,
