@@ -10,6 +10,7 @@
 // freeing, forking and growing 4 sequences of 300 tokens takes 15-17 us, four launches;
 // DRAM for long ones: 390 MB read and as much written in 135 us, 5.8 TB/s of 6.55, where the
 // device's own copy of as much takes 125.
+#include <algorithm>
 #include <climits>
 
 #include "kv.cuh"
@@ -94,6 +95,15 @@ constexpr int hash_slots(int n) {
   return m;
 }
 
+// Which of the pages p .. p + 3 are free, as bits.
+__device__ __forceinline__ int free_bits(const lx_kv_cache& c, int p) {
+  int bits = 0;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (p + x < c.n_pages && c.refs[p + x] == 0) bits |= 1 << x;
+  return bits;
+}
+
 // lx_kv_extend (COPY false: a = seqs, b = counts) and lx_kv_copy (a = src, b = dst).
 template <bool COPY>
 __global__ void __launch_bounds__(PLAN_THREADS)
@@ -109,6 +119,13 @@ __global__ void __launch_bounds__(PLAN_THREADS)
   __shared__ int moves;
   const int tid = threadIdx.x;
   if (tid == 0) moves = 0;
+  // how many pages are free, and which of this thread's of the first tile (bits): asked for before anything else waits
+  int count = 0, first = 0;
+  for (int p0 = 4 * tid; p0 < c.n_pages; p0 += TILE) {
+    const int bits = free_bits(c, p0);
+    count += __popc(bits);
+    if (p0 == 4 * tid) first = bits;
+  }
   named.clear();
   __syncthreads();
   for (int i = tid; i < n; i += PLAN_THREADS) {
@@ -168,20 +185,13 @@ __global__ void __launch_bounds__(PLAN_THREADS)
   }
   if (tid == 0) before[n] = static_cast<int>(min(base, MANY));
   __syncthreads();
-  // how many pages are free
-  int count = 0;
-  for (int p = tid; p < c.n_pages; p += PLAN_THREADS) count += c.refs[p] == 0;
   int n_free;
   block_scan(count, &n_free);
   // give them out
   const int wanted = before[n];
   int rank0 = 0;
   for (int p0 = 0; p0 < c.n_pages && rank0 < wanted; p0 += TILE) {
-    int is_free = 0;
-    for (int x = 0; x < 4; ++x) {
-      const int p = p0 + 4 * tid + x;
-      if (p < c.n_pages && c.refs[p] == 0) is_free |= 1 << x;
-    }
+    const int is_free = p0 == 0 ? first : free_bits(c, p0 + 4 * tid);
     int total;
     int rank = rank0 + block_scan(__popc(is_free), &total);
     rank0 += total;
@@ -423,9 +433,13 @@ bool batch_ok(const lx_kv_cache* c, int n, const void* a, const void* b) {
   return cache_ok(c) && n > 0 && n <= LX_KV_MAX_BATCH && a && b && aligned(a, 4) && aligned(b, 4);
 }
 
+// `most`: no more pages than this can be on the list.
 template <bool REMAP>
-bool move(const lx_kv_cache& c, cudaStream_t s) {
-  return launch(k_kv_move<REMAP>, dim3(16 * num_sms()), dim3(MOVE_THREADS), 0, s, c);
+bool move(const lx_kv_cache& c, long long most, cudaStream_t s) {
+  const long long bytes = static_cast<long long>(c.kv_heads) * (c.page / BLOCK) * block_bytes(c.head_dim, c.group);
+  const long long pieces = (bytes + PIECE - 1) / PIECE * c.n_layers;
+  const int grid = static_cast<int>(std::min<long long>(16 * num_sms(), std::min<long long>(most, c.n_pages) * pieces));
+  return launch(k_kv_move<REMAP>, dim3(grid), dim3(MOVE_THREADS), 0, s, c);
 }
 
 template <bool COPY>
@@ -436,7 +450,7 @@ int grow(const lx_kv_cache* c, int n, const int32_t* a, const int32_t* b, int32_
   if (!allow_smem(k_kv_grow<COPY>, 4, n)) return LX_ERR_CUDA;
   if (!launch(k_kv_grow<COPY>, dim3(1), dim3(PLAN_THREADS), plan_smem(4, n), s, *c, n, hash_slots(n), a, b, start))
     return LX_ERR_CUDA;
-  return move<false>(*c, s) ? LX_OK : LX_ERR_CUDA;
+  return move<false>(*c, COPY ? c->n_pages : n, s) ? LX_OK : LX_ERR_CUDA;
 }
 
 }  // namespace
@@ -517,7 +531,7 @@ int lx_kv_compact(const lx_kv_cache* c, int32_t* used, void* stream) {
   if (!on.ok()) return LX_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!launch(k_kv_compact, dim3(1), dim3(PLAN_THREADS), 0, s, *c, used)) return LX_ERR_CUDA;
-  return move<true>(*c, s) ? LX_OK : LX_ERR_CUDA;
+  return move<true>(*c, c->n_pages, s) ? LX_OK : LX_ERR_CUDA;
 }
 
 }  // extern "C"

@@ -6,7 +6,7 @@
 // so K needs no exchange; V's codes pass through shared memory.  In reading, V is
 // taken as it lies: lane (n, j) holds tokens 2 j + {0, 1, 8, 9} and channels
 // 64 h + 32 w + 4 n + {0..3}.  All of a lane's loads are in flight before the first is used.
-// A warp takes several heads of its block where there are more warps than run at once:
+// A warp takes up to three heads of its block where there are more warps than run at once:
 // finding the block (slot, length, page: three loads in a row) costs as much as two heads.
 //
 // Bound: DRAM for long fp32 rows (8 sequences of 3001-4099 tokens, 8 heads of 128
@@ -17,8 +17,8 @@
 // Quantising, per token and group (include/larynx_kv.h): the codes are those
 // of exact arithmetic, without branches (16-bit values meet ties in every other warp; a
 // second look at those cost four times the instructions).
+#include <algorithm>
 #include <cfloat>
-#include <cmath>
 
 #include "kv.cuh"
 
@@ -560,17 +560,12 @@ bool go(bool writes, const lx_kv_cache& c, int layer, const lx_kv_rows& r, void*
         void* v, int64_t v_row, int64_t v_head, cudaStream_t s) {
   const int blocks = (r.max_rows + BLOCK - 2) / BLOCK + 1;  // rows may begin inside a block
   const long long items = static_cast<long long>(r.n) * blocks;
-  // Heads a warp: finding the block costs as long as two heads of it, and about twenty warps run on an SM at once.
-  int heads = 1;
-  double best = 0.0;
-  for (int h = 1; h <= 8 && h <= c.kv_heads; ++h) {
-    const double warps = 2.0 * static_cast<double>(items) * ((c.kv_heads + h - 1) / h);
-    const double cost = std::ceil(warps / (20.0 * num_sms())) * (2 + h);
-    if (h == 1 || cost < best) {
-      best = cost;
-      heads = h;
-    }
-  }
+  // Heads a warp: up to three, where that leaves twenty warps for every SM (about as many as run at once).  Written, read,
+  // us, for 1, 2, 3, 4, 8 heads a warp: 96 x 50 rows of 16 heads: 20.6 + 10.1, 18.2 + 8.2, 17.4 + 7.7, 18.0 + 8.9, 18.6 + 8.6;
+  // 8 x 3001-4099 rows of 8 heads, 128 channels, fp32: 71.6 + 50.2, 65.6 + 54.9, 63.8 + 53.1, 67.6 + 57.0, 72.8 + 63.9;
+  // 64 x 1 rows of 2 heads: 3.3 + 2.3, 4.7 + 2.5.
+  const long long warps = 2 * items * c.kv_heads;
+  const int heads = static_cast<int>(std::max<long long>(1, std::min<long long>(3, warps / (20 * num_sms()))));
   const dim3 grid(static_cast<unsigned>((items + WARPS / 2 - 1) / (WARPS / 2)), (c.kv_heads + heads - 1) / heads);
   const bool wide = wide_rows<T>(k, k_row, k_head, v, v_row, v_head);
   if (writes)
