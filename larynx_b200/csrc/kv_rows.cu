@@ -10,15 +10,16 @@
 // finding the block (slot, length, page: three loads in a row) costs as much as two heads.
 //
 // Bound: DRAM for long fp32 rows (8 sequences of 3001-4099 tokens, 8 heads of 128
-// channels, written and read back: 125 us, 4.2 TB/s of 6.55, the lookups before the
-// first load of a block being what is missing), latency for short ones (96 x 50 rows of
-// 16 heads: 31 us of which the bytes are 8; 64 single tokens: two launches).
+// channels: written in 57 us, 4.7 TB/s of 6.55, the quantiser's instructions being what is
+// missing, and read in 53, 5.0 TB/s), latency for short ones (96 x 50 rows of 16 heads:
+// 15 and 8 us, of which the bytes are 4 and 4; 64 single tokens: 3 and 2, launches).
 //
 // Quantising, per token and group (include/larynx_kv.h): the codes are those
 // of exact arithmetic, without branches (16-bit values meet ties in every other warp; a
 // second look at those cost four times the instructions).
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "kv.cuh"
 
@@ -29,11 +30,6 @@ namespace {
 constexpr int WARPS = 4;
 constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float c;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-  return c;
-}
 __device__ __forceinline__ float min_nan(float a, float b, float c) {
   float d;
   asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -66,9 +62,16 @@ __device__ __forceinline__ uint32_t bf16_floor(float x) {
 __device__ __forceinline__ float bf16_value(uint32_t u) { return __uint_as_float(u << 16); }
 
 struct Params {
-  float s, m, inv;
+  float inv;        // 1 / s; negative for a step so small that products with it lose bits (and not all values equal)
   uint32_t packed;  // bf16 s in the low half, bf16 m in the high half
-  bool small;       // a step so small that products with it lose bits (and not all values equal)
+  __device__ __forceinline__ float step() const { return bf16_value(packed & 0xFFFFu); }
+  __device__ __forceinline__ float low() const { return __uint_as_float(packed & 0xFFFF0000u); }
+  __device__ __forceinline__ Params from(int lane) const {
+    Params p;
+    p.inv = __shfl_sync(0xffffffffu, inv, lane);
+    p.packed = __shfl_sync(0xffffffffu, packed, lane);
+    return p;
+  }
 };
 
 // Step and minimum of a group with smallest and largest value lo, hi (NaN where
@@ -80,10 +83,8 @@ __device__ __forceinline__ Params params_of(float lo, float hi) {
   const float m = bf16_value(mb), range = hi - m;
   const float rest = diff_error(hi, m, range);
   if (!(fabsf(lo) <= FLT_MAX) || !(fabsf(m) <= FLT_MAX) || !(fabsf(hi) <= FLT_MAX) || !(range <= FLT_MAX)) {
-    p.s = p.m = __uint_as_float(0x7fc00000u);
     p.inv = 0.0f;
     p.packed = 0x7fc07fc0u;
-    p.small = false;
     return p;
   }
   constexpr uint32_t least = 0x00800000u;  // 2^-126
@@ -96,11 +97,10 @@ __device__ __forceinline__ Params params_of(float lo, float hi) {
     top = 15.0f * __uint_as_float(sb - 0x10000u);
     if (top > range || (top == range && rest <= 0.0f)) sb -= 0x10000u;
   }
-  p.s = __uint_as_float(sb);
-  p.m = m;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(p.inv) : "f"(p.s));  // to an ulp, which is enough (codes_of)
+  const float s = __uint_as_float(sb);
+  asm("rcp.approx.f32 %0, %1;" : "=f"(p.inv) : "f"(s));  // to an ulp, which is enough (codes_of)
+  if (s < 7.8886091e-31f && range > 0.0f) p.inv = -p.inv;  // 2^-100
   p.packed = (sb >> 16) | (mb << 16);
-  p.small = p.s < 7.8886091e-31f && range > 0.0f;  // 2^-100
   return p;
 }
 
@@ -144,24 +144,25 @@ __device__ __noinline__ float small_code(float x, float m, float s) {
 //  * MAGIC + c has c in its low bits: a sum of products with powers of 16 packs the codes.
 template <bool K>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], const Params& p) {
+  const float s = p.step(), m = p.low(), to = fabsf(p.inv);
   float t[8];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const float2 v = make_float2(x[i], x[i + 1]), low = make_float2(-p.m, -p.m);
+    const float2 v = make_float2(x[i], x[i + 1]), low = make_float2(-m, -m);
     const float2 down = add2_rm(v, low), up = add2_rp(v, low);
     float2 d;
     d.x = __uint_as_float(__float_as_uint(down.x) | (__float_as_uint(up.x) - __float_as_uint(down.x)));
     d.y = __uint_as_float(__float_as_uint(down.y) | (__float_as_uint(up.y) - __float_as_uint(down.y)));
-    const float2 inv = make_float2(p.inv, p.inv);
+    const float2 inv = make_float2(to, to);
     const float2 y = __fmul2_rn(d, inv);
-    const float2 e = __ffma2_rn(make_float2(-y.x, -y.y), make_float2(p.s, p.s), d);
+    const float2 e = __ffma2_rn(make_float2(-y.x, -y.y), make_float2(s, s), d);
     const float2 r = __fadd2_rn(__ffma2_rn(e, inv, y), make_float2(MAGIC, MAGIC));
     t[i] = r.x;
     t[i + 1] = r.y;
   }
-  if (p.small) {
+  if (p.inv < 0.0f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = small_code(x[i], p.m, p.s);
+    for (int i = 0; i < 8; ++i) t[i] = small_code(x[i], m, s);
   }
   uint32_t bits = 0, magic = 0;
 #pragma unroll
@@ -256,6 +257,95 @@ struct Pack {
     }
   }
 };
+
+// The largest of some values and of their negatives (NaN where one of them is).
+template <typename T>
+struct Bounds {
+  uint32_t v;  // both as T, the negatives in the high half
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t c;
+    if (std::is_same<T, bf16>::value)
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    else
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+  }
+  static __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t c;
+    if (std::is_same<T, bf16>::value)
+      asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    else
+      asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+  }
+  template <int PARTS>
+  __device__ __forceinline__ void of(const Pack<T, 8>* x) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(x[0].e);
+    uint32_t hi = w[0], lo = w[0];
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      w = reinterpret_cast<const uint32_t*>(x[q].e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        hi = max2(hi, w[i]);
+        lo = min2(lo, w[i]);
+      }
+    }
+    lo ^= 0x80008000u;
+    v = max2(__byte_perm(hi, lo, 0x5410), __byte_perm(hi, lo, 0x7632));
+  }
+  __device__ __forceinline__ void add(const Bounds& b) { v = max2(v, b.v); }
+  __device__ __forceinline__ Bounds across(int lanes) const { return Bounds{__shfl_xor_sync(0xffffffffu, v, lanes)}; }
+  __device__ __forceinline__ float value(uint32_t bits) const {
+    const uint16_t h = static_cast<uint16_t>(bits);
+    return to_f32(*reinterpret_cast<const T*>(&h));
+  }
+  __device__ __forceinline__ float hi() const { return value(v & 0xFFFFu); }
+  __device__ __forceinline__ float lo() const { return -value(v >> 16); }
+};
+template <>
+struct Bounds<float> {
+  float top, neg;
+  template <int PARTS>
+  __device__ __forceinline__ void of(const Pack<float, 8>* x) {
+    float low = top = x[0].e[0];
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        low = min_nan(low, x[q].e[i], x[q].e[i + 1]);
+        top = max_nan(top, x[q].e[i], x[q].e[i + 1]);
+      }
+    neg = -low;
+  }
+  __device__ __forceinline__ void add(const Bounds& b) {
+    top = max_nan(top, b.top);
+    neg = max_nan(neg, b.neg);
+  }
+  __device__ __forceinline__ Bounds across(int lanes) const {
+    return Bounds{__shfl_xor_sync(0xffffffffu, top, lanes), __shfl_xor_sync(0xffffffffu, neg, lanes)};
+  }
+  __device__ __forceinline__ float hi() const { return top; }
+  __device__ __forceinline__ float lo() const { return -neg; }
+};
+
+// Of the bounds that the four lanes j of a quad hold of 4 (or 2) sets: those of set j (or j % 2), over all four lanes.
+template <typename B>
+__device__ __forceinline__ B gather(const B (&b)[4], int j) {
+  B keep[2] = {j & 2 ? b[2] : b[0], j & 2 ? b[3] : b[1]};
+  keep[0].add((j & 2 ? b[0] : b[2]).across(2));
+  keep[1].add((j & 2 ? b[1] : b[3]).across(2));
+  B one = j & 1 ? keep[1] : keep[0];
+  one.add((j & 1 ? keep[0] : keep[1]).across(1));
+  return one;
+}
+template <typename B>
+__device__ __forceinline__ B gather(const B (&b)[2], int j) {
+  B one = j & 1 ? b[1] : b[0];
+  one.add((j & 1 ? b[0] : b[1]).across(1));
+  one.add(one.across(2));
+  return one;
+}
 
 // Codes 0..3 of a 16-bit field (the low half of `word`) as floats: with the exponent of 2^(23 - 4 i) above it, code i
 // stands at the units of the float's mantissa.
@@ -379,36 +469,37 @@ __global__ void __launch_bounds__(32 * WARPS)
     } else if (head > 0) {
       bring(src, raw);
     }
+    // Set x of the 2 G pairs of a token n + 8 (x / G) and a group x % G: lane (n, x % 4) gets its bounds from the four
+    // lanes that hold the group, works out step and minimum, and gives them back.  (Every lane working out all of
+    // them: 17.4 and 63.8 us for the rows above, against 14.8 and 57.0.)
+    constexpr int SETS = 2 * G, PARTS = GROUP / 32;
+    Params mine[(SETS + 3) / 4];
+#pragma unroll
+    for (int x = 0; x < (SETS + 3) / 4; ++x) {
+      Bounds<T> b[SETS < 4 ? SETS : 4];
+#pragma unroll
+      for (int q = 0; q < (SETS < 4 ? SETS : 4); ++q) {
+        const int set = 4 * x + q;
+        b[q].template of<PARTS>(&raw[set / G][PARTS * (set % G)]);
+      }
+      const Bounds<T> all = gather(b, j);
+      mine[x] = params_of(all.lo(), all.hi());
+      const int set = 4 * x + j % SETS, at = n + 8 * (set / G);
+      if (j < SETS && at >= first && at < past)
+        *reinterpret_cast<uint32_t*>(block + param_offset(DIM) + 64 * (w.kv * G + set % G) + 4 * param_slot(at)) =
+            mine[x].packed;
+    }
     uint32_t word[2][2 * H];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = n + 8 * u;
+    for (int set = 0; set < SETS; ++set) {
+      const Params p = mine[set / 4].from(lane / 4 * 4 + set % 4);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        constexpr int PARTS = GROUP / 32;
-        float x[PARTS][8], lo = 0.0f, hi = 0.0f;
+      for (int q = 0; q < PARTS; ++q) {
+        const int hw = PARTS * (set % G) + q;
+        float x[8];
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[q][i] = to_f32(raw[u][PARTS * g + q].e[i]);
-          if (q == 0) lo = hi = x[0][0];
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            lo = min_nan(lo, x[q][i], x[q][i + 1]);
-            hi = max_nan(hi, x[q][i], x[q][i + 1]);
-          }
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o *= 2) {
-          lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-          hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-        const Params p = params_of(lo, hi);
-        if (j == 0 && t >= first && t < past)
-          *reinterpret_cast<uint32_t*>(block + param_offset(DIM) + 64 * (w.kv * G + g) + 4 * param_slot(t)) = p.packed;
-#pragma unroll
-        for (int q = 0; q < PARTS; ++q)
-          word[u][PARTS * g + q] = w.kv ? codes_of<false>(x[q], p) : codes_of<true>(x[q], p);
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(raw[set / G][hw].e[i]);
+        word[set / G][hw] = w.kv ? codes_of<false>(x, p) : codes_of<true>(x, p);
       }
     }
     if (!w.kv) {
@@ -560,10 +651,10 @@ bool go(bool writes, const lx_kv_cache& c, int layer, const lx_kv_rows& r, void*
         void* v, int64_t v_row, int64_t v_head, cudaStream_t s) {
   const int blocks = (r.max_rows + BLOCK - 2) / BLOCK + 1;  // rows may begin inside a block
   const long long items = static_cast<long long>(r.n) * blocks;
-  // Heads a warp: up to three, where that leaves twenty warps for every SM (about as many as run at once).  Written, read,
-  // us, for 1, 2, 3, 4, 8 heads a warp: 96 x 50 rows of 16 heads: 20.6 + 10.1, 18.2 + 8.2, 17.4 + 7.7, 18.0 + 8.9, 18.6 + 8.6;
-  // 8 x 3001-4099 rows of 8 heads, 128 channels, fp32: 71.6 + 50.2, 65.6 + 54.9, 63.8 + 53.1, 67.6 + 57.0, 72.8 + 63.9;
-  // 64 x 1 rows of 2 heads: 3.3 + 2.3, 4.7 + 2.5.
+  // Heads a warp: up to three, where that leaves twenty warps for every SM (about as many as run at once).  Written +
+  // read, us, for 1, 2, 3, 4, 8 heads a warp (before the lanes shared the parameters): 96 x 50 rows of 16 heads: 20.6 +
+  // 10.1, 18.2 + 8.2, 17.4 + 7.7, 18.0 + 8.9, 18.6 + 8.6; 8 x 3001-4099 rows of 8 heads, 128 channels, fp32: 71.6 + 50.2,
+  // 65.6 + 54.9, 63.8 + 53.1, 67.6 + 57.0, 72.8 + 63.9; 64 x 1 rows of 2 heads, 1 and 2: 3.3 + 2.3, 4.7 + 2.5.
   const long long warps = 2 * items * c.kv_heads;
   const int heads = static_cast<int>(std::max<long long>(1, std::min<long long>(3, warps / (20 * num_sms()))));
   const dim3 grid(static_cast<unsigned>((items + WARPS / 2 - 1) / (WARPS / 2)), (c.kv_heads + heads - 1) / heads);

@@ -211,6 +211,29 @@ def test_write_special_values():
         assert np.array_equal(got.cpu().numpy(), want, equal_nan=True)
 
 
+@pytest.mark.parametrize("dim,group", [(64, 64), (64, 32), (128, 64), (128, 32)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_write_16_bit_patterns(dim, group, dtype):
+    """Every value of the type, in groups of neighbours and in mixed ones; zeros of both signs; single NaN and infinities."""
+    rng = np.random.default_rng(dim + group)
+    bits = np.arange(65536, dtype=np.uint16)
+    mixed = rng.permutation(bits)
+    small = rng.integers(0, 2, 65536).astype(np.uint16) << 15  # +0 and -0
+    usual = (rng.integers(0, 4096, 65536) + (0x3F00 if dtype == "bf16" else 0x3800) * 1).astype(np.uint16)
+    odd = usual.copy()
+    odd[::1009] = rng.choice(np.uint16([0x7FC0, 0x7F80, 0xFF80] if dtype == "bf16" else [0x7E01, 0x7C00, 0xFC00]), len(odd[::1009]))
+    x = torch.from_numpy(np.concatenate([bits, mixed, small, odd]).view(np.int16)).view(TORCH[dtype]).view(-1, 1, dim)
+    n = len(x)
+    c = Cache(n_pages=n // 16, n_seq=1, max_pages=n // 16, heads=1, dim=dim, group=group)
+    d = x.cuda()
+    e = torch.flip(x, [0]).contiguous().cuda()
+    r = c.batch([n], start=c.grow([0], [n]))
+    c.write(d, e, r, dtype)
+    for got, y in zip(c.read(r, n), (d, e)):
+        want = ko.quantise(y.float().cpu().numpy(), group)
+        assert np.array_equal(got.cpu().numpy(), want, equal_nan=True)
+
+
 def test_write_many_random_bits():
     """Random fp32 values by the million: the codes are those of exact arithmetic (float64 division, whose ties are exact here)."""
     c = Cache(n_pages=300, n_seq=1, max_pages=300, heads=8, dim=128, group=64, page=16)
