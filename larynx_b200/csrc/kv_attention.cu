@@ -400,7 +400,8 @@ struct Part {
 // Joins the parts of KW key groups, and of the CTAs of the cluster, and writes
 // the rows.  A part is O [rows][DIM] and, per row, the maximum and the sum.
 template <typename T, int DIM, int KW, int ROWS, int THREADS>
-__device__ __forceinline__ void join(const Args& a, const Share& s, float* part_o, float* part_m, float* part_l) {
+__device__ __forceinline__ void join(const Args& a, const Share& s, float* part_o, float* part_m, float* part_l,
+                                     int thread) {
   constexpr int V = DIM / 4;
   auto local = [&](int row, int v) {
     Part p{make_float4(0, 0, 0, 0), part_m[row], 0.0f};
@@ -423,14 +424,14 @@ __device__ __forceinline__ void join(const Args& a, const Share& s, float* part_
           p.sum == 0.0f ? -INFINITY : (p.top + log2f(p.sum)) * 0.6931471805599453f;
   };
   if (a.split == 1) {
-    for (int x = threadIdx.x; x < s.n_rows * V; x += THREADS) write(x / V, x % V, local(x / V, x % V));
+    for (int x = thread; x < s.n_rows * V; x += THREADS) write(x / V, x % V, local(x / V, x % V));
     return;
   }
   float* cta_o = part_o + (KW > 1 ? KW * ROWS * DIM : 0);
   float* cta_m = part_m + (KW > 1 ? KW * ROWS : 0);
   float* cta_l = part_l + (KW > 1 ? KW * ROWS : 0);
   if (KW > 1) {
-    for (int x = threadIdx.x; x < s.n_rows * V; x += THREADS) {
+    for (int x = thread; x < s.n_rows * V; x += THREADS) {
       const int row = x / V, v = x % V;
       const Part p = local(row, v);
       reinterpret_cast<float4*>(cta_o + row * DIM)[v] = p.o;
@@ -442,7 +443,7 @@ __device__ __forceinline__ void join(const Args& a, const Share& s, float* part_
   }
   auto cluster = cg::this_cluster();
   cluster.sync();
-  for (int x = threadIdx.x + s.rank * THREADS; x < s.n_rows * V; x += a.split * THREADS) {
+  for (int x = thread + s.rank * THREADS; x < s.n_rows * V; x += a.split * THREADS) {
     const int row = x / V, v = x % V;
     Part p{make_float4(0, 0, 0, 0), -INFINITY, 0.0f};
     for (int k = 0; k < a.split; ++k) p.top = fmaxf(p.top, *cluster.map_shared_rank(cta_m + row, k));
@@ -827,7 +828,7 @@ __global__ void __launch_bounds__(32 * KW, KW > 4 ? 1 : (DIM == 64 ? 16 : 12) / 
       }
     }
   __syncthreads();
-  join<T, DIM, KW, S::ROWS, S::THREADS>(a, s, part_o, part_m, part_l);
+  join<T, DIM, KW, S::ROWS, S::THREADS>(a, s, part_o, part_m, part_l, threadIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -1225,7 +1226,7 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
     }
   if (a.split == 1) return;
   __syncthreads();
-  join<T, DIM, 1, S::ROWS, S::THREADS>(a, s, part_o, part_m, part_l);
+  join<T, DIM, 1, S::ROWS, S::THREADS>(a, s, part_o, part_m, part_l, threadIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -1268,6 +1269,8 @@ struct TileShape {
   static constexpr int LAUNCH_REGS = 128, UNPACK_REGS = 64, SOFTMAX_REGS = 192;
   static_assert(UNPACK_REGS + SOFTMAX_REGS <= 2 * LAUNCH_REGS, "register split");
   static_assert(O_COL + DIM <= COLS, "tensor memory");
+  // the parts of a split, in the place of the unpacked keys: O [row][DIM], maxima, sums
+  static constexpr int PART = TILE_ROWS * (DIM + 2) * 4;
   // shared memory
   static constexpr int Q_BYTES = H * TILE_ROWS * 128;
   static constexpr int K_BYTES = H * KEYS * 128;
@@ -1275,6 +1278,7 @@ struct TileShape {
   static constexpr int PAR = 4 * G * KEYS * 4;  // ks, km, vs, vm
   static constexpr int SLOT = K_BYTES + V_BYTES;
   static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * (SLOT + PAR) + 512;
+  static_assert(PART <= SLOTS * SLOT, "parts of a split");
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -1352,8 +1356,9 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
   Share s;
   bool any;
   {
-    const int block = static_cast<int>(blockIdx.x), back = a.items.over(block);
-    const int x = block - back * static_cast<int>(a.items.d), entry = a.heads.over(x);
+    const int item = a.split_by.over(static_cast<int>(blockIdx.x)), back = a.items.over(item);
+    const int x = item - back * static_cast<int>(a.items.d), entry = a.heads.over(x);
+    s.rank = static_cast<int>(blockIdx.x) - item * a.split;
     any = s.take_at(a, entry, x - entry * a.c.kv_heads, static_cast<int>(a.tiles.d) - 1 - back, TILE_ROWS);
   }
   int lo_cta = 0, hi_cta = 0, x_;
@@ -1361,11 +1366,18 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
     s.range(a, 0, lo_cta, x_);
     s.range(a, TILE_ROWS, x_, hi_cta);
   }
-  const int tile0 = lo_cta / S::KEYS;
-  const int n_tiles = any && hi_cta > lo_cta ? (hi_cta + S::KEYS - 1) / S::KEYS - tile0 : 0;
+  // this CTA's units of the cluster's
+  int tile0 = lo_cta / S::KEYS, n_tiles = 0;
+  if (hi_cta > lo_cta) {
+    const int count = (hi_cta + S::KEYS - 1) / S::KEYS - tile0, from = a.split_by.over(count * s.rank);
+    n_tiles = a.split_by.over(count * (s.rank + 1)) - from;
+    tile0 += from;
+  }
   auto wait = [&](uint64_t* bar, int use) {  // for the use-th completion of a barrier
     return mbar_wait(bar, static_cast<uint32_t>(use & 1), nullptr, abort_flag, 0);
   };
+
+  auto read_out = [] { asm volatile("bar.sync 1, 160;" ::: "memory"); };  // the softmax warps and warp 0
 
   // issue, by one thread: the product O += P V of unit t
   constexpr int PV_N = G == 1 ? DIM : GROUP;
@@ -1492,6 +1504,18 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[slot]);
       }
+    }
+    if (a.split > 1) {
+      __syncwarp();
+      if (warp == 0) {
+        // Tensor memory is given back before the waiting for the other CTAs: held meanwhile, two clusters (of this kernel
+        // or another) could wait for each other's.
+        read_out();
+        tc_fence_after();
+        tmem_dealloc(tmem, S::COLS);
+      }
+      cg::this_cluster().sync();  // with those of the joining
+      cg::this_cluster().sync();
     }
   } else {
     // ---- softmax: a thread a row
@@ -1720,9 +1744,11 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
       if (lane == 0) mbar_arrive(&p_full[t & 1]);
     }
     if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, wait(&empty[(n_tiles - 1) % S::SLOTS], (n_tiles - 1) / S::SLOTS));
+    float* part_o = reinterpret_cast<float*>(slots);  // (the last product is done, and with it every use of the slots)
+    float *part_m = part_o + TILE_ROWS * DIM, *part_l = part_m + TILE_ROWS;
     if (ok && live) {
       tc_fence_after();
-      const float sum = l.x + l.y, f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float sum = l.x + l.y, f = a.split > 1 ? pow2(-f_exp) : sum == 0.0f ? 0.0f : 1.0f / sum;
       const int r = s.row0 + row, q_row = a.per.over(r);
       const int64_t h = s.head_of(a, r, q_row);
       T* out = static_cast<T*>(a.out) + (s.e.row0 + q_row) * a.o_row + h * a.o_head;
@@ -1737,7 +1763,17 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
         }
         const float2 zg = G == 1 ? z[0] : z[32 * c / GROUP % G];
         const float low = zg.x + zg.y;
-        if (row < s.n_rows) {
+        if (a.split > 1) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // channels 4 i .. 4 i + 3
+            float4 e;
+            e.x = fmaf(y[i], 16777216.0f, low) * f;
+            e.y = fmaf(y[8 + i], 1048576.0f, low) * f;
+            e.z = fmaf(y[16 + i], 16777216.0f, low) * f;
+            e.w = fmaf(y[24 + i], 1048576.0f, low) * f;
+            reinterpret_cast<float4*>(part_o + row * DIM + 32 * c)[i] = e;
+          }
+        } else if (row < s.n_rows) {
           __align__(16) T e[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {  // column 8 i + n is channel 4 n + i, times 16 for odd i
@@ -1754,16 +1790,26 @@ __global__ void __launch_bounds__(256, TileShape<DIM, GROUP>::CTAS) k_kv_tile(co
           }
         }
       }
-      if (a.lse && row < s.n_rows)
+      if (a.split > 1) {
+        part_m[row] = limit - RAISE;
+        part_l[row] = sum * f;
+      } else if (a.lse && row < s.n_rows) {
         a.lse[static_cast<int64_t>(s.e.row0 + q_row) * a.q_heads + h] =
             sum == 0.0f ? -INFINITY : (limit - RAISE - f_exp + log2f(sum)) * 0.6931471805599453f;
+      }
+    }
+    if (a.split > 1) {
+      tc_fence_before();
+      __syncwarp();
+      read_out();
+      join<T, DIM, 1, TILE_ROWS, 128>(a, s, part_o, part_m, part_l, static_cast<int>(threadIdx.x) - 128);
     }
   }
 
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag) flag(a.c, LX_KV_STUCK);
-  if (warp == 0) {
+  if (warp == 0 && !(any && a.split > 1)) {
     tc_fence_after();
     tmem_dealloc(tmem, S::COLS);
   }
@@ -1815,7 +1861,7 @@ void set_up(K kernel, Launch& l, int threads, int smem, cudaLaunchConfig_t& cfg,
 // 119 for clusters of 1 to 4 (larger clusters fill the GPU less evenly: a thirtieth each).
 template <typename K>
 bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_rows, int groups, int units,
-           double whole, double joined, cudaStream_t s) {
+           double whole, double joined, double crowded, cudaStream_t s) {
   Launch& l = launches[a.c.device & 63];
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
@@ -1829,7 +1875,8 @@ bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_
   for (int k = 1; k <= most; ++k) {
     if (l.active[k] == 0) continue;
     const double rounds = static_cast<double>((items + l.active[k] - 1) / l.active[k]);
-    const double cost = rounds * ((k > 1 ? joined : whole) + (units + groups * k - 1) / (groups * k)) * (1 + (k - 1) / 30.0);
+    const double cost = rounds * ((k > 1 ? joined : whole) + (units + groups * k - 1) / (groups * k)) *
+                        (1 + (k - 1) / 30.0) * (items * k > num_sms() ? crowded : 1.0);
     if (k == 1 || cost < best) {
       best = cost;
       split = k;
@@ -1855,35 +1902,27 @@ template <typename T, int DIM, int GROUP, int NT, int KW>
 bool few(Args& a, int units, cudaStream_t s) {
   using S = FewShape<DIM, GROUP, NT, KW>;
   static Launch launches[64];
-  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, 6.0, 7.0, s);
+  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, 6.0, 7.0, 1.0, s);
 }
 template <typename T, int DIM, int GROUP, int MT, int MW>
 bool many(Args& a, int units, cudaStream_t s) {
   using S = ManyShape<DIM, GROUP, MT, MW>;
   static Launch launches[64];
-  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 1, units, 5.0, 15.0, s);
+  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 1, units, 5.0, 15.0, 1.0, s);
 }
 
 template <typename T, int DIM, int GROUP>
-bool tile(Args& a, cudaStream_t s) {
+bool tile(Args& a, int max_len, cudaStream_t s) {
   using S = TileShape<DIM, GROUP>;
-  static std::atomic<bool> ready[64];
+  static Launch launches[64];
   auto kernel = k_kv_tile<T, DIM, GROUP>;
-  std::atomic<bool>& done = ready[a.c.device & 63];
-  if (!done) {
+  if (!launches[a.c.device & 63].ready) {
     // setmaxnreg.inc waits for registers that the block was launched with: no launch unless they cover the split
     cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || (S::SPLIT && fa.numRegs < S::LAUNCH_REGS) ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess)
-      return false;
-    done = true;
+    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || (S::SPLIT && fa.numRegs < S::LAUNCH_REGS)) return false;
   }
-  const long long tiles = (static_cast<long long>(a.r.max_rows) * a.per.d + TILE_ROWS - 1) / TILE_ROWS;
-  const long long ctas = tiles * a.r.n * a.c.kv_heads;
-  if (ctas > 0x7fffffff) return false;
-  a.tiles = Divisor(static_cast<uint32_t>(tiles));
-  a.split = 1;
-  return launch(kernel, dim3(static_cast<unsigned>(ctas)), dim3(S::THREADS), S::SMEM, s, a);
+  return start(kernel, a, launches, S::THREADS, S::SMEM, TILE_ROWS, 1, (max_len + S::KEYS - 1) / S::KEYS, 2.5, 3.5,
+               S::CTAS == 2 ? 1.3 : 1.0, s);
 }
 
 template <typename T, int DIM, int GROUP>
@@ -1901,10 +1940,9 @@ bool go(Args& a, int max_len, cudaStream_t s) {
     return wide ? few<T, DIM, GROUP, 2, 8>(a, units, s) : few<T, DIM, GROUP, 2, 4>(a, units, s);
   }
   // Tiles of 128 rows win above 64 rows (64 x 8 items over 1000 keys, us: 64 rows 60 against 61, 96 rows 64 against
-  // 105, 128 rows 68 against 106), if there is one for every SM: they do not split the keys (8 tiles over 4000 keys: 73
-  // against 22).  Sums for four groups do not fit the tensor memory.
-  if (DIM / GROUP <= 2 && rows > 64 && items * ((rows + TILE_ROWS - 1) / TILE_ROWS) >= num_sms())
-    return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, s);
+  // 105, 128 rows 68 against 106).  Sums for four groups do not fit the tensor memory.
+  if (DIM / GROUP <= 2 && rows > 64)
+    return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, max_len, s);
   return rows <= 32 ? many<T, DIM, GROUP, 1, 2>(a, units, s) : many<T, DIM, GROUP, 1, 4>(a, units, s);
 }
 

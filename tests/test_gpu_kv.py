@@ -450,6 +450,35 @@ def test_attention_more_items_than_fit(dim, group, heads, per, count):
             at += n
 
 
+@pytest.mark.parametrize("dim,group,heads,per,lengths,counts,chunk,left", [
+    (64, 64, 1, 1, [3001], [100], 1, -1),           # sixteen CTAs a tile
+    (64, 32, 2, 3, [2100, 40, 0], [90, 30, 50], 0, -1),  # units of 64 keys; entries that do not fill a unit, or have none
+    (128, 64, 2, 4, [1700, 300], [70, 33], 1, -1),
+    (64, 64, 3, 2, [900, 1200], [301, 65], 50, 100),  # most CTAs of a tile see nothing of some rows
+    (128, 64, 1, 8, [130], [130], 1, -1),           # fewer units than CTAs
+    (64, 64, 2, 1, [70, 20], [90, 66], 1, -1),      # rows before the sequence
+])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attention_few_tiles(dim, group, heads, per, lengths, counts, chunk, left, dtype):
+    """More than 64 rows an entry but few entries: the keys of a tile are split over CTAs."""
+    c = Cache(n_pages=sum(-(-n // 16) for n in lengths) + 1, n_seq=len(lengths), max_pages=200, heads=heads, dim=dim, group=group)
+    held = c.fill(lengths, seed=len(lengths) + dim)
+    g = torch.Generator().manual_seed(dim + per)
+    q = torch.randn(sum(counts) + 2, heads * per, dim, generator=g).to(TORCH[dtype])
+    out, lse = c.attend(q.cuda(), c.batch(counts), dtype, scale=dim ** -0.5, chunk=chunk, left=left)
+    torch.cuda.synchronize()
+    assert c.c.status() == 0
+    assert (out[-2:] == 3).all() and (lse[-2:] == 3).all()
+    at = 0
+    for (k, v, st), n in zip(held, counts):
+        pos = [len(k) - n + t for t in range(n)]
+        want = ko.attention(q[at:at + n].double().numpy(), k, v, st, pos, dim ** -0.5, chunk, left)
+        check(out[at:at + n], lse[at:at + n], want, dtype)
+        at += n
+    again, _ = c.attend(q.cuda(), c.batch(counts), dtype, scale=dim ** -0.5, chunk=chunk, left=left)
+    assert torch.equal(out, again)
+
+
 @pytest.mark.parametrize("length", [1, 15, 16, 255, 1025, 4099])
 @pytest.mark.parametrize("dim,per", [(64, 1), (128, 4)])
 def test_attention_long(length, dim, per):
