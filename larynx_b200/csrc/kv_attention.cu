@@ -24,12 +24,12 @@
 // Three forms, by the rows (query rows x query heads of one kv head) of an entry:
 //   k_kv_few   up to 16: every warp has all rows, the warps split the keys;
 //   k_kv_many  above:    warps of 16 rows share the keys that one of them brings;
-//   k_kv_tile  above 64: tiles of 128 rows on tcgen05, where there are tiles for every SM.
+//   k_kv_tile  above 64: tiles of 128 rows on tcgen05, unless there are few over few keys.
 // (mma.sync reaches 550 TFLOP/s here, a third of the tensor cores; up to 16 rows
-// the bytes and the unpacking bound, not the products.)  In the first two a cluster of
+// the bytes and the unpacking bound, not the products.)  A cluster of
 // CTAs splits the keys of long sequences, joined through shared memory in a fixed
 // order: no workspace in global memory, so calls may overlap, and the same call
-// gives the same bits.  Their bytes come through rings of bulk copies, two blocks a stage.
+// gives the same bits.  The bytes of the first two come through rings of bulk copies, two blocks a stage.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -1243,8 +1243,8 @@ __global__ void __launch_bounds__(32 * MW, MT * DIM == 64 ? 16 / MW : 8 / MW) k_
 // also needs no unpacking, against eight rows and unpacking in every warp in the forms above.
 //   Bound: the softmax (a row of 128 scores is read, raised, exponentiated and packed
 // by one thread) and the unpacking beside it, with two CTAs an SM taking turns: four
-// entries of 701-1500 rows, 16 heads of 64 channels: 86 us, against 14 for the
-// products; with k_kv_many 203.
+// entries of 701-1500 rows, 16 heads of 64 channels: 85 us, against 14 for the
+// products; with k_kv_many 203.  Few tiles split their keys over a cluster (`Cost`).
 //   V's tile holds the channels of 32 in the order 8 i + n for channel 4 n + i,
 // which is how the unpacking warps write it without bank conflicts; the rows
 // are put in order when they are written out.
@@ -1854,14 +1854,23 @@ void set_up(K kernel, Launch& l, int threads, int smem, cudaLaunchConfig_t& cfg,
   l.ready.store(l.active[1] > 0, std::memory_order_release);
 }
 
-// Launches `items` (tiles of rows x kv heads) with the keys of each split over a cluster of the size that
-// costs least: as many rounds of the GPU as it takes, of a fixed part and the units that a key group (`groups` a CTA)
-// then has.  The fixed part, in units: `whole` for a CTA of its own, `joined` for one of a cluster.  Few rows, 128
-// channels, 512 items, us a call: 32 keys 9 in two rounds, then 1.1 a unit a round; over 4099-8191 keys 116, 105, 114,
-// 119 for clusters of 1 to 4 (larger clusters fill the GPU less evenly: a thirtieth each).
+// What a block costs, in units of keys: its fixed part, for a CTA of its own and for one of a cluster, and by how much
+// two on an SM slow each other down; and the cluster sizes to choose from.  Measured, us a call:
+//  * k_kv_few, 128 channels, 512 items: 32 keys 9 in two rounds, then 1.1 a unit a round; over 4099-8191 keys 116, 105,
+//    114, 119 for clusters of 1 to 4 (larger clusters fill the GPU less evenly: a thirtieth each).
+//  * k_kv_tile, 64 channels, over 4000 keys, clusters of 1, 2, 4, 8, 16: 6 tiles 70, 45, 27, 18, 14; 32 tiles 71, 46,
+//    27, 25, 50; 64 tiles 71, 46, 37, 48, 87; 128 tiles 72, 67, 72, 93, 167; over 600 keys, 64 tiles: 17, 20, 19, 32, 73.
+//    (Of 3, 5, 6: 64 tiles 48, 58, 56.)
+struct Cost {
+  double whole, joined, crowded;
+  bool powers;  // clusters of 1, 2, 4, 8, 16 only
+};
+
+// Launches `items` (tiles of rows x kv heads) with the keys of each split over a cluster of the size that costs least: as
+// many rounds of the GPU as it takes, of the fixed part and the units that a key group (`groups` a CTA) then has.
 template <typename K>
 bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_rows, int groups, int units,
-           double whole, double joined, double crowded, cudaStream_t s) {
+           const Cost& c, cudaStream_t s) {
   Launch& l = launches[a.c.device & 63];
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
@@ -1873,10 +1882,10 @@ bool start(K kernel, Args& a, Launch* launches, int threads, int smem, int tile_
   int split = 1;
   double best = 0.0;
   for (int k = 1; k <= most; ++k) {
-    if (l.active[k] == 0) continue;
+    if (l.active[k] == 0 || (c.powers && (k & (k - 1)) != 0)) continue;
     const double rounds = static_cast<double>((items + l.active[k] - 1) / l.active[k]);
-    const double cost = rounds * ((k > 1 ? joined : whole) + (units + groups * k - 1) / (groups * k)) *
-                        (1 + (k - 1) / 30.0) * (items * k > num_sms() ? crowded : 1.0);
+    const double cost = rounds * ((k > 1 ? c.joined : c.whole) + (units + groups * k - 1) / (groups * k)) *
+                        (1 + (k - 1) / 30.0) * (items * k > num_sms() ? c.crowded : 1.0);
     if (k == 1 || cost < best) {
       best = cost;
       split = k;
@@ -1902,13 +1911,15 @@ template <typename T, int DIM, int GROUP, int NT, int KW>
 bool few(Args& a, int units, cudaStream_t s) {
   using S = FewShape<DIM, GROUP, NT, KW>;
   static Launch launches[64];
-  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units, 6.0, 7.0, 1.0, s);
+  return start(k_kv_few<T, DIM, GROUP, NT, KW>, a, launches, S::THREADS, S::SMEM, S::ROWS, KW, units,
+               Cost{6.0, 7.0, 1.0, false}, s);
 }
 template <typename T, int DIM, int GROUP, int MT, int MW>
 bool many(Args& a, int units, cudaStream_t s) {
   using S = ManyShape<DIM, GROUP, MT, MW>;
   static Launch launches[64];
-  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 1, units, 5.0, 15.0, 1.0, s);
+  return start(k_kv_many<T, DIM, GROUP, MT, MW>, a, launches, S::THREADS, S::SMEM, S::ROWS, 1, units,
+               Cost{5.0, 15.0, 1.0, false}, s);
 }
 
 template <typename T, int DIM, int GROUP>
@@ -1921,8 +1932,8 @@ bool tile(Args& a, int max_len, cudaStream_t s) {
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || (S::SPLIT && fa.numRegs < S::LAUNCH_REGS)) return false;
   }
-  return start(kernel, a, launches, S::THREADS, S::SMEM, TILE_ROWS, 1, (max_len + S::KEYS - 1) / S::KEYS, 2.5, 3.5,
-               S::CTAS == 2 ? 1.3 : 1.0, s);
+  return start(kernel, a, launches, S::THREADS, S::SMEM, TILE_ROWS, 1, (max_len + S::KEYS - 1) / S::KEYS,
+               Cost{3.0, 6.0, S::CTAS == 2 ? 1.4 : 1.0, true}, s);
 }
 
 template <typename T, int DIM, int GROUP>
@@ -1940,8 +1951,12 @@ bool go(Args& a, int max_len, cudaStream_t s) {
     return wide ? few<T, DIM, GROUP, 2, 8>(a, units, s) : few<T, DIM, GROUP, 2, 4>(a, units, s);
   }
   // Tiles of 128 rows win above 64 rows (64 x 8 items over 1000 keys, us: 64 rows 60 against 61, 96 rows 64 against
-  // 105, 128 rows 68 against 106).  Sums for four groups do not fit the tensor memory.
-  if (DIM / GROUP <= 2 && rows > 64)
+  // 105, 128 rows 68 against 106) unless there are few of them over few keys (64 channels: 6 tiles over 600 keys 17
+  // against 11, 32 over 600 17 against 15, 6 over 4000 14 against 19, 64 over 4000 46 against 60; 128 channels: 6 over 600
+  // 24 against 15, 32 over 1200 28 against 26, 64 over 600 25 against 28, 64 over 4000 74 against 111).
+  // Sums for four groups do not fit the tensor memory.
+  const long long tiles = items * ((rows + TILE_ROWS - 1) / TILE_ROWS);
+  if (DIM / GROUP <= 2 && rows > 64 && tiles * ((max_len + 127) / 128) >= num_sms() * (DIM / 64))
     return tile<T, DIM, DIM / GROUP <= 2 ? GROUP : 64>(a, max_len, s);
   return rows <= 32 ? many<T, DIM, GROUP, 1, 2>(a, units, s) : many<T, DIM, GROUP, 1, 4>(a, units, s);
 }
