@@ -127,7 +127,8 @@ int lx_kv_status(const lx_kv_cache* c, int32_t* bits, void* stream);
  * sequence is replaced by a copy first (all layers), so that lx_kv_write never
  * changes a fork.  Entry i is served if the pages needed by entries 0 .. i fit
  * the free ones; an entry that is not served gets start[i] = LX_KV_REFUSED (its rows are skipped by the
- * other calls) and leaves its sequence as it was. */
+ * other calls) and leaves its sequence as it was.  start must not overlap seqs
+ * or counts. */
 int lx_kv_extend(const lx_kv_cache* c, int32_t n, const int32_t* seqs, const int32_t* counts, int32_t* start,
                  void* stream);
 

@@ -106,6 +106,7 @@ inline bool cache_ok(const lx_kv_cache* c) {
 inline bool rows_ok(const lx_kv_rows* r) {
   if (!r || r->n <= 0 || r->total < 0 || r->max_rows < 0 || r->total > MAX_ROWS || r->max_rows > MAX_ROWS)
     return false;
+  if (!aligned(r->seqs, 4) || !aligned(r->row0, 4) || !aligned(r->start, 4)) return false;
   return r->row0 || static_cast<long long>(r->n) * r->max_rows == r->total;
 }
 

@@ -113,6 +113,15 @@ def test_rows_refused(bad):
     assert lib.lx_kv_attention(ref, 0, rows, 2, 0, P, 128, 64, P, 128, 64, None, 0.1, 1, -1, 0, None) == 1
 
 
+@pytest.mark.parametrize("bad", [dict(seqs=P + 2), dict(row0=P + 1), dict(start=P + 3)])
+def test_unaligned_rows_refused(bad):
+    lib, c, r = _lib(), _cache(), _rows(**bad)
+    ref, rows = ctypes.byref(c), ctypes.byref(r)
+    assert lib.lx_kv_write(ref, 0, rows, 0, P, 128, 64, P, 128, 64, None) == 1
+    assert lib.lx_kv_read(ref, 0, rows, 0, P, 128, 64, P, 128, 64, None) == 1
+    assert lib.lx_kv_attention(ref, 0, rows, 2, 0, P, 128, 64, P, 128, 64, None, 0.1, 1, -1, 0, None) == 1
+
+
 def test_row_calls_refused():
     lib, c, r = _lib(), _cache(), _rows()
     ref, rows = ctypes.byref(c), ctypes.byref(r)
