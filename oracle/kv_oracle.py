@@ -1,6 +1,6 @@
 """CPU oracle for the paged 4-bit key/value cache (TEST INFRASTRUCTURE ONLY).
 
-The parity checker for the operators of ``include/larynx_kv.h``: quantising in
+The oracle for the operators of ``include/larynx_kv.h``: quantising in
 exact rational arithmetic where it matters, attention in float64, the page
 operations as plain Python over lists.  No reference counterpart: the reference
 keeps no keys or values between calls.  Only ``tests/`` may import this module.
