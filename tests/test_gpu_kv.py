@@ -682,6 +682,29 @@ class Both:
             assert data[:, p].tobytes() == self.o.data[p], p
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_overlapping_attention_calls(dim):
+    """Calls of the three forms, keys split and not, on four streams at once: the bits of each alone."""
+    c = Cache(n_pages=700, n_seq=6, max_pages=130, heads=2, dim=dim, group=64)
+    c.fill([2000, 1500, 33, 640, 1, 900], seed=dim)
+    calls = []
+    for n, per in ((1, 4), (20, 2), (100, 1), (90, 8)):
+        q = torch.randn(6 * n, 2 * per, dim, generator=torch.Generator().manual_seed(n)).bfloat16().cuda()
+        rows = c.batch([n] * 6)
+        alone, lse = c.attend(q, rows, "bf16", chunk=1)
+        torch.cuda.synchronize()
+        calls.append((q, rows, alone, lse, torch.cuda.Stream()))
+    outs = [[torch.zeros_like(q) for _ in range(12)] for q, *_ in calls]
+    torch.cuda.synchronize()
+    for k in range(12):
+        for x, (q, rows, _, _, s) in enumerate(calls):
+            c.c.attention(0, rows, q.shape[1], "bf16", q.data_ptr(), outs[x][k].data_ptr(), chunk=1, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert c.c.status() == 0
+    for x, (_, _, alone, _, _) in enumerate(calls):
+        assert all(torch.equal(o, alone) for o in outs[x])
+
+
 FIRST = """
 import sys, threading
 sys.path.insert(0, sys.argv[1]); sys.path.insert(0, sys.argv[1] + "/tests")
